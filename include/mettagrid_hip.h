@@ -310,6 +310,85 @@ int mg_compute_advantage(const float* values, const float* rewards, const float*
                          float* advantages, float gamma, float lambda, float rho_clip, float c_clip, int num_rows,
                          int horizon, void* stream);
 
+/* ---- recurrent core and action head of a policy ------------------------------------------------------------------
+ * Element types of the tensors below (all device memory, columns adjacent, strides in elements). */
+#define MG_F32 0
+#define MG_BF16 1
+#define MG_F16 2
+
+/* Gated linear recurrence over [rows][steps][width], per row and column, with a = sigmoid(gate):
+ *   h[t] = a[t] * (resets[t] ? 0 : h[t-1]) + (1 - a[t]) * x[t],  h[-1] = state
+ * x and gate are of `type` and may be strided (halves of one projection, time-major views); state f32 [rows][width] and
+ * resets u8 [rows][steps] are contiguous and may be NULL (zeros / none). */
+typedef struct mg_recurrence {
+  const void* x;
+  const void* gate;
+  const float* state;
+  const uint8_t* resets;
+  int64_t rows, steps, width;      /* rows * width up to 2^31 */
+  int64_t x_row, x_step, gate_row, gate_step;
+  int32_t type;
+} mg_recurrence;
+
+/* The states kept for the backward pass: the one entering every 16th step after step 0. */
+#define MG_RECURRENCE_MARK_STEPS 16
+
+/* h [rows][steps][width] of `type` (NULL: only the last state is wanted), last f32 [rows][width], marks f32
+ * [rows][(steps - 1) / 16][width] or NULL (no backward pass will follow, or h is f32 and serves as marks).  `last` may
+ * be `state` itself.  Nothing is written where rows, steps or width is 0. */
+int mg_gated_recurrence(const mg_recurrence* r, void* h, float* last, float* marks, void* stream);
+
+/* Gradients of the above: dh (of `type`, strided) and dlast (f32 [rows][width]) in, each may be NULL (zeros); dx and
+ * dgate (of `type`, strided), dstate (f32 [rows][width], may be NULL) out. */
+typedef struct mg_recurrence_gradients {
+  const void* dh;
+  const float* dlast;
+  void* dx;
+  void* dgate;
+  float* dstate;
+  int64_t dh_row, dh_step, dx_row, dx_step, dgate_row, dgate_step;
+} mg_recurrence_gradients;
+
+/* The state entering step 16 k (k >= 1) of a row is read at marks[row * marks_row + (k - 1) * marks_stride + column]:
+ * the marks of the forward pass, or an f32 h at 15 * width. */
+int mg_gated_recurrence_backward(const mg_recurrence* r, const float* marks, int64_t marks_row, int64_t marks_stride,
+                                 const mg_recurrence_gradients* d, void* stream);
+
+/* Logits [rows][width] of `type` and their controls.  Per row, with c = occurrences of v in its history:
+ *   l1 = c > 0 ? (l > 0 ? l / repetition : l * repetition) : l;   l2 = l1 - frequency * c - presence * (c > 0)
+ *   adjusted = allowed ? (l2 + bias) / temperature : -infinity
+ * allowed: one byte per token (MG_ALLOWED_BOOL) or bit v % 32 of i32 word v / 32 (MG_ALLOWED_BITS); bias f32; history
+ * i32, entries outside [0, width) count for nothing.  A row stride of 0 shares a control among all rows; NULL: none. */
+#define MG_ALLOWED_BOOL 1
+#define MG_ALLOWED_BITS 2
+typedef struct mg_logits {
+  const void* logits;
+  const float* bias;
+  const void* allowed;
+  const int32_t* history;
+  int64_t rows;
+  int64_t logits_row, bias_row, allowed_row, history_row;
+  double temperature, repetition, presence, frequency;
+  int32_t width, history_len, allowed_kind, type;
+} mg_logits;
+
+/* Adjusted logits, contiguous and of `type`; backward: dlogits = dout * d adjusted / d logits (0 where masked). */
+int mg_adjust_logits(const mg_logits* a, void* out, void* stream);
+int mg_adjust_logits_backward(const mg_logits* a, const void* dout, void* dlogits, void* stream);
+
+/* One action per row from the adjusted logits: the first v whose running sum of exp exceeds u * (the whole sum), as
+ * 64-bit arithmetic finds it; without uniforms (NULL) the first of the largest.  log_prob and entropy f32 [rows].
+ * A row without an allowed token: -1, 0, 0; with NaN or +infinity at an allowed token: -1, NaN, NaN. */
+int mg_sample_actions(const mg_logits* a, const float* uniforms, int32_t* actions, float* log_prob, float* entropy,
+                      void* stream);
+
+/* log_prob and entropy of given actions; an action that is masked or outside [0, width) has -infinity and passes no
+ * gradient.  stats f64 [rows][2] (may be NULL) is what the backward pass wants back. */
+int mg_evaluate_actions(const mg_logits* a, const int32_t* actions, float* log_prob, float* entropy, double* stats,
+                        void* stream);
+int mg_evaluate_actions_backward(const mg_logits* a, const int32_t* actions, const float* entropy, const double* stats,
+                                 const float* dlog_prob, const float* dentropy, void* dlogits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

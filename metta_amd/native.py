@@ -36,6 +36,64 @@ class MgBuffers(ct.Structure):
     ]
 
 
+class MgRecurrence(ct.Structure):
+    _fields_ = [
+        ("x", ct.c_void_p),
+        ("gate", ct.c_void_p),
+        ("state", ct.c_void_p),
+        ("resets", ct.c_void_p),
+        ("rows", ct.c_int64),
+        ("steps", ct.c_int64),
+        ("width", ct.c_int64),
+        ("x_row", ct.c_int64),
+        ("x_step", ct.c_int64),
+        ("gate_row", ct.c_int64),
+        ("gate_step", ct.c_int64),
+        ("type", ct.c_int32),
+    ]
+
+
+class MgRecurrenceGradients(ct.Structure):
+    _fields_ = [
+        ("dh", ct.c_void_p),
+        ("dlast", ct.c_void_p),
+        ("dx", ct.c_void_p),
+        ("dgate", ct.c_void_p),
+        ("dstate", ct.c_void_p),
+        ("dh_row", ct.c_int64),
+        ("dh_step", ct.c_int64),
+        ("dx_row", ct.c_int64),
+        ("dx_step", ct.c_int64),
+        ("dgate_row", ct.c_int64),
+        ("dgate_step", ct.c_int64),
+    ]
+
+
+class MgLogits(ct.Structure):
+    _fields_ = [
+        ("logits", ct.c_void_p),
+        ("bias", ct.c_void_p),
+        ("allowed", ct.c_void_p),
+        ("history", ct.c_void_p),
+        ("rows", ct.c_int64),
+        ("logits_row", ct.c_int64),
+        ("bias_row", ct.c_int64),
+        ("allowed_row", ct.c_int64),
+        ("history_row", ct.c_int64),
+        ("temperature", ct.c_double),
+        ("repetition", ct.c_double),
+        ("presence", ct.c_double),
+        ("frequency", ct.c_double),
+        ("width", ct.c_int32),
+        ("history_len", ct.c_int32),
+        ("allowed_kind", ct.c_int32),
+        ("type", ct.c_int32),
+    ]
+
+
+MARK_STEPS = 16  # MG_RECURRENCE_MARK_STEPS
+ALLOWED_BOOL, ALLOWED_BITS = 1, 2  # MG_ALLOWED_*
+
 # name -> (restype, argtypes); every symbol include/mettagrid_hip.h declares
 _vp, _i32p, _u32p, _u8p, _f32p, _f64p = (
     ct.c_void_p,
@@ -102,6 +160,16 @@ SYMBOLS = {
         ct.c_int,
         [_vp, _vp, _vp, _vp, _vp, ct.c_float, ct.c_float, ct.c_float, ct.c_float, ct.c_int, ct.c_int, _vp],
     ),
+    "mg_gated_recurrence": (ct.c_int, [ct.POINTER(MgRecurrence), _vp, _vp, _vp, _vp]),
+    "mg_gated_recurrence_backward": (
+        ct.c_int,
+        [ct.POINTER(MgRecurrence), _vp, ct.c_int64, ct.c_int64, ct.POINTER(MgRecurrenceGradients), _vp],
+    ),
+    "mg_adjust_logits": (ct.c_int, [ct.POINTER(MgLogits), _vp, _vp]),
+    "mg_adjust_logits_backward": (ct.c_int, [ct.POINTER(MgLogits), _vp, _vp, _vp]),
+    "mg_sample_actions": (ct.c_int, [ct.POINTER(MgLogits), _vp, _vp, _vp, _vp, _vp]),
+    "mg_evaluate_actions": (ct.c_int, [ct.POINTER(MgLogits), _vp, _vp, _vp, _vp, _vp]),
+    "mg_evaluate_actions_backward": (ct.c_int, [ct.POINTER(MgLogits), _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
 }
 
 
