@@ -327,15 +327,20 @@ typedef struct mg_recurrence {
   const uint8_t* resets;
   int64_t rows, steps, width;      /* rows * width up to 2^31 */
   int64_t x_row, x_step, gate_row, gate_step;
+  void* workspace;                 /* mg_gated_recurrence_workspace bytes of device memory, for this call alone */
+  int64_t workspace_bytes;
   int32_t type;
 } mg_recurrence;
+
+/* Bytes of workspace that a call with this shape needs, forward or backward (0: none; few columns and many steps). */
+int64_t mg_gated_recurrence_workspace(const mg_recurrence* r);
 
 /* The states kept for the backward pass: the one entering every 16th step after step 0. */
 #define MG_RECURRENCE_MARK_STEPS 16
 
 /* h [rows][steps][width] of `type` (NULL: only the last state is wanted), last f32 [rows][width], marks f32
  * [rows][(steps - 1) / 16][width] or NULL (no backward pass will follow, or h is f32 and serves as marks).  `last` may
- * be `state` itself.  Nothing is written where rows, steps or width is 0. */
+ * be `state` itself where steps is 1.  Nothing is written where rows, steps or width is 0. */
 int mg_gated_recurrence(const mg_recurrence* r, void* h, float* last, float* marks, void* stream);
 
 /* Gradients of the above: dh (of `type`, strided) and dlast (f32 [rows][width]) in, each may be NULL (zeros); dx and

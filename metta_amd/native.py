@@ -49,6 +49,8 @@ class MgRecurrence(ct.Structure):
         ("x_step", ct.c_int64),
         ("gate_row", ct.c_int64),
         ("gate_step", ct.c_int64),
+        ("workspace", ct.c_void_p),
+        ("workspace_bytes", ct.c_int64),
         ("type", ct.c_int32),
     ]
 
@@ -160,6 +162,7 @@ SYMBOLS = {
         ct.c_int,
         [_vp, _vp, _vp, _vp, _vp, ct.c_float, ct.c_float, ct.c_float, ct.c_float, ct.c_int, ct.c_int, _vp],
     ),
+    "mg_gated_recurrence_workspace": (ct.c_int64, [ct.POINTER(MgRecurrence)]),
     "mg_gated_recurrence": (ct.c_int, [ct.POINTER(MgRecurrence), _vp, _vp, _vp, _vp]),
     "mg_gated_recurrence_backward": (
         ct.c_int,

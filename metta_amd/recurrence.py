@@ -78,8 +78,18 @@ def _args(x: Tensor, gate: Tensor, state: Optional[Tensor], resets: Optional[Ten
     one = x.dim() == 2  # a single step: [rows, width]
     return native.MgRecurrence(
         x.data_ptr(), gate.data_ptr(), None if state is None else state.data_ptr(), None if resets is None else resets.data_ptr(),
-        x.size(0), steps, x.size(-1), x.stride(0), 0 if one else x.stride(1), gate.stride(0), 0 if one else gate.stride(1), TYPES[x.dtype],
+        x.size(0), steps, x.size(-1), x.stride(0), 0 if one else x.stride(1), gate.stride(0), 0 if one else gate.stride(1), None, 0, TYPES[x.dtype],
     )  # fmt: skip
+
+
+def _workspace(args: native.MgRecurrence, device: torch.device) -> Optional[Tensor]:
+    """Memory of this call's own (torch's allocator keeps it for the stream, and for a captured graph), set in `args`."""
+    size = native.load().mg_gated_recurrence_workspace(ct.byref(args))
+    if not size:
+        return None
+    w = torch.empty(size, dtype=torch.uint8, device=device)
+    args.workspace, args.workspace_bytes = w.data_ptr(), size
+    return w
 
 
 class _GatedRecurrence(torch.autograd.Function):
@@ -95,8 +105,10 @@ class _GatedRecurrence(torch.autograd.Function):
         marks = None
         if x.dtype != torch.float32 and any(ctx.needs_input_grad):
             marks = torch.empty(rows, (steps - 1) // native.MARK_STEPS, width, dtype=torch.float32, device=x.device)
-        _launch("mg_gated_recurrence", x.device, ct.byref(_args(xs, gs, state, resets, steps)), h.data_ptr(), last.data_ptr(),
-                None if marks is None else marks.data_ptr())  # fmt: skip
+        args = _args(xs, gs, state, resets, steps)
+        w = _workspace(args, x.device)
+        _launch("mg_gated_recurrence", x.device, ct.byref(args), h.data_ptr(), last.data_ptr(), None if marks is None else marks.data_ptr())
+        del w
         # an f32 output holds the states itself, in shorter types they are kept apart
         ctx.save_for_backward(x, gate, state, resets, h if marks is None else marks)
         ctx.packed = packed
@@ -130,7 +142,10 @@ class _GatedRecurrence(torch.autograd.Function):
         )  # fmt: skip
         at = marks.data_ptr() + (4 * (native.MARK_STEPS - 1) * width if f32 else 0)
         strides = (steps * width, native.MARK_STEPS * width) if f32 else ((steps - 1) // native.MARK_STEPS * width, width)
-        _launch("mg_gated_recurrence_backward", x.device, ct.byref(_args(xs, gs, state, resets, steps)), at, *strides, ct.byref(grads))
+        args = _args(xs, gs, state, resets, steps)
+        w = _workspace(args, x.device)
+        _launch("mg_gated_recurrence_backward", x.device, ct.byref(args), at, *strides, ct.byref(grads))
+        del w
         return dx, dgate, dstate, None, None
 
 
