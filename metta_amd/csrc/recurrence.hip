@@ -75,15 +75,28 @@ struct RecGrads {
 template <typename T, int VEC>
 struct RecTile { rec_vec<T, VEC> v[REC_L]; };
 
-// n steps (uniform over the wave) from p on; the steps behind the n-th hold zeros
+// n steps (uniform over the wave) from p on; the steps behind the n-th are filled.  Candidates and gradients of 0 and gates
+// of +infinity leave state and gradient as they are, so that nothing but the stores has to know where time ends.
 template <typename T, int VEC>
-__device__ __forceinline__ void rec_load(RecTile<T, VEC>& x, const T* p, long step, int n) {
+__device__ __forceinline__ void rec_load(RecTile<T, VEC>& x, const T* p, long step, int n, float fill) {
   if (n >= REC_L) {
 #pragma unroll
-    for (int i = 0; i < REC_L; i++) x.v[i] = *(const rec_vec<T, VEC>*)(p + i * step);
+    for (int i = 0; i < REC_L; i++, p += step) x.v[i] = *(const rec_vec<T, VEC>*)p;
   } else {
 #pragma unroll
-    for (int i = 0; i < REC_L; i++) x.v[i] = i < n ? *(const rec_vec<T, VEC>*)(p + i * step) : rec_vec<T, VEC>(0);
+    for (int i = 0; i < REC_L; i++, p += step) x.v[i] = i < n ? *(const rec_vec<T, VEC>*)p : rec_vec<T, VEC>((T)fill);
+  }
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void rec_store(const RecTile<T, VEC>& x, T* p, long step, int n) {
+  if (n >= REC_L) {
+#pragma unroll
+    for (int i = 0; i < REC_L; i++, p += step) *(rec_vec<T, VEC>*)p = x.v[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < REC_L; i++, p += step)
+      if (i < n) *(rec_vec<T, VEC>*)p = x.v[i];
   }
 }
 
@@ -105,24 +118,25 @@ __device__ __forceinline__ unsigned rec_resets(const unsigned char* p, int n) {
   return bits;
 }
 
-template <typename T, int VEC>
-struct RecPlace {  // a thread's columns
+// A thread's columns.  The threads behind the last group do the last group's work once more (the same values to the same
+// places): how many steps there are is then the same for a whole wave, and known to it as a scalar.
+template <int VEC>
+struct RecPlace {
   unsigned row, col;
-  bool live;
   __device__ RecPlace(const RecArgs& a, unsigned group) {
-    live = group < a.groups;
+    group = min(group, a.groups - 1);
     const unsigned per_row = a.width / VEC;
-    row = live ? group / per_row : 0;
-    col = live ? (group - row * per_row) * VEC : 0;
+    row = group / per_row;
+    col = (group - row * per_row) * VEC;
   }
 };
+__device__ __forceinline__ int rec_wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 // ---- many columns: a thread walks through all of time, the next REC_L steps on their way while it computes ------------
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void mg_recurrence_kernel(RecArgs a, T* __restrict__ h, float* __restrict__ last,
                                                             float* __restrict__ marks) {
-  const RecPlace<T, VEC> at(a, blockIdx.x * 256 + threadIdx.x);
-  if (!at.live) return;
+  const RecPlace<VEC> at(a, blockIdx.x * 256 + threadIdx.x);
   const T* x = (const T*)a.x + at.row * a.x_row + at.col;
   const T* g = (const T*)a.gate + at.row * a.g_row + at.col;
   const unsigned char* rs = a.resets ? a.resets + at.row * a.steps : nullptr;
@@ -138,8 +152,8 @@ __global__ __launch_bounds__(256) void mg_recurrence_kernel(RecArgs a, T* __rest
   auto fetch = [&](int k, long t) {
     const int n = (int)min((long)REC_L, a.steps - t);
     if (n <= 0) return;
-    rec_load<T, VEC>(xt[k], x + t * a.x_step, a.x_step, n);
-    rec_load<T, VEC>(gt[k], g + t * a.g_step, a.g_step, n);
+    rec_load<T, VEC>(xt[k], x + t * a.x_step, a.x_step, n, 0.f);
+    rec_load<T, VEC>(gt[k], g + t * a.g_step, a.g_step, n, INFINITY);
     rt[k] = rec_resets(rs ? rs + t : nullptr, n);
   };
   auto walk = [&](int k, long t) {
@@ -151,26 +165,19 @@ __global__ __launch_bounds__(256) void mg_recurrence_kernel(RecArgs a, T* __rest
       for (int j = 0; j < VEC; j++) m[j] = s[j];
       *(rec_vec<float, VEC>*)(mark + (t / REC_L - 1) * a.width) = m;
     }
-    auto step = [&](int i) {
-      rec_vec<T, VEC> o;
+    RecTile<T, VEC> o;
+#pragma unroll
+    for (int i = 0; i < REC_L; i++) {
 #pragma unroll
       for (int j = 0; j < VEC; j++) {
         float ga, gw;
         rec_gate((float)gt[k].v[i][j], ga, gw);
         const float q = gw * (float)xt[k].v[i][j];
         s[j] = (rt[k] >> i) & 1 ? q : fmaf(ga, s[j], q);
-        o[j] = (T)s[j];
+        o.v[i][j] = (T)s[j];
       }
-      if (out) *(rec_vec<T, VEC>*)(out + (t + i) * a.width) = o;
-    };
-    if (n == REC_L) {
-#pragma unroll
-      for (int i = 0; i < REC_L; i++) step(i);
-    } else {
-#pragma unroll
-      for (int i = 0; i < REC_L; i++)
-        if (i < n) step(i);
     }
+    if (out) rec_store<T, VEC>(o, out + t * a.width, a.width, n);
   };
   fetch(0, 0);
   for (long t = 0; t < a.steps; t += 2 * REC_L) {
@@ -186,8 +193,8 @@ __global__ __launch_bounds__(256) void mg_recurrence_kernel(RecArgs a, T* __rest
 // one step, no marks: a flat pass over the columns
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void mg_recurrence_step_kernel(RecArgs a, T* __restrict__ h, float* last) {
-  const RecPlace<T, VEC> at(a, blockIdx.x * 256 + threadIdx.x);
-  if (!at.live) return;
+  if (blockIdx.x * 256 + threadIdx.x >= a.groups) return;  // (the state may be overwritten in place)
+  const RecPlace<VEC> at(a, blockIdx.x * 256 + threadIdx.x);
   const rec_vec<T, VEC> x = *(const rec_vec<T, VEC>*)((const T*)a.x + at.row * a.x_row + at.col);
   const rec_vec<T, VEC> g = *(const rec_vec<T, VEC>*)((const T*)a.gate + at.row * a.g_row + at.col);
   const long flat = (long)at.row * a.width + at.col;
@@ -208,8 +215,7 @@ __global__ __launch_bounds__(256) void mg_recurrence_step_kernel(RecArgs a, T* _
 
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void mg_recurrence_backward_kernel(RecArgs a, RecMarks m, RecGrads d) {
-  const RecPlace<T, VEC> at(a, blockIdx.x * 256 + threadIdx.x);
-  if (!at.live) return;
+  const RecPlace<VEC> at(a, blockIdx.x * 256 + threadIdx.x);
   const T* x = (const T*)a.x + at.row * a.x_row + at.col;
   const T* g = (const T*)a.gate + at.row * a.g_row + at.col;
   const T* dh = d.dh ? (const T*)d.dh + at.row * d.dh_row + at.col : nullptr;
@@ -225,9 +231,9 @@ __global__ __launch_bounds__(256) void mg_recurrence_backward_kernel(RecArgs a, 
     const long t0 = k * REC_L;
     const int n = (int)min((long)REC_L, a.steps - t0);
     RecTile<T, VEC> xt, gt, dt;
-    rec_load<T, VEC>(xt, x + t0 * a.x_step, a.x_step, n);
-    rec_load<T, VEC>(gt, g + t0 * a.g_step, a.g_step, n);
-    if (dh) rec_load<T, VEC>(dt, dh + t0 * d.dh_step, d.dh_step, n);
+    rec_load<T, VEC>(xt, x + t0 * a.x_step, a.x_step, n, 0.f);
+    rec_load<T, VEC>(gt, g + t0 * a.g_step, a.g_step, n, INFINITY);
+    if (dh) rec_load<T, VEC>(dt, dh + t0 * d.dh_step, d.dh_step, n, 0.f);
     const unsigned rt = rec_resets(rs ? rs + t0 : nullptr, n);
     float s[VEC];
 #pragma unroll
@@ -243,21 +249,19 @@ __global__ __launch_bounds__(256) void mg_recurrence_backward_kernel(RecArgs a, 
         s[j] = (rt >> i) & 1 ? q : fmaf(ga[i][j], s[j], q);
       }
     }
+    RecTile<T, VEC> ox, og;
 #pragma unroll
     for (int i = REC_L - 1; i >= 0; i--) {
-      if (i < n) {
-        rec_vec<T, VEC> ox, og;
 #pragma unroll
-        for (int j = 0; j < VEC; j++) {
-          const float dd = dh ? v[j] + (float)dt.v[i][j] : v[j];
-          ox[j] = (T)(gw[i][j] * dd);
-          og[j] = (T)(dd * (before[i][j] - (float)xt.v[i][j]) * (ga[i][j] * gw[i][j]));
-          v[j] = (rt >> i) & 1 ? 0.f : ga[i][j] * dd;
-        }
-        *(rec_vec<T, VEC>*)(dx + (t0 + i) * d.dx_step) = ox;
-        *(rec_vec<T, VEC>*)(dg + (t0 + i) * d.dg_step) = og;
+      for (int j = 0; j < VEC; j++) {
+        const float dd = dh ? v[j] + (float)dt.v[i][j] : v[j];
+        ox.v[i][j] = (T)(gw[i][j] * dd);
+        og.v[i][j] = (T)(dd * (before[i][j] - (float)xt.v[i][j]) * (ga[i][j] * gw[i][j]));
+        v[j] = (rt >> i) & 1 ? 0.f : ga[i][j] * dd;
       }
     }
+    rec_store<T, VEC>(ox, dx + t0 * d.dx_step, d.dx_step, n);
+    rec_store<T, VEC>(og, dg + t0 * d.dg_step, d.dg_step, n);
   }
   if (d.dstate) {
 #pragma unroll
@@ -282,20 +286,29 @@ struct RecExchange { float p[2][REC_W][VEC][64], q[2][REC_W][VEC][64]; };
 // the compositions of the blocks that come before this one in the order of the pass (step = 1: forwards in time;
 // -1: backwards), applied to s.  Wave w composes a share of them, then all waves compose the shares.
 template <int VEC>
-__device__ __forceinline__ void rec_join(const RecArgs& a, RecExchange<VEC>& ex, long flat, bool live, int first, int count,
+__device__ __forceinline__ void rec_join(const RecArgs& a, RecExchange<VEC>& ex, long flat, int first, int count,
                                          int step, int wave, int lane, float* s) {
   const long cols = (long)a.rows * a.width;
   const int each = (count + REC_W - 1) / REC_W;
   float p[VEC], q[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; j++) p[j] = 1.f, q[j] = 0.f;
-  if (live) {
+  {
     const int end = min(count, (wave + 1) * each);
-#pragma unroll 4
-    for (int i = wave * each; i < end; i++) {
-      const float* pair = a.pairs + 2 * cols * (first + i * step) + flat;
+    for (int i0 = wave * each; i0 < end; i0 += 8) {  // eight pairs on their way at a time
+      rec_vec<float, VEC> pw[8], qw[8];
 #pragma unroll
-      for (int j = 0; j < VEC; j++) rec_compose(pair[j], pair[cols + j], p[j], q[j]);
+      for (int u = 0; u < 8; u++) {
+        const float* pair = a.pairs + 2 * cols * (first + min(i0 + u, end - 1) * step) + flat;
+        pw[u] = *(const rec_vec<float, VEC>*)pair;
+        qw[u] = *(const rec_vec<float, VEC>*)(pair + cols);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; u++)
+        if (i0 + u < end) {
+#pragma unroll
+          for (int j = 0; j < VEC; j++) rec_compose(pw[u][j], qw[u][j], p[j], q[j]);
+        }
     }
   }
 #pragma unroll
@@ -311,8 +324,8 @@ __device__ __forceinline__ void rec_join(const RecArgs& a, RecExchange<VEC>& ex,
 template <typename T, int VEC, bool BACK>
 __global__ __launch_bounds__(64 * REC_W) void mg_recurrence_pairs_kernel(RecArgs a, RecGrads d) {
   __shared__ RecExchange<VEC> ex;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const RecPlace<T, VEC> at(a, blockIdx.x * 64 + lane);
+  const int lane = threadIdx.x & 63, wave = rec_wave();
+  const RecPlace<VEC> at(a, blockIdx.x * 64 + lane);
   const T* x = BACK ? (d.dh ? (const T*)d.dh + at.row * d.dh_row + at.col : nullptr) : (const T*)a.x + at.row * a.x_row + at.col;
   const long x_step = BACK ? d.dh_step : a.x_step;
   const T* g = (const T*)a.gate + at.row * a.g_row + at.col;
@@ -326,35 +339,33 @@ __global__ __launch_bounds__(64 * REC_W) void mg_recurrence_pairs_kernel(RecArgs
     const unsigned k = BACK ? a.tiles_each - 1 - kk : kk;
     const long t = t_begin + (long)k * REC_L;
     const int n = (int)min((long)REC_L, a.steps - t);
-    if (n <= 0 || !at.live) continue;
+    if (n <= 0) continue;
     RecTile<T, VEC> xt, gt;
-    if (x) rec_load<T, VEC>(xt, x + t * x_step, x_step, n);
-    rec_load<T, VEC>(gt, g + t * a.g_step, a.g_step, n);
+    if (x) rec_load<T, VEC>(xt, x + t * x_step, x_step, n, 0.f);
+    rec_load<T, VEC>(gt, g + t * a.g_step, a.g_step, n, INFINITY);
     const unsigned rt = rec_resets(rs ? rs + t : nullptr, n);
 #pragma unroll
     for (int ii = 0; ii < REC_L; ii++) {
       const int i = BACK ? REC_L - 1 - ii : ii;
-      if (i < n) {
 #pragma unroll
-        for (int j = 0; j < VEC; j++) {
-          float ga, gw;
-          rec_gate((float)gt.v[i][j], ga, gw);
-          const bool reset = (rt >> i) & 1;
-          if (BACK) {
-            q[j] = reset ? 0.f : ga * (x ? q[j] + (float)xt.v[i][j] : q[j]);
-          } else {
-            const float b = gw * (float)xt.v[i][j];
-            q[j] = reset ? b : fmaf(ga, q[j], b);
-          }
-          p[j] = reset ? -0.f : p[j] * ga;
+      for (int j = 0; j < VEC; j++) {
+        float ga, gw;
+        rec_gate((float)gt.v[i][j], ga, gw);
+        const bool reset = (rt >> i) & 1;
+        if (BACK) {
+          q[j] = reset ? 0.f : ga * (x ? q[j] + (float)xt.v[i][j] : q[j]);
+        } else {
+          const float b = gw * (float)xt.v[i][j];
+          q[j] = reset ? b : fmaf(ga, q[j], b);
         }
+        p[j] = reset ? -0.f : p[j] * ga;
       }
     }
   }
 #pragma unroll
   for (int j = 0; j < VEC; j++) ex.p[0][wave][j][lane] = p[j], ex.q[0][wave][j][lane] = q[j];
   __syncthreads();
-  if (wave || !at.live) return;
+  if (wave) return;
   const long cols = (long)a.rows * a.width;
   float* pair = a.pairs + 2 * cols * blockIdx.y + (long)at.row * a.width + at.col;
 #pragma unroll
@@ -373,8 +384,8 @@ template <typename T, int VEC>
 __global__ __launch_bounds__(64 * REC_W) void mg_recurrence_tile_kernel(RecArgs a, T* __restrict__ h, float* __restrict__ last,
                                                                         float* __restrict__ marks) {
   __shared__ RecExchange<VEC> ex;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const RecPlace<T, VEC> at(a, blockIdx.x * 64 + lane);
+  const int lane = threadIdx.x & 63, wave = rec_wave();
+  const RecPlace<VEC> at(a, blockIdx.x * 64 + lane);
   const T* x = (const T*)a.x + at.row * a.x_row + at.col;
   const T* g = (const T*)a.gate + at.row * a.g_row + at.col;
   const unsigned char* rs = a.resets ? a.resets + at.row * a.steps : nullptr;
@@ -384,21 +395,28 @@ __global__ __launch_bounds__(64 * REC_W) void mg_recurrence_tile_kernel(RecArgs 
   float s[VEC];  // the state entering the tile, the same in all waves
 #pragma unroll
   for (int j = 0; j < VEC; j++) s[j] = a.state ? a.state[flat + j] : 0.f;
-  if (gridDim.y > 1) rec_join<VEC>(a, ex, flat, at.live, 0, blockIdx.y, 1, wave, lane, s);
   const unsigned k_begin = blockIdx.y * a.tiles_each, k_end = min(a.tiles, k_begin + a.tiles_each);
+  RecTile<T, VEC> xt, gt;
+  unsigned rt = 0;
+  auto fetch = [&](unsigned k) {
+    const long t = (long)k * REC_TILE + wave * REC_L;
+    const int n = (int)min((long)REC_L, a.steps - t);
+    if (n <= 0) return;
+    rec_load<T, VEC>(xt, x + t * a.x_step, a.x_step, n, 0.f);
+    rec_load<T, VEC>(gt, g + t * a.g_step, a.g_step, n, INFINITY);
+    rt = rec_resets(rs ? rs + t : nullptr, n);
+  };
+  fetch(k_begin);
+  if (gridDim.y > 1) rec_join<VEC>(a, ex, flat, 0, blockIdx.y, 1, wave, lane, s);
   for (unsigned k = k_begin; k < k_end; k++) {
     const int buf = (k - k_begin) & 1;
     const long t = (long)k * REC_TILE + wave * REC_L;
-    const int n = at.live ? (int)min((long)REC_L, a.steps - t) : 0;
+    const int n = (int)min((long)REC_L, a.steps - t);
+    if (k != k_begin) fetch(k);
     float ga[REC_L][VEC], q[REC_L][VEC], p[VEC], c[VEC];
-    unsigned rt = 0;
 #pragma unroll
     for (int j = 0; j < VEC; j++) p[j] = 1.f, c[j] = 0.f;
     if (n > 0) {
-      RecTile<T, VEC> xt, gt;
-      rec_load<T, VEC>(xt, x + t * a.x_step, a.x_step, n);
-      rec_load<T, VEC>(gt, g + t * a.g_step, a.g_step, n);
-      rt = rec_resets(rs ? rs + t : nullptr, n);
 #pragma unroll
       for (int i = 0; i < REC_L; i++) {
 #pragma unroll
@@ -406,11 +424,9 @@ __global__ __launch_bounds__(64 * REC_W) void mg_recurrence_tile_kernel(RecArgs 
           float gw;
           rec_gate((float)gt.v[i][j], ga[i][j], gw);
           q[i][j] = gw * (float)xt.v[i][j];
-          if (i < n) {
-            const bool reset = (rt >> i) & 1;
-            c[j] = reset ? q[i][j] : fmaf(ga[i][j], c[j], q[i][j]);
-            p[j] = reset ? -0.f : p[j] * ga[i][j];
-          }
+          const bool reset = (rt >> i) & 1;
+          c[j] = reset ? q[i][j] : fmaf(ga[i][j], c[j], q[i][j]);
+          p[j] = reset ? -0.f : p[j] * ga[i][j];
         }
       }
     }
@@ -432,21 +448,19 @@ __global__ __launch_bounds__(64 * REC_W) void mg_recurrence_tile_kernel(RecArgs 
         for (int j = 0; j < VEC; j++) mv[j] = mine[j];
         *(rec_vec<float, VEC>*)(mark + (t / REC_L - 1) * a.width) = mv;
       }
+      RecTile<T, VEC> o;
 #pragma unroll
       for (int i = 0; i < REC_L; i++) {
-        if (i < n) {
-          rec_vec<T, VEC> o;
 #pragma unroll
-          for (int j = 0; j < VEC; j++) {
-            mine[j] = (rt >> i) & 1 ? q[i][j] : fmaf(ga[i][j], mine[j], q[i][j]);
-            o[j] = (T)mine[j];
-          }
-          if (out) *(rec_vec<T, VEC>*)(out + (t + i) * a.width) = o;
+        for (int j = 0; j < VEC; j++) {
+          mine[j] = (rt >> i) & 1 ? q[i][j] : fmaf(ga[i][j], mine[j], q[i][j]);
+          o.v[i][j] = (T)mine[j];
         }
       }
+      if (out) rec_store<T, VEC>(o, out + t * a.width, a.width, n);
     }
   }
-  if (at.live && wave == 0 && k_end == a.tiles) {
+  if (wave == 0 && k_end == a.tiles) {
 #pragma unroll
     for (int j = 0; j < VEC; j++) last[flat + j] = s[j];
   }
@@ -455,8 +469,8 @@ __global__ __launch_bounds__(64 * REC_W) void mg_recurrence_tile_kernel(RecArgs 
 template <typename T, int VEC>
 __global__ __launch_bounds__(64 * REC_W) void mg_recurrence_tile_backward_kernel(RecArgs a, RecMarks m, RecGrads d) {
   __shared__ RecExchange<VEC> ex;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const RecPlace<T, VEC> at(a, blockIdx.x * 64 + lane);
+  const int lane = threadIdx.x & 63, wave = rec_wave();
+  const RecPlace<VEC> at(a, blockIdx.x * 64 + lane);
   const T* x = (const T*)a.x + at.row * a.x_row + at.col;
   const T* g = (const T*)a.gate + at.row * a.g_row + at.col;
   const T* dh = d.dh ? (const T*)d.dh + at.row * d.dh_row + at.col : nullptr;
@@ -468,45 +482,52 @@ __global__ __launch_bounds__(64 * REC_W) void mg_recurrence_tile_backward_kernel
   float v[VEC];  // what flows into the tile from the steps behind it, the same in all waves
 #pragma unroll
   for (int j = 0; j < VEC; j++) v[j] = d.dlast ? d.dlast[flat + j] : 0.f;
-  if (gridDim.y > 1) rec_join<VEC>(a, ex, flat, at.live, gridDim.y - 1, gridDim.y - 1 - blockIdx.y, -1, wave, lane, v);
   const unsigned k_begin = blockIdx.y * a.tiles_each, k_end = min(a.tiles, k_begin + a.tiles_each);
+  RecTile<T, VEC> xt, gt, dt;
+  unsigned rt = 0;
+  float s[VEC];
+  auto fetch = [&](unsigned k) {
+    const long t0 = (long)k * REC_TILE + wave * REC_L;
+    const int n = (int)min((long)REC_L, a.steps - t0);
+    if (n <= 0) return;
+    rec_load<T, VEC>(xt, x + t0 * a.x_step, a.x_step, n, 0.f);
+    rec_load<T, VEC>(gt, g + t0 * a.g_step, a.g_step, n, INFINITY);
+    if (dh) rec_load<T, VEC>(dt, dh + t0 * d.dh_step, d.dh_step, n, 0.f);
+    rt = rec_resets(rs ? rs + t0 : nullptr, n);
+#pragma unroll
+    for (int j = 0; j < VEC; j++) s[j] = t0 ? mark[(t0 / REC_L - 1) * m.stride + j] : a.state ? a.state[flat + j] : 0.f;
+  };
+  fetch(k_end - 1);
+  if (gridDim.y > 1) rec_join<VEC>(a, ex, flat, gridDim.y - 1, gridDim.y - 1 - blockIdx.y, -1, wave, lane, v);
   for (unsigned k = k_end; k-- > k_begin;) {
     const int buf = (k_end - 1 - k) & 1;
     const long t0 = (long)k * REC_TILE + wave * REC_L;
-    const int n = at.live ? (int)min((long)REC_L, a.steps - t0) : 0;
-    float before[REC_L][VEC], ga[REC_L][VEC], gw[REC_L][VEC], p[VEC], c[VEC];
-    RecTile<T, VEC> xt, dt;
-    unsigned rt = 0;
+    const int n = (int)min((long)REC_L, a.steps - t0);
+    float ak[REC_L][VEC], gw[REC_L][VEC], e[REC_L][VEC], p[VEC], c[VEC];  // ak: a, or -0 at a reset; e: dgate / d
 #pragma unroll
     for (int j = 0; j < VEC; j++) p[j] = 1.f, c[j] = 0.f;
+    if (k + 1 < k_end) fetch(k);
     if (n > 0) {
-      RecTile<T, VEC> gt;
-      rec_load<T, VEC>(xt, x + t0 * a.x_step, a.x_step, n);
-      rec_load<T, VEC>(gt, g + t0 * a.g_step, a.g_step, n);
-      if (dh) rec_load<T, VEC>(dt, dh + t0 * d.dh_step, d.dh_step, n);
-      rt = rec_resets(rs ? rs + t0 : nullptr, n);
-      float s[VEC];
-#pragma unroll
-      for (int j = 0; j < VEC; j++) s[j] = t0 ? mark[(t0 / REC_L - 1) * m.stride + j] : a.state ? a.state[flat + j] : 0.f;
 #pragma unroll
       for (int i = 0; i < REC_L; i++) {
 #pragma unroll
         for (int j = 0; j < VEC; j++) {
-          rec_gate((float)gt.v[i][j], ga[i][j], gw[i][j]);
-          const float q = gw[i][j] * (float)xt.v[i][j];
-          before[i][j] = (rt >> i) & 1 ? 0.f : s[j];
-          s[j] = (rt >> i) & 1 ? q : fmaf(ga[i][j], s[j], q);
+          float ga;
+          rec_gate((float)gt.v[i][j], ga, gw[i][j]);
+          const float xv = (float)xt.v[i][j], q = gw[i][j] * xv;
+          const bool reset = (rt >> i) & 1;
+          e[i][j] = ((reset ? 0.f : s[j]) - xv) * (ga * gw[i][j]);
+          ak[i][j] = reset ? -0.f : ga;
+          s[j] = rec_apply(ak[i][j], q, s[j]);
         }
       }
 #pragma unroll
       for (int i = REC_L - 1; i >= 0; i--) {
-        if (i < n) {
 #pragma unroll
-          for (int j = 0; j < VEC; j++) {
-            const bool reset = (rt >> i) & 1;
-            c[j] = reset ? 0.f : ga[i][j] * (dh ? c[j] + (float)dt.v[i][j] : c[j]);
-            p[j] = reset ? -0.f : p[j] * ga[i][j];
-          }
+        for (int j = 0; j < VEC; j++) {
+          const float cd = dh ? c[j] + (float)dt.v[i][j] : c[j];
+          c[j] = rec_apply(ak[i][j], 0.f, cd);
+          p[j] = __float_as_int(ak[i][j]) < 0 ? -0.f : p[j] * ak[i][j];
         }
       }
     }
@@ -522,24 +543,22 @@ __global__ __launch_bounds__(64 * REC_W) void mg_recurrence_tile_backward_kernel
       }
     }
     if (n > 0) {
+      RecTile<T, VEC> ox, og;
 #pragma unroll
       for (int i = REC_L - 1; i >= 0; i--) {
-        if (i < n) {
-          rec_vec<T, VEC> ox, og;
 #pragma unroll
-          for (int j = 0; j < VEC; j++) {
-            const float dd = dh ? mine[j] + (float)dt.v[i][j] : mine[j];
-            ox[j] = (T)(gw[i][j] * dd);
-            og[j] = (T)(dd * (before[i][j] - (float)xt.v[i][j]) * (ga[i][j] * gw[i][j]));
-            mine[j] = (rt >> i) & 1 ? 0.f : ga[i][j] * dd;
-          }
-          *(rec_vec<T, VEC>*)(dx + (t0 + i) * d.dx_step) = ox;
-          *(rec_vec<T, VEC>*)(dg + (t0 + i) * d.dg_step) = og;
+        for (int j = 0; j < VEC; j++) {
+          const float dd = dh ? mine[j] + (float)dt.v[i][j] : mine[j];
+          ox.v[i][j] = (T)(gw[i][j] * dd);
+          og.v[i][j] = (T)(dd * e[i][j]);
+          mine[j] = rec_apply(ak[i][j], 0.f, dd);
         }
       }
+      rec_store<T, VEC>(ox, dx + t0 * d.dx_step, d.dx_step, n);
+      rec_store<T, VEC>(og, dg + t0 * d.dg_step, d.dg_step, n);
     }
   }
-  if (d.dstate && at.live && wave == 0 && k_begin == 0) {
+  if (d.dstate && wave == 0 && k_begin == 0) {
 #pragma unroll
     for (int j = 0; j < VEC; j++) d.dstate[flat + j] = v[j];
   }
@@ -559,16 +578,17 @@ static int rec_check(const char* who, const mg_recurrence* r) {
 }
 
 // How the work is laid out; a function of the shape alone, so that results do not depend on addresses.
-struct RecPlan { bool shared; unsigned tiles, tiles_each, splits; };
+struct RecPlan { bool shared; unsigned tiles, tiles_each, splits; int vec; };
 
 static RecPlan rec_plan(const mg_recurrence* r) {
-  RecPlan p{false, (unsigned)((r->steps + REC_TILE - 1) / REC_TILE), 0, 1};
-  const int64_t waves = (r->rows * r->width + 127) / 128;  // of 64 lanes with two columns each
+  RecPlan p{false, (unsigned)((r->steps + REC_TILE - 1) / REC_TILE), 0, 1, 2};
+  const int64_t waves = (r->rows * r->width + 127) / (r->type == MG_F32 ? 64 : 128);
   p.shared = waves < 2048 && r->steps > REC_L;
   if (p.shared && p.tiles >= 4) {
     const int64_t want = (512 + waves - 1) / waves;
     p.splits = (unsigned)(want < p.tiles ? want : p.tiles);
   }
+  if (p.shared && r->type == MG_F32) p.vec = 1;
   p.tiles_each = (p.tiles + p.splits - 1) / p.splits;
   p.splits = (p.tiles + p.tiles_each - 1) / p.tiles_each;
   return p;
@@ -641,7 +661,7 @@ extern "C" int mg_gated_recurrence(const mg_recurrence* r, void* h, float* last,
       return rec_launched(who);
     };
     const int64_t e = sizeof(T);
-    if (rec_fits(2, e, r->width, {r->x, r->gate, h}, {r->state, last, marks}, {r->x_row, r->x_step, r->gate_row, r->gate_step}))
+    if (p.vec == 2 && rec_fits(2, e, r->width, {r->x, r->gate, h}, {r->state, last, marks}, {r->x_row, r->x_step, r->gate_row, r->gate_step}))
       return with(rec_int<2>());
     return with(rec_int<1>());
   });
@@ -677,7 +697,7 @@ extern "C" int mg_gated_recurrence_backward(const mg_recurrence* r, const float*
       return rec_launched(who);
     };
     const int64_t e = sizeof(T);
-    if (rec_fits(2, e, r->width, {r->x, r->gate, d->dh, d->dx, d->dgate}, {},
+    if (p.vec == 2 && rec_fits(2, e, r->width, {r->x, r->gate, d->dh, d->dx, d->dgate}, {},
                  {r->x_row, r->x_step, r->gate_row, r->gate_step, d->dh_row, d->dh_step, d->dx_row, d->dx_step, d->dgate_row, d->dgate_step}))
       return with(rec_int<2>());
     return with(rec_int<1>());

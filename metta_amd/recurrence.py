@@ -28,11 +28,12 @@ TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # MG_F32, MG_BF
 
 def _launch(name: str, device: torch.device, *args) -> None:
     L = native.load()
+    stream = torch._C._cuda_getCurrentRawStream(device.index)  # current_stream(device).cuda_stream without the objects
     if device.index == torch.cuda.current_device():
-        rc = getattr(L, name)(*args, torch.cuda.current_stream().cuda_stream)
+        rc = getattr(L, name)(*args, stream)
     else:
         with torch.cuda.device(device):
-            rc = getattr(L, name)(*args, torch.cuda.current_stream(device).cuda_stream)
+            rc = getattr(L, name)(*args, stream)
     if rc:
         native.check(rc, L)
 
