@@ -366,6 +366,8 @@ int mg_gated_recurrence_backward(const mg_recurrence* r, const float* marks, int
  * i32, entries outside [0, width) count for nothing.  A row stride of 0 shares a control among all rows; NULL: none. */
 #define MG_ALLOWED_BOOL 1
 #define MG_ALLOWED_BITS 2
+/* Rows up to this many tokens stay in registers: their backward pass wants neither stats nor entropy back. */
+#define MG_EVALUATE_STATS_WIDTH 1024
 typedef struct mg_logits {
   const void* logits;
   const float* bias;
@@ -374,8 +376,13 @@ typedef struct mg_logits {
   int64_t rows;
   int64_t logits_row, bias_row, allowed_row, history_row;
   double temperature, repetition, presence, frequency;
+  void* workspace;                 /* mg_logits_workspace bytes of device memory, for this call alone */
+  int64_t workspace_bytes;
   int32_t width, history_len, allowed_kind, type;
 } mg_logits;
+
+/* Bytes of workspace that mg_sample_actions and mg_evaluate_actions need (0 up to MG_EVALUATE_STATS_WIDTH tokens). */
+int64_t mg_logits_workspace(const mg_logits* a);
 
 /* Adjusted logits, contiguous and of `type`; backward: dlogits = dout * d adjusted / d logits (0 where masked). */
 int mg_adjust_logits(const mg_logits* a, void* out, void* stream);

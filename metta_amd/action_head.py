@@ -85,6 +85,8 @@ class _Head:
                 raise RuntimeError("history must be int32")
             if history.shape[:-1] != lead or history.dim() < 1:
                 raise RuntimeError("history must be [..., L] with the logits' leading dimensions")
+            if history.size(-1) > 1 << 30:
+                raise RuntimeError("history must have at most 2^30 entries")
             if history.size(-1) == 0 or (repetition == 1.0 and presence == 0.0 and frequency == 0.0):
                 history = None
         elif repetition != 1.0 or presence != 0.0 or frequency != 0.0:
@@ -99,7 +101,7 @@ class _Head:
         self.args = native.MgLogits(
             logits.data_ptr(), None if bias is None else bias.data_ptr(), None if allowed is None else allowed.data_ptr(),
             None if history is None else history.data_ptr(), logits.size(0), logits.stride(0), bias_row, allowed_row,
-            0 if history is None else history.stride(0), temperature, repetition, presence, frequency, v,
+            0 if history is None else history.stride(0), temperature, repetition, presence, frequency, None, 0, v,
             0 if history is None else history.size(1), kind, TYPES[logits.dtype],
         )  # fmt: skip
 
@@ -121,6 +123,16 @@ class _Head:
             return t.detach().contiguous(), 0
         t = self._rows(t)
         return t, t.stride(0)
+
+
+def _workspace(args: native.MgLogits, device: torch.device) -> Optional[Tensor]:
+    """Memory of this call's own (torch's allocator keeps it for the stream, and for a captured graph), set in `args`."""
+    if args.width <= native.STATS_WIDTH:
+        return None
+    size = native.load().mg_logits_workspace(ct.byref(args))
+    w = torch.empty(size, dtype=torch.uint8, device=device)
+    args.workspace, args.workspace_bytes = w.data_ptr(), size
+    return w
 
 
 def _per_row(name: str, t: Tensor, dtypes, lead, device) -> Tensor:
@@ -173,10 +185,13 @@ class _EvaluateActions(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         logp = torch.empty(head.lead, dtype=torch.float32, device=logits.device)
         entropy = torch.empty_like(logp)
-        stats = torch.empty(*head.lead, 2, dtype=torch.float64, device=logits.device) if ctx.needs_input_grad[0] else None
+        wide = ctx.needs_input_grad[0] and logits.size(-1) > native.STATS_WIDTH
+        stats = torch.empty(*head.lead, 2, dtype=torch.float64, device=logits.device) if wide else None
         if logp.numel():
+            w = _workspace(head.args, logits.device)
             _launch("mg_evaluate_actions", logits.device, ct.byref(head.args), actions.data_ptr(), logp.data_ptr(), entropy.data_ptr(),
                     None if stats is None else stats.data_ptr())  # fmt: skip
+            del w
         _save(ctx, logits, head, actions, entropy, stats)
         return logp, entropy
 
@@ -189,7 +204,7 @@ class _EvaluateActions(torch.autograd.Function):
         d = torch.empty(ctx.shape, dtype=logits.dtype, device=logits.device)
         if d.numel():
             dlogp, dentropy = (None if g is None else g.contiguous() for g in (dlogp, dentropy))
-            _launch("mg_evaluate_actions_backward", d.device, ct.byref(head.args), actions.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
+            _launch("mg_evaluate_actions_backward", d.device, ct.byref(head.args), actions.data_ptr(), entropy.data_ptr(), None if stats is None else stats.data_ptr(),
                     None if dlogp is None else dlogp.data_ptr(), None if dentropy is None else dentropy.data_ptr(), d.data_ptr())  # fmt: skip
         return d, None, None
 
@@ -236,8 +251,10 @@ def sample_actions(
     logp = torch.empty(head.lead, dtype=torch.float32, device=logits.device)
     entropy = torch.empty_like(logp)
     if actions.numel():
+        w = _workspace(head.args, logits.device)
         _launch("mg_sample_actions", logits.device, ct.byref(head.args), None if uniforms is None else uniforms.data_ptr(), actions.data_ptr(),
                 logp.data_ptr(), entropy.data_ptr())  # fmt: skip
+        del w
     return actions, logp, entropy
 
 

@@ -86,6 +86,8 @@ class MgLogits(ct.Structure):
         ("repetition", ct.c_double),
         ("presence", ct.c_double),
         ("frequency", ct.c_double),
+        ("workspace", ct.c_void_p),
+        ("workspace_bytes", ct.c_int64),
         ("width", ct.c_int32),
         ("history_len", ct.c_int32),
         ("allowed_kind", ct.c_int32),
@@ -94,6 +96,7 @@ class MgLogits(ct.Structure):
 
 
 MARK_STEPS = 16  # MG_RECURRENCE_MARK_STEPS
+STATS_WIDTH = 1024  # MG_EVALUATE_STATS_WIDTH
 ALLOWED_BOOL, ALLOWED_BITS = 1, 2  # MG_ALLOWED_*
 
 # name -> (restype, argtypes); every symbol include/mettagrid_hip.h declares
@@ -168,6 +171,7 @@ SYMBOLS = {
         ct.c_int,
         [ct.POINTER(MgRecurrence), _vp, ct.c_int64, ct.c_int64, ct.POINTER(MgRecurrenceGradients), _vp],
     ),
+    "mg_logits_workspace": (ct.c_int64, [ct.POINTER(MgLogits)]),
     "mg_adjust_logits": (ct.c_int, [ct.POINTER(MgLogits), _vp, _vp]),
     "mg_adjust_logits_backward": (ct.c_int, [ct.POINTER(MgLogits), _vp, _vp, _vp]),
     "mg_sample_actions": (ct.c_int, [ct.POINTER(MgLogits), _vp, _vp, _vp, _vp, _vp]),
