@@ -12,8 +12,8 @@
 // or +infinity among its allowed tokens has action -1 and NaN.
 //
 // Rows of up to HEAD_NARROW columns are held in registers, E adjacent columns per lane, by as many lanes as that takes
-// (one lane for five actions, a wave for a thousand), so logits are read once.  Wider rows are cut into parts of
-// HEAD_PART columns, a block each; what a part found (maximum, sum, ...) goes to a workspace and a second launch joins
+// (one lane for five actions, a wave for a thousand), so logits are read once.  Wider rows are cut into parts of one or
+// four times HEAD_CHUNK columns, a block each; what a part found (maximum, sum, ...) goes to a workspace and a second launch joins
 // the parts of a row.  A history is counted in LDS by the block that needs it, for the columns that it holds.
 //
 // Sampling is done in 64 bits from the exponential on: an action that falls next to a border of the distribution is then
@@ -31,8 +31,6 @@
 #define HEAD_THREADS 256
 #define HEAD_NARROW MG_EVALUATE_STATS_WIDTH
 #define HEAD_CHUNK (HEAD_THREADS * 8)  // columns that a block holds as 8 per thread
-#define HEAD_CHUNKS 4
-#define HEAD_PART (HEAD_CHUNKS * HEAD_CHUNK)
 #define HEAD_FOUND 5  // doubles per part in the workspace: M, Z, sum d exp(-d), bad, first column of M
 
 extern int mg_fail_msg(const std::string& m);  // mettagrid_hip.hip: sets mg_last_error(), returns 1
@@ -110,13 +108,30 @@ __device__ __forceinline__ double head_exp(double d) {
   p = fma(p, r, 1.0);
   return d > 746.0 ? 0.0 : ldexp(p, (int)n);  // (the smallest denormal is e^-745)
 }
-// the same in 32 bits: exp2 of a product carried in two parts
-__device__ __forceinline__ float head_exp(float d) {
-  const float hi = d * -1.44269502f;  // log2 e = 1.44269502 + 1.92596303e-8
-  const float lo = fmaf(d, -1.92596303e-8f, fmaf(d, -1.44269502f, -hi));
-  const float e = __builtin_amdgcn_exp2f(hi);
-  return hi < -126.f ? 0.f : fmaf(e, lo * 0.693147182f, e);
-}
+
+// What a row's exponentials and gradients are scaled by: weight(t) = exp(-t / temperature) for t = M - x.  In 32 bits the
+// scale and log2 e are one factor, and the hardware's exp2 does the rest: the difference, the factor and the product
+// round once each, 3 u t / temperature relative, plus the 2 u of exp2.
+template <typename X> struct HeadScale;
+template <> struct HeadScale<double> {
+  double inv_temp;
+  __device__ explicit HeadScale(double i) : inv_temp(i) {}
+  __device__ __forceinline__ double weight(double t) const { return head_exp(t * inv_temp); }
+  __device__ __forceinline__ double weight(double t, double log_z) const { return head_exp(t * inv_temp + log_z); }
+};
+template <> struct HeadScale<float> {
+  float inv_temp, k;
+  __device__ explicit HeadScale(double i) : inv_temp((float)i), k((float)(i * -1.4426950408889634)) {}
+  __device__ __forceinline__ float weight(float t) const { return __builtin_amdgcn_exp2f(t * k); }
+  __device__ __forceinline__ float weight(float t, float log_z) const { return __builtin_amdgcn_exp2f(fmaf(t, k, log_z * -1.44269504f)); }
+};
+__device__ __forceinline__ double head_fma(double a, double b, double c) { return fma(a, b, c); }
+__device__ __forceinline__ float head_fma(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ double head_max(double a, double b) { return fmax(a, b); }  // (a NaN loses)
+__device__ __forceinline__ float head_max(float a, float b) { return fmaxf(a, b); }
+// t kept finite: its weight is 0 long before, and 0 * t has to be 0
+__device__ __forceinline__ double head_finite(double t) { return fmin(t, 1e300); }
+__device__ __forceinline__ float head_finite(float t) { return fminf(t, 1e37f); }
 __device__ __forceinline__ double head_log(double z) { return log(z); }
 __device__ __forceinline__ float head_log(float z) { return logf(z); }
 
@@ -165,37 +180,43 @@ __device__ __forceinline__ unsigned head_allowed(const HeadRow& r, int v0, int n
   return inside;
 }
 
-// the whole factor of a gradient, from what head_columns leaves in `slope`
-__device__ __forceinline__ double head_slope(const HeadRow& r, float slope) { return slope * r.inv_temp; }
+// bit e of `bits` over a whole word
+__device__ __forceinline__ unsigned head_bit(unsigned bits, int e) { return (unsigned)((int)(bits << (31 - e)) >> 31); }
 
 // E adjacent columns from v0 on, n of them in the row: x, and (GRAD) what a gradient of x is multiplied by besides 1 /
-// temperature.  counts: of these columns in the history.
-template <int E, bool GRAD, typename X>
-__device__ __forceinline__ void head_columns(const HeadRow& r, const void* logits, int type, long at, int v0, int n,
-                                             const unsigned* counts, X* x, float* slope) {
+// temperature (0 where masked; only where ADJUST, else the bits tell).  counts: of these columns in the history.
+// ADJUST: whether there may be a bias or a history at all.  Returns the bits of the allowed columns.
+template <int E, bool GRAD, bool ADJUST, typename X>
+__device__ __forceinline__ unsigned head_columns(const HeadRow& r, const void* logits, int type, long at, int v0, int n,
+                                                 const unsigned* counts, X* x, float* slope) {
   float l[E];
   head_load<E>(logits, type, at + v0, n, l);
   const unsigned ok = head_allowed<E>(r, v0, n);
-  float b[E];
-  if (std::is_same<X, double>::value && r.bias) head_load<E>(r.bias, MG_F32, v0, n, b);
 #pragma unroll
   for (int e = 0; e < E; e++) {
-    X y = l[e];
-    if (GRAD) slope[e] = 1.f;
-    if (std::is_same<X, double>::value) {
-      if (r.counted) {
-        const unsigned c = counts[e];
-        if (c) {
-          if (GRAD) slope[e] = (float)(y > 0 ? r.inv_rep : r.rep);
-          y = (y > 0 ? y * r.inv_rep : y * r.rep) - r.frequency * c - r.presence;
-        }
-      }
-      if (r.bias) y += b[e];
-    }
-    const bool in = (ok >> e) & 1;
-    x[e] = in ? y : (X)-INFINITY;
-    if (GRAD && !in) slope[e] = 0.f;
+    const unsigned in = head_bit(ok, e);
+    x[e] = (X)__uint_as_float((__float_as_uint(l[e]) & in) | (0xFF800000u & ~in));  // masked: -infinity
   }
+  if (!ADJUST) return ok;
+  if (r.counted) {
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      const unsigned c = counts[e];
+      const X y = (x[e] > 0 ? x[e] * r.inv_rep : x[e] * r.rep) - r.frequency * c - r.presence;
+      if (GRAD) slope[e] = !head_bit(ok, e) ? 0.f : c ? (float)(x[e] > 0 ? r.inv_rep : r.rep) : 1.f;
+      x[e] = c ? y : x[e];
+    }
+  } else if (GRAD) {
+#pragma unroll
+    for (int e = 0; e < E; e++) slope[e] = head_bit(ok, e) ? 1.f : 0.f;
+  }
+  if (r.bias) {
+    float b[E];
+    head_load<E>(r.bias, MG_F32, v0, n, b);
+#pragma unroll
+    for (int e = 0; e < E; e++) x[e] += __uint_as_float(__float_as_uint(b[e]) & head_bit(ok, e));
+  }
+  return ok;
 }
 
 // ---- lanes ------------------------------------------------------------------------------------------------------------
@@ -232,11 +253,40 @@ __device__ __forceinline__ double head_group_before(double x, int lanes, int lan
   return sum - x;
 }
 
+// adjusted logits of E columns, or their gradient
+template <int E>
+__device__ __forceinline__ void head_adjust_columns(const mg_logits& a, const HeadRow& r, long row, int v0, int n, const unsigned* counts,
+                                                    void* out, const void* dout, void* dlogits) {
+  double x[E];
+  float slope[E], y[E];
+  if (out) {
+    head_columns<E, false, true>(r, a.logits, a.type, row * a.logits_row, v0, n, counts, x, slope);
+#pragma unroll
+    for (int e = 0; e < E; e++) y[e] = (float)(x[e] * r.inv_temp);
+    head_store<E>(out, a.type, row * a.width + v0, n, y);
+  } else if (r.counted) {
+    float go[E];
+    head_columns<E, true, true>(r, a.logits, a.type, row * a.logits_row, v0, n, counts, x, slope);
+    head_load<E>(dout, a.type, row * a.width + v0, n, go);
+#pragma unroll
+    for (int e = 0; e < E; e++) y[e] = slope[e] == 0.f ? 0.f : (float)((double)go[e] * (slope[e] * r.inv_temp));
+    head_store<E>(dlogits, a.type, row * a.width + v0, n, y);
+  } else {  // without penalties the gradient does not depend on the logits: they are not read
+    float go[E];
+    const unsigned ok = head_allowed<E>(r, v0, n);
+    head_load<E>(dout, a.type, row * a.width + v0, n, go);
+#pragma unroll
+    for (int e = 0; e < E; e++) y[e] = __uint_as_float(__float_as_uint((float)(go[e] * r.inv_temp)) & head_bit(ok, e));
+    head_store<E>(dlogits, a.type, row * a.width + v0, n, y);
+  }
+}
+
 // ---- narrow rows ------------------------------------------------------------------------------------------------------
 
-struct HeadNarrow { int lanes, rows; };  // lanes per row (a power of two), rows per block
+struct HeadNarrow { int lanes, rows; };  // lanes per row, rows per block
 
-// counts[row * lanes + lane][e] over the block's rows, all threads together; barriers inside
+// counts[row * lanes + lane][e] over the block's rows, all threads together, eight entries on their way at a time;
+// barriers inside
 template <int E>
 __device__ __forceinline__ void head_count_rows(const mg_logits& a, const HeadNarrow& g, long row0, unsigned (*counts)[E + 1]) {
   __syncthreads();
@@ -247,155 +297,151 @@ __device__ __forceinline__ void head_count_rows(const mg_logits& a, const HeadNa
   // entry threadIdx.x, then every 256th of the block's rows * history_len, row and place kept without a division a step
   const int len = a.history_len, skip = HEAD_THREADS / len, rest = HEAD_THREADS - skip * len;
   int row = threadIdx.x / len, place = threadIdx.x - row * len;
+  const int* h = a.history + row0 * a.history_row;
   while (row < rows) {
-    const int v = a.history[(row0 + row) * a.history_row + place];
-    if (v >= 0 && v < a.width) atomicAdd(&counts[row * g.lanes + v / E][v % E], 1u);
-    row += skip;
-    place += rest;
-    if (place >= len) place -= len, row++;
+    int v[8], slot[8];
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+      v[u] = row < rows ? h[row * a.history_row + place] : -1;
+      slot[u] = row * g.lanes;
+      row += skip;
+      place += rest;
+      if (place >= len) place -= len, row++;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; u++)
+      if (v[u] >= 0 && v[u] < a.width) atomicAdd(&counts[slot[u] + v[u] / E][v[u] % E], 1u);
   }
   __syncthreads();
 }
 
-// what a group of lanes knows of its row
-template <int E, typename X>
+// What the lanes of a row know of it.  ONE: a lane per row, so that the number of columns is a scalar.
+template <int E, bool ONE, typename X>
 struct HeadHeld {
-  X x[E], d[E], e[E], m, z, s;  // d and e stay unset where the row is bad or empty
+  X x[E], t[E], w[E], m, z, s, z_lane;  // t = M - x, w = its weight; t and w say nothing where the row is bad or empty
   float slope[E];
-  long row;      // clamped: the groups behind the last row do that row's work once more
-  int lane, v0, n;
+  unsigned ok;
+  long row;         // clamped: the groups behind the last row do that row's work once more
+  int lane, v0, n;  // this lane's columns, n of them (or fewer than one) in the row
   bool bad, empty, mine;  // mine: the row is this group's own
+
+  __device__ __forceinline__ void place(const mg_logits& a, const HeadNarrow& g, long row0) {
+    const long at = row0 + (ONE ? threadIdx.x : threadIdx.x / g.lanes);
+    lane = ONE ? 0 : threadIdx.x % g.lanes;
+    mine = at < a.rows && (ONE || (int)threadIdx.x < g.rows * g.lanes);
+    row = mine ? at : a.rows - 1;
+    v0 = lane * E;
+    n = a.width - v0;
+  }
+
+  template <bool GRAD>
+  __device__ __forceinline__ void hold(const mg_logits& a, const HeadNarrow& g, const HeadRow& r, const HeadScale<X>& scale, const unsigned* counts) {
+    ok = head_columns<E, GRAD, std::is_same<X, double>::value>(r, a.logits, a.type, row * a.logits_row, v0, n, counts, x, slope);
+    m = x[0];
+#pragma unroll
+    for (int e = 1; e < E; e++) m = head_max(m, x[e]);
+    if (!ONE) m = head_group(m, g.lanes, [](X p, X q) { return head_max(p, q); });
+    const X top = m < (X)INFINITY && m > (X)-INFINITY ? m : (X)0;
+    z = s = 0;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      if (!ONE || e < n) {
+        t[e] = head_finite(top - x[e]);
+        w[e] = scale.weight(top - x[e]);
+        z += w[e];
+        s = head_fma(t[e], w[e], s);
+      } else {
+        t[e] = w[e] = 0;
+      }
+    }
+    z_lane = z;
+    if (!ONE) {
+      z = head_group(z, g.lanes, [](X p, X q) { return p + q; });
+      s = head_group(s, g.lanes, [](X p, X q) { return p + q; });
+    }
+    s *= scale.inv_temp;
+    // +infinity is the largest, NaN has lost to everything but makes the sum NaN
+    bad = !(m < (X)INFINITY) || z != z;
+    empty = !bad && m == (X)-INFINITY;
+  }
 };
-
-template <int E, bool GRAD, typename X>
-__device__ __forceinline__ void head_hold(const mg_logits& a, const HeadNarrow& g, const HeadRow& r, const unsigned* counts, HeadHeld<E, X>& h) {
-  h.v0 = h.lane * E;
-  h.n = a.width - h.v0;
-  head_columns<E, GRAD>(r, a.logits, a.type, h.row * a.logits_row, h.v0, h.n, counts, h.x, h.slope);
-  X m = -INFINITY;
-  bool bad = false;
-#pragma unroll
-  for (int e = 0; e < E; e++) {
-    if (!(h.x[e] < (X)INFINITY)) bad = true;
-    m = h.x[e] > m ? h.x[e] : m;
-  }
-  h.m = head_group_max(m, g.lanes);
-  h.bad = head_group_max((int)bad, g.lanes) != 0;
-  h.empty = !h.bad && h.m == (X)-INFINITY;
-  const X top = h.bad || h.empty ? (X)0 : h.m, inv_temp = (X)r.inv_temp;
-  X z = 0, s = 0;
-#pragma unroll
-  for (int e = 0; e < E; e++) {
-    h.d[e] = (top - h.x[e]) * inv_temp;
-    h.e[e] = head_exp(h.d[e]);
-    z += h.e[e];
-    s += h.e[e] > 0 ? h.d[e] * h.e[e] : 0;
-  }
-  h.z = head_group_sum(z, g.lanes);
-  h.s = head_group_sum(s, g.lanes);
-}
-
-template <int E, typename X>
-__device__ __forceinline__ void head_place(const mg_logits& a, const HeadNarrow& g, long row0, HeadHeld<E, X>& h) {
-  const long row = row0 + threadIdx.x / g.lanes;
-  h.mine = row < a.rows;
-  h.row = h.mine ? row : a.rows - 1;
-  h.lane = threadIdx.x & (g.lanes - 1);
-}
 
 template <int E>
 __global__ __launch_bounds__(HEAD_THREADS) void mg_adjust_narrow_kernel(mg_logits a, HeadNarrow g, void* __restrict__ out,
                                                                        const void* __restrict__ dout, void* __restrict__ dlogits) {
-  using X = double;
   __shared__ unsigned counts[HEAD_THREADS][E + 1];
   for (long row0 = (long)blockIdx.x * g.rows; row0 < a.rows; row0 += (long)gridDim.x * g.rows) {
     if (a.history) head_count_rows<E>(a, g, row0, counts);
-    HeadHeld<E, X> h;
-    head_place(a, g, row0, h);
+    HeadHeld<E, false, double> h;
+    h.place(a, g, row0);
+    if (!h.mine) continue;
     const HeadRow r = head_row(a, h.row);
-    h.v0 = h.lane * E;
-    h.n = h.mine ? a.width - h.v0 : 0;
-    float y[E];
-    if (out) {
-      head_columns<E, false>(r, a.logits, a.type, h.row * a.logits_row, h.v0, h.n, counts[threadIdx.x], h.x, h.slope);
-#pragma unroll
-      for (int e = 0; e < E; e++) y[e] = (float)(h.x[e] * r.inv_temp);
-      head_store<E>(out, a.type, h.row * a.width + h.v0, h.n, y);
-    } else {
-      float go[E];
-      head_columns<E, true>(r, a.logits, a.type, h.row * a.logits_row, h.v0, h.n, counts[threadIdx.x], h.x, h.slope);
-      head_load<E>(dout, a.type, h.row * a.width + h.v0, h.n, go);
-#pragma unroll
-      for (int e = 0; e < E; e++) y[e] = h.slope[e] == 0.f ? 0.f : (float)((double)go[e] * head_slope(r, h.slope[e]));
-      head_store<E>(dlogits, a.type, h.row * a.width + h.v0, h.n, y);
-    }
+    head_adjust_columns<E>(a, r, h.row, h.v0, h.n, counts[threadIdx.x], out, dout, dlogits);
   }
 }
 
-template <int E>
+template <int E, bool ONE>
 __global__ __launch_bounds__(HEAD_THREADS) void mg_sample_narrow_kernel(mg_logits a, HeadNarrow g, const float* __restrict__ uniforms,
                                                                        int* __restrict__ actions, float* __restrict__ log_prob,
                                                                        float* __restrict__ entropy) {
-  using X = double;
   __shared__ unsigned counts[HEAD_THREADS][E + 1];
   for (long row0 = (long)blockIdx.x * g.rows; row0 < a.rows; row0 += (long)gridDim.x * g.rows) {
     if (a.history) head_count_rows<E>(a, g, row0, counts);
-    HeadHeld<E, X> h;
-    head_place(a, g, row0, h);
+    HeadHeld<E, ONE, double> h;
+    h.place(a, g, row0);
     const HeadRow r = head_row(a, h.row);
-    head_hold<E, false>(a, g, r, counts[threadIdx.x], h);
+    const HeadScale<double> scale(r.inv_temp);
+    h.template hold<false>(a, g, r, scale, counts[threadIdx.x]);
     int hit = a.width, last = -1;
     if (uniforms) {
       const double target = fmax((double)uniforms[h.row], 0.0) * h.z;
-      double mine = 0.0;
+      double run = ONE ? 0.0 : head_group_before(h.z_lane, g.lanes, h.lane);
 #pragma unroll
-      for (int e = 0; e < E; e++) mine += h.e[e];
-      double run = head_group_before(mine, g.lanes, h.lane);
+      for (int e = E - 1; e >= 0; e--) last = last < 0 && h.w[e] > 0.0 ? h.v0 + e : last;
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        run += h.e[e];
+        run += h.w[e];
         if (run > target && hit == a.width && e < h.n) hit = h.v0 + e;
-        if (h.e[e] > 0.0) last = h.v0 + e;
       }
-      hit = head_group_min(hit, g.lanes);
-      last = head_group_max(last, g.lanes);
-      if (hit == a.width) hit = last;  // a uniform of 1 or more
     } else {
 #pragma unroll
       for (int e = E - 1; e >= 0; e--)
         if (h.x[e] == h.m && e < h.n) hit = h.v0 + e;
-      hit = head_group_min(hit, g.lanes);
     }
-    double d = 0.0;
+    if (!ONE) {
+      hit = head_group_min(hit, g.lanes);
+      last = head_group_max(last, g.lanes);
+    }
+    if (hit == a.width) hit = last;  // a uniform of 1 or more
+    double t = 0.0;
 #pragma unroll
-    for (int e = 0; e < E; e++) if (h.v0 + e == hit) d = h.d[e];
-    d = __shfl(d, (head_lane() & ~(g.lanes - 1)) + (hit >= 0 && hit < a.width ? hit / E : 0));
+    for (int e = 0; e < E; e++) t = h.v0 + e == hit ? h.t[e] : t;
+    if (!ONE) t = __shfl(t, (head_lane() & ~(g.lanes - 1)) + (hit >= 0 && hit < a.width ? hit / E : 0));
     if (h.mine && h.lane == 0) {
       const double log_z = head_log(h.z);
-      const bool none = h.bad || h.empty;
-      actions[h.row] = none ? -1 : hit;
-      log_prob[h.row] = h.bad ? NAN : h.empty ? 0.f : (float)(-d - log_z);
+      actions[h.row] = h.bad || h.empty ? -1 : hit;
+      log_prob[h.row] = h.bad ? NAN : h.empty ? 0.f : (float)(-t * scale.inv_temp - log_z);
       entropy[h.row] = h.bad ? NAN : h.empty ? 0.f : (float)(log_z + h.s / h.z);
     }
   }
 }
 
-template <int E, typename X>
+template <int E, bool ONE, typename X>
 __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_kernel(mg_logits a, HeadNarrow g, const int* __restrict__ actions,
                                                                          float* __restrict__ log_prob, float* __restrict__ entropy) {
   __shared__ unsigned counts[HEAD_THREADS][E + 1];
   for (long row0 = (long)blockIdx.x * g.rows; row0 < a.rows; row0 += (long)gridDim.x * g.rows) {
     if (a.history) head_count_rows<E>(a, g, row0, counts);
-    HeadHeld<E, X> h;
-    head_place(a, g, row0, h);
+    HeadHeld<E, ONE, X> h;
+    h.place(a, g, row0);
     const HeadRow r = head_row(a, h.row);
-    head_hold<E, false>(a, g, r, counts[threadIdx.x], h);
+    const HeadScale<X> scale(r.inv_temp);
     const int act = actions[h.row];
-    const bool inside = act >= 0 && act < a.width;
+    h.template hold<false>(a, g, r, scale, counts[threadIdx.x]);
     X d = INFINITY;
 #pragma unroll
-    for (int e = 0; e < E; e++) if (inside && h.v0 + e == act) d = h.d[e];
-    d = head_group_min(d, g.lanes);
+    for (int e = 0; e < E; e++) d = h.v0 + e == act && e < h.n ? (h.x[e] == (X)-INFINITY ? (X)INFINITY : h.t[e] * scale.inv_temp) : d;
+    if (!ONE) d = head_group_min(d, g.lanes);
     if (h.mine && h.lane == 0) {
       const X log_z = head_log(h.z);
       log_prob[h.row] = h.bad ? NAN : h.empty ? 0.f : (float)(-d - log_z);
@@ -404,7 +450,7 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_kernel(mg_log
   }
 }
 
-template <int E, typename X>
+template <int E, bool ONE, typename X>
 __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_backward_kernel(mg_logits a, HeadNarrow g, const int* __restrict__ actions,
                                                                                   const float* __restrict__ dlog_prob,
                                                                                   const float* __restrict__ dentropy,
@@ -412,31 +458,34 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_backward_kern
   __shared__ unsigned counts[HEAD_THREADS][E + 1];
   for (long row0 = (long)blockIdx.x * g.rows; row0 < a.rows; row0 += (long)gridDim.x * g.rows) {
     if (a.history) head_count_rows<E>(a, g, row0, counts);
-    HeadHeld<E, X> h;
-    head_place(a, g, row0, h);
+    HeadHeld<E, ONE, X> h;
+    h.place(a, g, row0);
     const HeadRow r = head_row(a, h.row);
-    head_hold<E, true>(a, g, r, counts[threadIdx.x], h);
+    const HeadScale<X> scale(r.inv_temp);
     const int act = actions[h.row];
-    X da = INFINITY;
+    const X gp_row = dlog_prob ? dlog_prob[h.row] : 0.f, gh = (dentropy ? dentropy[h.row] : 0.f) * scale.inv_temp;
+    h.template hold<true>(a, g, r, scale, counts[threadIdx.x]);
+    bool left = false;  // whether the action is a token that is left
 #pragma unroll
-    for (int e = 0; e < E; e++) if (e < h.n && h.v0 + e == act) da = h.x[e] == (X)-INFINITY ? (X)INFINITY : (X)0;
-    const bool counts_for = head_group_min(da, g.lanes) == 0;  // the action is a token of the row that is left
-    const X gp = dlog_prob && counts_for ? dlog_prob[h.row] : 0.f, gh = dentropy ? dentropy[h.row] : 0.f;
-    const X log_z = head_log(h.z), inv_z = 1 / h.z, ent = log_z + h.s * inv_z, inv_temp = (X)r.inv_temp;
+    for (int e = 0; e < E; e++) left = left || (h.v0 + e == act && e < h.n && h.x[e] > (X)-INFINITY);
+    if (!ONE) left = head_group_max((int)left, g.lanes) != 0;
+    const X gp = left ? gp_row * scale.inv_temp : (X)0, inv_z = 1 / h.z;
+    const X past = h.s * inv_z;  // H - log Z: H + log q = past - t / temperature
     float y[E];
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      const X q = h.e[e] * inv_z;
-      X d = gp * ((h.v0 + e == act ? (X)1 : (X)0) - q) - (h.e[e] > 0 ? gh * q * (ent - log_z - h.d[e]) : 0);
-      if (h.bad) d = NAN;
-      y[e] = h.empty || h.x[e] == (X)-INFINITY ? 0.f : (float)(d * inv_temp * h.slope[e]);
+      if (ONE && e >= h.n) continue;
+      const X q = h.w[e] * inv_z;
+      X d = (h.v0 + e == act ? gp : (X)0) - q * head_fma(gh, past - h.t[e] * scale.inv_temp, gp);
+      if (std::is_same<X, double>::value) d *= h.slope[e];
+      y[e] = h.empty || !(h.x[e] != (X)-INFINITY) ? 0.f : h.bad ? NAN : (float)d;
     }
     if (h.mine) head_store<E>(dlogits, a.type, h.row * a.width + h.v0, h.n, y);
   }
 }
 
 // ---- wide rows --------------------------------------------------------------------------------------------------------
-// Thread t of a block holds columns part * HEAD_PART + chunk * HEAD_CHUNK + 8 t ... + 7 of each of the part's chunks.
+// Thread t of a block holds columns 8 t ... 8 t + 7 of each of its part's chunks.
 
 // counts of the n columns from v0 on, all threads together; barriers inside
 __device__ __forceinline__ void head_count_columns(const mg_logits& a, long row, unsigned* counts, long v0, int n) {
@@ -451,127 +500,150 @@ __device__ __forceinline__ void head_count_columns(const mg_logits& a, long row,
   __syncthreads();
 }
 
-// over the block; every thread gets the result
+// x of the lane that DPP control C names (row_shr 1 ... 8 within 16 lanes, then the last lane of a row of 16 to the next
+// row, and of the first 32 lanes to the others); `none` where there is none
+template <int C, typename V>
+__device__ __forceinline__ V head_dpp(V x, V none) {
+  if constexpr (sizeof(V) == 4) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, x), C, 0xF, 0xF, false));
+  } else {
+    const long long xs = __builtin_bit_cast(long long, x), ns = __builtin_bit_cast(long long, none);
+    const unsigned lo = __builtin_amdgcn_update_dpp((int)ns, (int)xs, C, 0xF, 0xF, false);
+    const unsigned hi = __builtin_amdgcn_update_dpp((int)(ns >> 32), (int)(xs >> 32), C, 0xF, 0xF, false);
+    return __builtin_bit_cast(V, (long long)hi << 32 | lo);
+  }
+}
+// lane l: f over lanes 0 ... l
 template <typename V, typename F>
-__device__ __forceinline__ V head_block(V x, V* red, F f) {
-  for (int o = 1; o < 64; o <<= 1) x = f(x, __shfl_xor(x, o));
+__device__ __forceinline__ V head_scan(V x, V none, F f) {
+  x = f(head_dpp<0x111>(x, none), x);
+  x = f(head_dpp<0x112>(x, none), x);
+  x = f(head_dpp<0x114>(x, none), x);
+  x = f(head_dpp<0x118>(x, none), x);
+  const V a = head_dpp<0x142>(x, none);  // rows 1 and 3 take the row before them
+  x = (head_lane() & 16) ? f(a, x) : x;
+  const V b = head_dpp<0x143>(x, none);  // lanes 32 ... 63 take lane 31
+  return (head_lane() & 32) ? f(b, x) : x;
+}
+template <typename V>
+__device__ __forceinline__ V head_lane_of(V x, int lane) {
+  if constexpr (sizeof(V) == 4) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane));
+  } else {
+    const long long xs = __builtin_bit_cast(long long, x);
+    const unsigned lo = __builtin_amdgcn_readlane((int)xs, lane), hi = __builtin_amdgcn_readlane((int)(xs >> 32), lane);
+    return __builtin_bit_cast(V, (long long)hi << 32 | lo);
+  }
+}
+
+// over a block of up to 16 waves; every thread gets the result
+template <typename V, typename F>
+__device__ __forceinline__ V head_block(V x, V none, V* red, F f) {
+  x = head_lane_of(head_scan(x, none, f), 63);
   __syncthreads();
   if (head_lane() == 0) red[threadIdx.x >> 6] = x;
   __syncthreads();
   V y = red[0];
-#pragma unroll
-  for (int w = 1; w < HEAD_THREADS / 64; w++) y = f(y, red[w]);
+  for (int w = 1; w < (int)(blockDim.x >> 6); w++) y = f(y, red[w]);
   return y;
 }
 template <typename V>
 __device__ __forceinline__ V head_block_max(V x, V* red) {
-  return head_block(x, red, [](V a, V b) { return a > b ? a : b; });
+  return head_block<V>(x, std::is_same<V, int>::value ? (V)-1 : (V)-INFINITY, red, [](V a, V b) { return a > b ? a : b; });
 }
-template <typename V>
-__device__ __forceinline__ V head_block_min(V x, V* red) {
-  return head_block(x, red, [](V a, V b) { return a < b ? a : b; });
+__device__ __forceinline__ int head_block_min(int x, int* red) {
+  return head_block<int>(x, 0x7FFFFFFF, red, [](int a, int b) { return a < b ? a : b; });
 }
 template <typename V>
 __device__ __forceinline__ V head_block_sum(V x, V* red) {
-  return head_block(x, red, [](V a, V b) { return a + b; });
+  return head_block<V>(x, (V)0, red, [](V a, V b) { return a + b; });
 }
 // the sum of the threads before this one, and of all
 __device__ __forceinline__ double head_block_before(double x, double* red, double& all) {
-  const double in_wave = head_group_before(x, 64, head_lane());
+  const double to_here = head_scan(x, 0.0, [](double a, double b) { return a + b; });
   __syncthreads();
-  if (head_lane() == 63) red[threadIdx.x >> 6] = in_wave + x;
+  if (head_lane() == 63) red[threadIdx.x >> 6] = to_here;
   __syncthreads();
   double base = 0.0;
   all = 0.0;
-#pragma unroll
-  for (int w = 0; w < HEAD_THREADS / 64; w++) {
+  for (int w = 0; w < (int)(blockDim.x >> 6); w++) {
     if (w == (int)(threadIdx.x >> 6)) base = all;
     all += red[w];
   }
-  return base + in_wave;
+  return base + (to_here - x);
 }
 
+// A part is CHUNKS * HEAD_CHUNK columns.
 #define HEAD_PART_COUNTS()                                                                      \
-  __shared__ unsigned counts[HEAD_PART];                                                        \
-  const long part0 = (long)blockIdx.x * HEAD_PART;                                              \
-  const int part_n = (int)min((long)HEAD_PART, a.width - part0);                                \
+  __shared__ unsigned counts[CHUNKS * HEAD_CHUNK];                                              \
+  const long part0 = (long)blockIdx.x * (CHUNKS * HEAD_CHUNK);                                  \
+  const int part_n = (int)min((long)CHUNKS * HEAD_CHUNK, a.width - part0);                      \
   if (a.history) head_count_columns(a, row, counts, part0, part_n);
 
+template <int CHUNKS>
 __global__ __launch_bounds__(HEAD_THREADS) void mg_adjust_wide_kernel(mg_logits a, void* __restrict__ out, const void* __restrict__ dout,
                                                                      void* __restrict__ dlogits) {
   for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
     HEAD_PART_COUNTS()
     const HeadRow r = head_row(a, row);
 #pragma unroll
-    for (int c = 0; c < HEAD_CHUNKS; c++) {
+    for (int c = 0; c < CHUNKS; c++) {
       const int at = c * HEAD_CHUNK + threadIdx.x * 8, n = part_n - at;
-      if (n <= 0) continue;
-      const int v0 = (int)(part0 + at);
-      double x[8];
-      float slope[8], y[8];
-      if (out) {
-        head_columns<8, false>(r, a.logits, a.type, row * a.logits_row, v0, n, counts + at, x, slope);
-#pragma unroll
-        for (int e = 0; e < 8; e++) y[e] = (float)(x[e] * r.inv_temp);
-        head_store<8>(out, a.type, row * a.width + v0, n, y);
-      } else {
-        float go[8];
-        head_columns<8, true>(r, a.logits, a.type, row * a.logits_row, v0, n, counts + at, x, slope);
-        head_load<8>(dout, a.type, row * a.width + v0, n, go);
-#pragma unroll
-        for (int e = 0; e < 8; e++) y[e] = slope[e] == 0.f ? 0.f : (float)((double)go[e] * head_slope(r, slope[e]));
-        head_store<8>(dlogits, a.type, row * a.width + v0, n, y);
-      }
+      if (n > 0) head_adjust_columns<8>(a, r, row, (int)(part0 + at), n, counts + at, out, dout, dlogits);
     }
   }
 }
 
-// what a part knows: found[row][part] = M, Z, sum d exp(-d) (against its own M), bad, first column of M
-template <typename X>
+// what a part knows: found[row][part] = M, Z, sum (M - x) exp(-d) / temperature (against its own M), bad, first column of M
+template <int CHUNKS, bool FIRST, typename X>
 __global__ __launch_bounds__(HEAD_THREADS) void mg_head_parts_kernel(mg_logits a, double* __restrict__ found) {
-  __shared__ double red[HEAD_THREADS / 64];
+  __shared__ X red[HEAD_THREADS / 64], red_s[HEAD_THREADS / 64];
   __shared__ int red_int[HEAD_THREADS / 64];
   for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
     HEAD_PART_COUNTS()
     const HeadRow r = head_row(a, row);
-    X x[HEAD_CHUNKS][8], m = -INFINITY;
-    bool bad = false;
+    const HeadScale<X> scale(r.inv_temp);
+    X x[CHUNKS][8], m = -INFINITY;
 #pragma unroll
-    for (int c = 0; c < HEAD_CHUNKS; c++) {
+    for (int c = 0; c < CHUNKS; c++) {
       const int at = c * HEAD_CHUNK + threadIdx.x * 8, n = part_n - at;
-      if (n > 0) {
-        head_columns<8, false>(r, a.logits, a.type, row * a.logits_row, (int)(part0 + at), n, counts + at, x[c], (float*)nullptr);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[c][e] = -INFINITY;
-      }
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        if (!(x[c][e] < (X)INFINITY)) bad = true;
-        m = x[c][e] > m ? x[c][e] : m;
-      }
+      head_columns<8, false, std::is_same<X, double>::value>(r, a.logits, a.type, row * a.logits_row, (int)(part0 + at), n, counts + at, x[c],
+                                                             (float*)nullptr);
     }
-    const double top = head_block_max((double)m, red);
-    const bool any_bad = head_block_max((int)bad, red_int) != 0;
-    int first = a.width;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; c++) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) m = head_max(m, x[c][e]);
+    }
+    const X most = head_block<X>(m, -INFINITY, red, [](X p, X q) { return head_max(p, q); });
+    const X top = most < (X)INFINITY && most > (X)-INFINITY ? most : (X)0;
     X z = 0, s = 0;
-    const X inv_temp = (X)r.inv_temp, base = any_bad || top == -INFINITY ? (X)0 : (X)top;
+    int first = 0x7FFFFFFF;
 #pragma unroll
-    for (int c = 0; c < HEAD_CHUNKS; c++) {
+    for (int c = CHUNKS - 1; c >= 0; c--) {
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const X d = (base - x[c][e]) * inv_temp, w = head_exp(d);
+      for (int e = 7; e >= 0; e--) {
+        const X t = top - x[c][e], w = scale.weight(t);
         z += w;
-        s += w > 0 ? d * w : 0;
-        if (x[c][e] == base) first = min(first, (int)(part0 + c * HEAD_CHUNK + threadIdx.x * 8 + e));
+        s = head_fma(head_finite(t), w, s);
+        if (FIRST && x[c][e] == most) first = (int)(part0 + c * HEAD_CHUNK + threadIdx.x * 8 + e);
       }
     }
-    const double zz = head_block_sum((double)z, red), ss = head_block_sum((double)s, red);
-    first = head_block_min(first, red_int);
+    auto add = [](X p, X q) { return p + q; };
+    z = head_lane_of(head_scan<X>(z, 0, add), 63);
+    s = head_lane_of(head_scan<X>(s, 0, add), 63);
+    __syncthreads();
+    if (head_lane() == 0) red[threadIdx.x >> 6] = z, red_s[threadIdx.x >> 6] = s;
+    if (FIRST) first = head_block_min(first, red_int);
+    else __syncthreads();
     if (threadIdx.x == 0) {
+      double zz = 0.0, ss = 0.0;
+      for (int w = 0; w < HEAD_THREADS / 64; w++) zz += red[w], ss += red_s[w];
       double* f = found + (row * gridDim.x + blockIdx.x) * HEAD_FOUND;
-      f[0] = top; f[1] = zz; f[2] = ss; f[3] = any_bad ? 1.0 : 0.0; f[4] = first;
+      // +infinity is the largest, NaN has lost to everything but makes the sum NaN
+      f[0] = most; f[1] = zz; f[2] = ss * scale.inv_temp; f[3] = !(most < (X)INFINITY) || zz != zz ? 1.0 : 0.0; f[4] = first;
     }
+    __syncthreads();
   }
 }
 
@@ -602,41 +674,44 @@ __device__ __forceinline__ HeadJoined head_join(const double* f, int parts, doub
   return j;
 }
 
-__global__ __launch_bounds__(HEAD_THREADS) void mg_sample_join_kernel(mg_logits a, int parts, const double* __restrict__ found,
-                                                                     const float* __restrict__ uniforms, int* __restrict__ actions,
-                                                                     float* __restrict__ log_prob, float* __restrict__ entropy) {
-  __shared__ unsigned counts[HEAD_CHUNK];
-  __shared__ double red[HEAD_THREADS / 64], picked_d, picked_run;
-  __shared__ int red_int[HEAD_THREADS / 64], picked;
+// THREADS * 8 columns are a whole part
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void mg_sample_join_kernel(mg_logits a, int parts, const double* __restrict__ found,
+                                                                const float* __restrict__ uniforms, int* __restrict__ actions,
+                                                                float* __restrict__ log_prob, float* __restrict__ entropy) {
+  constexpr int PART = THREADS * 8;
+  __shared__ unsigned counts[PART];
+  __shared__ double red[THREADS / 64], picked_t, picked_run;
+  __shared__ int red_int[THREADS / 64], picked;
   for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const HeadRow r = head_row(a, row);
+    const HeadScale<double> scale(r.inv_temp);
     const double* f = found + row * parts * HEAD_FOUND;
     const HeadJoined j = head_join(f, parts, r.inv_temp, head_lane());
     int hit = -1;
-    double d_hit = 0.0;
+    double t_hit = 0.0;
     if (!j.bad && !j.empty) {
       const double target = uniforms ? fmax((double)uniforms[row], 0.0) * j.z : 0.0;
-      __syncthreads();
       if (threadIdx.x < 64) {  // one wave finds the part: the first whose running sum is above the target, or the last with any
         double run = 0.0, before = 0.0;
         int part = -1, last = -1, best = a.width;
         for (int i0 = 0; i0 < parts && part < 0; i0 += 64) {
           const int i = i0 + threadIdx.x;
           const double mi = i < parts ? f[i * HEAD_FOUND] : -INFINITY;
-          const double w = mi == -INFINITY ? 0.0 : head_exp((j.m - mi) * r.inv_temp) * f[i * HEAD_FOUND + 1];
-          const double lead = run + head_group_before(w, 64, head_lane());
+          const double w = mi == -INFINITY ? 0.0 : scale.weight(j.m - mi) * f[i * HEAD_FOUND + 1];
+          const double to_here = run + head_scan(w, 0.0, [](double p, double q) { return p + q; });
           if (!uniforms && mi == j.m) best = min(best, (int)f[i * HEAD_FOUND + 4]);
-          const unsigned long long over = __ballot(w > 0.0 && lead + w > target), some = __ballot(w > 0.0);
+          const unsigned long long over = __ballot(w > 0.0 && to_here > target), some = __ballot(w > 0.0);
           if (uniforms && over) {
-            const int k = __ffsll((unsigned long long)over) - 1;
+            const int k = __ffsll(over) - 1;
             part = i0 + k;
-            before = __shfl(lead, k);
+            before = head_lane_of(to_here - w, k);
           } else if (some) {
             const int k = 63 - __clzll((long long)some);
             last = i0 + k;
-            before = __shfl(lead, k);
+            before = head_lane_of(to_here - w, k);
           }
-          run = __shfl(lead + w, 63);
+          run = head_lane_of(to_here, 63);
         }
         best = head_group_min(best, 64);
         if (threadIdx.x == 0) picked = !uniforms ? best : part >= 0 ? part : last, picked_run = before;
@@ -645,56 +720,43 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_sample_join_kernel(mg_logits 
       if (!uniforms) {
         hit = picked;
       } else {
-        const long part0 = (long)picked * HEAD_PART;
-        double run = picked_run;
-        int last = -1;
-        double d_last = 0.0;
-        hit = a.width;
-        for (int c = 0; c < HEAD_CHUNKS && hit == a.width; c++) {
-          const long chunk0 = part0 + c * HEAD_CHUNK;
-          const int chunk_n = (int)min((long)HEAD_CHUNK, a.width - chunk0);
-          if (chunk_n <= 0) break;
-          if (a.history) head_count_columns(a, row, counts, chunk0, chunk_n);
-          const int at = threadIdx.x * 8, n = chunk_n - at;
-          double x[8], d[8], e8[8], mine = 0.0;
-          head_columns<8, false>(r, a.logits, a.type, row * a.logits_row, (int)(chunk0 + at), n, counts + at, x, (float*)nullptr);
+        const long part0 = (long)picked * PART;
+        const int part_n = (int)min((long)PART, a.width - part0);
+        if (a.history) head_count_columns(a, row, counts, part0, part_n);
+        const int at = threadIdx.x * 8, n = part_n - at;
+        double x[8], t[8], w[8], mine = 0.0;
+        head_columns<8, false, true>(r, a.logits, a.type, row * a.logits_row, (int)(part0 + at), n, counts + at, x, (float*)nullptr);
 #pragma unroll
-          for (int e = 0; e < 8; e++) {
-            d[e] = (j.m - x[e]) * r.inv_temp;
-            e8[e] = head_exp(d[e]);
-            mine += e8[e];
-          }
-          double all;
-          double sum = run + head_block_before(mine, red, all);
-          int h = a.width, l = -1;
-          double dh = 0.0, dl = 0.0;
-#pragma unroll
-          for (int e = 0; e < 8; e++) {
-            sum += e8[e];
-            if (sum > target && h == a.width && e < n) h = (int)(chunk0 + at + e), dh = d[e];
-            if (e8[e] > 0.0) l = (int)(chunk0 + at + e), dl = d[e];
-          }
-          const int h_all = head_block_min(h, red_int), l_all = head_block_max(l, red_int);
-          if (h_all < a.width && h == h_all) picked_d = dh;
-          __syncthreads();
-          if (h_all < a.width) {
-            hit = h_all;
-            d_hit = picked_d;
-          } else if (l_all >= 0) {
-            if (l == l_all) picked_run = dl;
-            __syncthreads();
-            last = l_all;
-            d_last = picked_run;
-          }
-          run += all;
+        for (int e = 0; e < 8; e++) {
+          t[e] = j.m - x[e];
+          w[e] = scale.weight(t[e]);
+          mine += w[e];
         }
-        if (hit == a.width) hit = last, d_hit = d_last;  // a uniform of 1 or more, or one that the roundings of a border took
+        double all;
+        double run = picked_run + head_block_before(mine, red, all);
+        int over = a.width, last = -1;
+        double t_over = 0.0, t_last = 0.0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          run += w[e];
+          if (run > target && over == a.width && e < n) over = (int)(part0 + at + e), t_over = t[e];
+          if (w[e] > 0.0) last = (int)(part0 + at + e), t_last = t[e];
+        }
+        hit = head_block_min(over, red_int);
+        if (hit < a.width) {
+          if (over == hit) picked_t = t_over;
+        } else {  // a uniform of 1 or more, or one that the roundings of a border took
+          hit = head_block_max(last, red_int);
+          if (last == hit) picked_t = t_last;
+        }
+        __syncthreads();
+        t_hit = picked_t;
       }
     }
     if (threadIdx.x == 0) {
       const double log_z = head_log(j.z);
       actions[row] = j.bad || j.empty ? -1 : hit;
-      log_prob[row] = j.bad ? NAN : j.empty ? 0.f : (float)(-d_hit - log_z);
+      log_prob[row] = j.bad ? NAN : j.empty ? 0.f : (float)(-t_hit * scale.inv_temp - log_z);
       entropy[row] = j.bad ? NAN : j.empty ? 0.f : (float)(log_z + j.s / j.z);
     }
     __syncthreads();
@@ -722,7 +784,7 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_join_kernel(mg_logit
     HeadRow one = r;
     if (r.kind == MG_ALLOWED_BITS) one.kind = 0;
     double y[1];
-    head_columns<1, false>(one, a.logits, a.type, row * a.logits_row, act, 1, &count, y, (float*)nullptr);
+    head_columns<1, false, true>(one, a.logits, a.type, row * a.logits_row, act, 1, &count, y, (float*)nullptr);
     const bool ok = r.kind != MG_ALLOWED_BITS || ((((const unsigned*)r.allowed)[act >> 5] >> (act & 31)) & 1);
     x = ok ? y[0] : -INFINITY;
   }
@@ -734,7 +796,7 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_join_kernel(mg_logit
   }
 }
 
-template <typename X>
+template <int CHUNKS, typename X>
 __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_wide_backward_kernel(mg_logits a, const int* __restrict__ actions,
                                                                                 const float* __restrict__ entropy,
                                                                                 const double* __restrict__ stats,
@@ -744,36 +806,47 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_wide_backward_kernel
   for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
     HEAD_PART_COUNTS()
     const HeadRow r = head_row(a, row);
+    const HeadScale<X> scale(r.inv_temp);
     const double m = stats[2 * row];
-    const X log_z = (X)stats[2 * row + 1], ent = entropy[row], inv_temp = (X)r.inv_temp;
+    const X log_z = (X)stats[2 * row + 1], past = (X)((double)entropy[row] - stats[2 * row + 1]);  // H + log q = past - t / temperature
     const bool bad = m != m, empty = m == -INFINITY;
     const X top = bad || empty ? (X)0 : (X)m;
     const int act = actions[row];
     X gp = 0;
-    const X gh = dentropy ? dentropy[row] : 0.f;
+    const X gh = (dentropy ? dentropy[row] : 0.f) * scale.inv_temp;
     if (dlog_prob && act >= 0 && act < a.width) {  // the action's token is left if it is allowed and not at -infinity
-      float l[1], b[1] = {0.f};
+      float l[1];
       head_load<1>(a.logits, a.type, row * a.logits_row + act, 1, l);
-      if (r.bias) b[0] = r.bias[act];
-      bool ok = l[0] > -INFINITY && b[0] > -INFINITY;
+      bool ok = l[0] > -INFINITY && (!r.bias || r.bias[act] > -INFINITY);
       if (r.kind == MG_ALLOWED_BOOL) ok = ok && ((const unsigned char*)r.allowed)[act];
       if (r.kind == MG_ALLOWED_BITS) ok = ok && ((((const unsigned*)r.allowed)[act >> 5] >> (act & 31)) & 1);
-      if (ok) gp = dlog_prob[row];
+      if (ok) gp = dlog_prob[row] * scale.inv_temp;
     }
 #pragma unroll
-    for (int c = 0; c < HEAD_CHUNKS; c++) {
+    for (int c = 0; c < CHUNKS; c++) {
       const int at = c * HEAD_CHUNK + threadIdx.x * 8, n = part_n - at;
       if (n <= 0) continue;
       const int v0 = (int)(part0 + at);
-      X x[8];
+      X x[8], g[8];
       float slope[8], y[8];
-      head_columns<8, true>(r, a.logits, a.type, row * a.logits_row, v0, n, counts + at, x, slope);
+      const unsigned ok = head_columns<8, true, std::is_same<X, double>::value>(r, a.logits, a.type, row * a.logits_row, v0, n, counts + at, x, slope);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        const X d = (top - x[e]) * inv_temp, q = head_exp(d + log_z);
-        X g = gp * ((v0 + e == act ? (X)1 : (X)0) - q) + (q > 0 ? gh * q * (d + log_z - ent) : 0);
-        if (bad) g = NAN;
-        y[e] = empty || x[e] == (X)-INFINITY ? 0.f : (float)(g * inv_temp * slope[e]);
+        const X t = top - x[e];
+        g[e] = -scale.weight(t, log_z) * head_fma(gh, past - head_finite(t) * scale.inv_temp, gp);
+      }
+      if ((unsigned)(act - v0) < 8u) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) if (v0 + e == act) g[e] += gp;
+      }
+      if (bad || empty) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) g[e] = bad ? NAN : 0;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        if (std::is_same<X, double>::value) g[e] *= slope[e];
+        y[e] = __uint_as_float(__float_as_uint((float)g[e]) & head_bit(ok, e));
       }
       head_store<8>(dlogits, a.type, row * a.width + v0, n, y);
     }
@@ -797,13 +870,17 @@ static int head_check(const char* who, const mg_logits* a) {
   return 0;
 }
 
-static int head_parts(const mg_logits* a) { return (int)(((int64_t)a->width + HEAD_PART - 1) / HEAD_PART); }
+// A part is four chunks where that leaves enough blocks to fill the GPU, else one.
+static int head_chunks(const mg_logits* a) {
+  return (int64_t)((a->width - 1) / (4 * HEAD_CHUNK) + 1) * a->rows >= 2048 ? 4 : 1;
+}
+static int head_parts(const mg_logits* a) { return (a->width - 1) / (head_chunks(a) * HEAD_CHUNK) + 1; }
 static dim3 head_wide_grid(const mg_logits* a) { return dim3(head_parts(a), (unsigned)(a->rows < 32768 ? a->rows : 32768)); }
 static bool head_narrow(const mg_logits* a) { return a->width <= HEAD_NARROW; }
 
-// lanes per row: as many as hold the row with E columns each
-static HeadNarrow head_layout(const mg_logits* a, int e) {
-  int lanes = 1;
+// lanes per row: as many as hold the row with E columns each; a power of two where they work on it together
+static HeadNarrow head_layout(const mg_logits* a, int e, bool together) {
+  int lanes = together ? 1 : (a->width + e - 1) / e;
   while (lanes * e < a->width) lanes *= 2;
   return HeadNarrow{lanes, HEAD_THREADS / lanes};
 }
@@ -813,10 +890,17 @@ static unsigned head_blocks(int64_t rows, int per_block) {
 }
 
 template <int V> using head_int = std::integral_constant<int, V>;
+template <bool V> using head_bool = std::integral_constant<bool, V>;
 template <typename F>
 static void head_by_width(const mg_logits* a, F f) {
-  if (a->width <= 64 * 8) f(head_int<8>(), head_layout(a, 8));
-  else f(head_int<16>(), head_layout(a, 16));
+  if (a->width <= 8) f(head_int<8>(), head_bool<true>(), head_layout(a, 8, true));
+  else if (a->width <= 64 * 8) f(head_int<8>(), head_bool<false>(), head_layout(a, 8, true));
+  else f(head_int<16>(), head_bool<false>(), head_layout(a, 16, true));
+}
+template <typename F>
+static void head_by_chunks(const mg_logits* a, F f) {
+  if (head_chunks(a) == 4) f(head_int<4>());
+  else f(head_int<1>());
 }
 // the arithmetic of given actions: 64 bits where a bias or a penalty could cancel large logits
 template <typename F>
@@ -842,12 +926,14 @@ extern "C" int64_t mg_logits_workspace(const mg_logits* a) {
 
 static int head_adjust(const char* who, const mg_logits* a, void* out, const void* dout, void* dlogits, void* stream) {
   const hipStream_t s = (hipStream_t)stream;
-  if (head_narrow(a))
-    head_by_width(a, [&](auto e, HeadNarrow g) {
-      hipLaunchKernelGGL(mg_adjust_narrow_kernel<decltype(e)::value>, dim3(head_blocks(a->rows, g.rows)), dim3(HEAD_THREADS), 0, s, *a, g, out, dout, dlogits);
+  if (head_narrow(a)) {
+    const HeadNarrow g = head_layout(a, 8, false);
+    hipLaunchKernelGGL(mg_adjust_narrow_kernel<8>, dim3(head_blocks(a->rows, g.rows)), dim3(HEAD_THREADS), 0, s, *a, g, out, dout, dlogits);
+  } else {
+    head_by_chunks(a, [&](auto c) {
+      hipLaunchKernelGGL(mg_adjust_wide_kernel<decltype(c)::value>, head_wide_grid(a), dim3(HEAD_THREADS), 0, s, *a, out, dout, dlogits);
     });
-  else
-    hipLaunchKernelGGL(mg_adjust_wide_kernel, head_wide_grid(a), dim3(HEAD_THREADS), 0, s, *a, out, dout, dlogits);
+  }
   return head_launched(who);
 }
 
@@ -878,14 +964,18 @@ extern "C" int mg_sample_actions(const mg_logits* a, const float* uniforms, int3
   if (const int rc = head_workspace(who, a)) return rc;
   const hipStream_t s = (hipStream_t)stream;
   if (head_narrow(a)) {
-    head_by_width(a, [&](auto e, HeadNarrow g) {
-      hipLaunchKernelGGL(mg_sample_narrow_kernel<decltype(e)::value>, dim3(head_blocks(a->rows, g.rows)), dim3(HEAD_THREADS), 0, s, *a, g,
+    head_by_width(a, [&](auto e, auto one, HeadNarrow g) {
+      hipLaunchKernelGGL((mg_sample_narrow_kernel<decltype(e)::value, decltype(one)::value>), dim3(head_blocks(a->rows, g.rows)), dim3(HEAD_THREADS), 0, s, *a, g,
                          uniforms, actions, log_prob, entropy);
     });
   } else {
-    hipLaunchKernelGGL(mg_head_parts_kernel<double>, head_wide_grid(a), dim3(HEAD_THREADS), 0, s, *a, (double*)a->workspace);
-    hipLaunchKernelGGL(mg_sample_join_kernel, dim3(head_blocks(a->rows, 1)), dim3(HEAD_THREADS), 0, s, *a, head_parts(a),
-                       (const double*)a->workspace, uniforms, actions, log_prob, entropy);
+    head_by_chunks(a, [&](auto c) {
+      constexpr int C = decltype(c)::value;
+      if (uniforms) hipLaunchKernelGGL((mg_head_parts_kernel<C, false, double>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, *a, (double*)a->workspace);
+      else hipLaunchKernelGGL((mg_head_parts_kernel<C, true, double>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, *a, (double*)a->workspace);
+      hipLaunchKernelGGL(mg_sample_join_kernel<C * HEAD_THREADS>, dim3((unsigned)(a->rows < 1 << 20 ? a->rows : 1 << 20)), dim3(C * HEAD_THREADS), 0, s,
+                         *a, head_parts(a), (const double*)a->workspace, uniforms, actions, log_prob, entropy);
+    });
   }
   return head_launched(who);
 } catch (...) {
@@ -903,12 +993,14 @@ extern "C" int mg_evaluate_actions(const mg_logits* a, const int32_t* actions, f
   head_by_controls(a, [&](auto* null) {
     using X = std::remove_pointer_t<decltype(null)>;
     if (head_narrow(a)) {
-      head_by_width(a, [&](auto e, HeadNarrow g) {
-        hipLaunchKernelGGL((mg_evaluate_narrow_kernel<decltype(e)::value, X>), dim3(head_blocks(a->rows, g.rows)), dim3(HEAD_THREADS), 0, s,
+      head_by_width(a, [&](auto e, auto one, HeadNarrow g) {
+        hipLaunchKernelGGL((mg_evaluate_narrow_kernel<decltype(e)::value, decltype(one)::value, X>), dim3(head_blocks(a->rows, g.rows)), dim3(HEAD_THREADS), 0, s,
                            *a, g, actions, log_prob, entropy);
       });
     } else {
-      hipLaunchKernelGGL(mg_head_parts_kernel<X>, head_wide_grid(a), dim3(HEAD_THREADS), 0, s, *a, (double*)a->workspace);
+      head_by_chunks(a, [&](auto c) {
+        hipLaunchKernelGGL((mg_head_parts_kernel<decltype(c)::value, false, X>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, *a, (double*)a->workspace);
+      });
     }
   });
   if (!head_narrow(a))
@@ -930,13 +1022,15 @@ extern "C" int mg_evaluate_actions_backward(const mg_logits* a, const int32_t* a
   head_by_controls(a, [&](auto* null) {
     using X = std::remove_pointer_t<decltype(null)>;
     if (head_narrow(a))
-      head_by_width(a, [&](auto e, HeadNarrow g) {
-        hipLaunchKernelGGL((mg_evaluate_narrow_backward_kernel<decltype(e)::value, X>), dim3(head_blocks(a->rows, g.rows)), dim3(HEAD_THREADS),
+      head_by_width(a, [&](auto e, auto one, HeadNarrow g) {
+        hipLaunchKernelGGL((mg_evaluate_narrow_backward_kernel<decltype(e)::value, decltype(one)::value, X>), dim3(head_blocks(a->rows, g.rows)), dim3(HEAD_THREADS),
                            0, s, *a, g, actions, dlog_prob, dentropy, dlogits);
       });
     else
-      hipLaunchKernelGGL(mg_evaluate_wide_backward_kernel<X>, head_wide_grid(a), dim3(HEAD_THREADS), 0, s, *a, actions, entropy, stats,
-                         dlog_prob, dentropy, dlogits);
+      head_by_chunks(a, [&](auto c) {
+        hipLaunchKernelGGL((mg_evaluate_wide_backward_kernel<decltype(c)::value, X>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, *a, actions,
+                           entropy, stats, dlog_prob, dentropy, dlogits);
+      });
   });
   return head_launched(who);
 } catch (...) {
