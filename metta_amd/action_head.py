@@ -52,7 +52,7 @@ class _Head:
 
     __slots__ = ("logits", "bias", "allowed", "history", "args", "lead")
 
-    def __init__(self, logits, allowed, bias, history, temperature, repetition, presence, frequency):
+    def __init__(self, logits, allowed, bias, history, temperature, repetition, presence, frequency, gradient=True):
         if logits.dim() < 1 or logits.size(-1) < 1:
             raise RuntimeError("logits must be [..., V] with at least one token")
         if logits.dtype not in TYPES:
@@ -78,7 +78,7 @@ class _Head:
         if bias is not None:
             if bias.dtype != torch.float32:
                 raise RuntimeError("bias must be float32")
-            if bias.requires_grad and torch.is_grad_enabled():
+            if gradient and bias.requires_grad and torch.is_grad_enabled():
                 raise RuntimeError("bias is a constant: it must not require a gradient")
         if history is not None:
             if history.dtype != torch.int32:
@@ -225,7 +225,6 @@ def adjust_logits(
     return _AdjustLogits.apply(logits, _Head(logits, allowed, bias, history, temperature, repetition, presence, frequency))
 
 
-@torch.no_grad()
 def sample_actions(
     logits: Tensor,
     uniforms: Optional[Tensor] = None,
@@ -244,7 +243,7 @@ def sample_actions(
     running sum of the probabilities exceeds the uniform, as 64-bit arithmetic finds it: the same numbers give the same
     actions whatever the shape of the batch.  Without, it is the most likely token (the lowest of equals).  Carries no
     gradient; `evaluate_actions` does."""
-    head = _Head(logits, allowed, bias, history, temperature, repetition, presence, frequency)
+    head = _Head(logits, allowed, bias, history, temperature, repetition, presence, frequency, gradient=False)
     if uniforms is not None:
         uniforms = _per_row("uniforms", uniforms, (torch.float32,), head.lead, logits.device)
     actions = torch.empty(head.lead, dtype=torch.int32, device=logits.device)

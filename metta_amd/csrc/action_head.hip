@@ -38,30 +38,6 @@ extern int mg_fail_msg(const std::string& m);  // mettagrid_hip.hip: sets mg_las
 // ---- elements: the tensors' type is a scalar branch around the loads and stores ---------------------------------------
 
 template <int E>
-__device__ __forceinline__ void head_load(const void* p, int type, long at, int n, float* out) {
-  if (type == MG_F32) {
-    const float* q = (const float*)p + at;
-    if (n >= E) {
-      __builtin_memcpy(out, q, 4 * E);  // (rows of any width: the start is aligned to an element only)
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; e++) out[e] = e < n ? q[e] : 0.f;
-    }
-    return;
-  }
-  const unsigned short* q = (const unsigned short*)p + at;
-  unsigned short raw[E];
-  if (n >= E) {
-    __builtin_memcpy(raw, q, 2 * E);
-  } else {
-#pragma unroll
-    for (int e = 0; e < E; e++) raw[e] = e < n ? q[e] : (unsigned short)0;
-  }
-#pragma unroll
-  for (int e = 0; e < E; e++) out[e] = type == MG_BF16 ? __uint_as_float((unsigned)raw[e] << 16) : (float)__builtin_bit_cast(_Float16, raw[e]);
-}
-
-template <int E>
 __device__ __forceinline__ void head_store(void* p, int type, long at, int n, const float* x) {
   if (type == MG_F32) {
     float* q = (float*)p + at;
@@ -75,8 +51,13 @@ __device__ __forceinline__ void head_store(void* p, int type, long at, int n, co
   }
   unsigned short* q = (unsigned short*)p + at;
   unsigned short raw[E];
+  if (type == MG_BF16) {
 #pragma unroll
-  for (int e = 0; e < E; e++) raw[e] = type == MG_BF16 ? __builtin_bit_cast(unsigned short, (__bf16)x[e]) : __builtin_bit_cast(unsigned short, (_Float16)x[e]);
+    for (int e = 0; e < E; e++) raw[e] = __builtin_bit_cast(unsigned short, (__bf16)x[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; e++) raw[e] = __builtin_bit_cast(unsigned short, (_Float16)x[e]);
+  }
   if (n >= E) {
     __builtin_memcpy(q, raw, 2 * E);
   } else {
@@ -109,19 +90,56 @@ __device__ __forceinline__ double head_exp(double d) {
   return d > 746.0 ? 0.0 : ldexp(p, (int)n);  // (the smallest denormal is e^-745)
 }
 
+// 1 / z; in 32 bits by the hardware's reciprocal and one Newton step
+__device__ __forceinline__ double head_inverse(double z) { return 1.0 / z; }
+__device__ __forceinline__ float head_inverse(float z) {
+  const float r = __builtin_amdgcn_rcpf(z);
+  return fmaf(fmaf(-z, r, 1.0f), r, r);
+}
+__device__ __forceinline__ double head_log(double z) { return log(z); }
+__device__ __forceinline__ float head_log(float z) { return logf(z); }
+
+// The call's arguments, with the quotients that every row wants (a 64-bit division costs a wave as much as a dozen tokens).
+struct HeadArgs : mg_logits {
+  double inv_temp, inv_rep;
+  float weight_scale;  // -log2 e / temperature
+};
+
+// One row's controls.
+struct HeadRow {
+  const float* bias;
+  const void* allowed;
+  int kind;
+  bool counted;
+  double inv_rep, rep, presence, frequency, inv_temp;
+  float weight_scale;
+};
+
+__device__ __forceinline__ HeadRow head_row(const HeadArgs& a, long row) {
+  HeadRow r;
+  r.bias = a.bias ? a.bias + row * a.bias_row : nullptr;
+  r.kind = a.allowed ? a.allowed_kind : 0;
+  r.allowed = !a.allowed ? nullptr : r.kind == MG_ALLOWED_BOOL ? (const void*)((const unsigned char*)a.allowed + row * a.allowed_row)
+                                                               : (const void*)((const int*)a.allowed + row * a.allowed_row);
+  r.counted = a.history != nullptr;
+  r.rep = a.repetition; r.inv_rep = a.inv_rep;
+  r.presence = a.presence; r.frequency = a.frequency; r.inv_temp = a.inv_temp; r.weight_scale = a.weight_scale;
+  return r;
+}
+
 // What a row's exponentials and gradients are scaled by: weight(t) = exp(-t / temperature) for t = M - x.  In 32 bits the
 // scale and log2 e are one factor, and the hardware's exp2 does the rest: the difference, the factor and the product
 // round once each, 3 u t / temperature relative, plus the 2 u of exp2.
 template <typename X> struct HeadScale;
 template <> struct HeadScale<double> {
   double inv_temp;
-  __device__ explicit HeadScale(double i) : inv_temp(i) {}
+  __device__ explicit HeadScale(const HeadRow& r) : inv_temp(r.inv_temp) {}
   __device__ __forceinline__ double weight(double t) const { return head_exp(t * inv_temp); }
   __device__ __forceinline__ double weight(double t, double log_z) const { return head_exp(t * inv_temp + log_z); }
 };
 template <> struct HeadScale<float> {
   float inv_temp, k;
-  __device__ explicit HeadScale(double i) : inv_temp((float)i), k((float)(i * -1.4426950408889634)) {}
+  __device__ explicit HeadScale(const HeadRow& r) : inv_temp((float)r.inv_temp), k(r.weight_scale) {}
   __device__ __forceinline__ float weight(float t) const { return __builtin_amdgcn_exp2f(t * k); }
   __device__ __forceinline__ float weight(float t, float log_z) const { return __builtin_amdgcn_exp2f(fmaf(t, k, log_z * -1.44269504f)); }
 };
@@ -132,92 +150,158 @@ __device__ __forceinline__ float head_max(float a, float b) { return fmaxf(a, b)
 // t kept finite: its weight is 0 long before, and 0 * t has to be 0
 __device__ __forceinline__ double head_finite(double t) { return fmin(t, 1e300); }
 __device__ __forceinline__ float head_finite(float t) { return fminf(t, 1e37f); }
-__device__ __forceinline__ double head_log(double z) { return log(z); }
-__device__ __forceinline__ float head_log(float z) { return logf(z); }
 
-// One row's controls.
-struct HeadRow {
-  const float* bias;
-  const void* allowed;
-  int kind;
-  bool counted;
-  double inv_rep, rep, presence, frequency, inv_temp;
-};
-
-__device__ __forceinline__ HeadRow head_row(const mg_logits& a, long row) {
-  HeadRow r;
-  r.bias = a.bias ? a.bias + row * a.bias_row : nullptr;
-  r.kind = a.allowed ? a.allowed_kind : 0;
-  r.allowed = !a.allowed ? nullptr : r.kind == MG_ALLOWED_BOOL ? (const void*)((const unsigned char*)a.allowed + row * a.allowed_row)
-                                                               : (const void*)((const int*)a.allowed + row * a.allowed_row);
-  r.counted = a.history != nullptr;
-  r.rep = a.repetition; r.inv_rep = 1.0 / a.repetition;
-  r.presence = a.presence; r.frequency = a.frequency; r.inv_temp = 1.0 / a.temperature;
-  return r;
-}
-
-// bit e: column v0 + e is allowed, e < n
-template <int E>
-__device__ __forceinline__ unsigned head_allowed(const HeadRow& r, int v0, int n) {
-  static_assert(E <= 16, "bits of one half word");
-  if (n <= 0) return 0;
-  const unsigned inside = n >= E ? (1u << E) - 1 : (1u << n) - 1;
-  if (r.kind == MG_ALLOWED_BITS) return (((const unsigned*)r.allowed)[v0 >> 5] >> (v0 & 31)) & inside;  // (E divides 32)
-  if (r.kind == MG_ALLOWED_BOOL) {
-    const unsigned char* p = (const unsigned char*)r.allowed + v0;
-    unsigned bits = 0;
-    if (n >= E) {
-      unsigned b[(E + 3) / 4];
-      __builtin_memcpy(b, p, E);
-#pragma unroll
-      for (int e = 0; e < E; e++) bits |= ((b[e / 4] >> (8 * (e % 4))) & 0xFFu) ? 1u << e : 0u;
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; e++) if (e < n) bits |= p[e] ? 1u << e : 0u;
-    }
-    return bits;
-  }
-  return inside;
+__device__ __forceinline__ bool head_allowed(const HeadRow& r, int v) {
+  if (r.kind == MG_ALLOWED_BITS) return (((const unsigned*)r.allowed)[v >> 5] >> (v & 31)) & 1;
+  return r.kind != MG_ALLOWED_BOOL || ((const unsigned char*)r.allowed)[v] != 0;
 }
 
 // bit e of `bits` over a whole word
 __device__ __forceinline__ unsigned head_bit(unsigned bits, int e) { return (unsigned)((int)(bits << (31 - e)) >> 31); }
 
-// E adjacent columns from v0 on, n of them in the row: x, and (GRAD) what a gradient of x is multiplied by besides 1 /
-// temperature (0 where masked; only where ADJUST, else the bits tell).  counts: of these columns in the history.
-// ADJUST: whether there may be a bias or a history at all.  Returns the bits of the allowed columns.
-template <int E, bool GRAD, bool ADJUST, typename X>
-__device__ __forceinline__ unsigned head_columns(const HeadRow& r, const void* logits, int type, long at, int v0, int n,
-                                                 const unsigned* counts, X* x, float* slope) {
-  float l[E];
-  head_load<E>(logits, type, at + v0, n, l);
-  const unsigned ok = head_allowed<E>(r, v0, n);
+// N words from an address that is aligned to an element of its tensor only
+template <int N>
+__device__ __forceinline__ void head_words(const void* p, unsigned* out) {
+  typedef unsigned four __attribute__((ext_vector_type(4), aligned(1)));
+  typedef unsigned two __attribute__((ext_vector_type(2), aligned(1)));
+  static_assert(N == 2 || N % 4 == 0, "whole vectors");
+  if constexpr (N == 2) {
+    const two w = *(const two*)p;
+    out[0] = w.x, out[1] = w.y;
+  } else {
 #pragma unroll
-  for (int e = 0; e < E; e++) {
-    const unsigned in = head_bit(ok, e);
-    x[e] = (X)__uint_as_float((__float_as_uint(l[e]) & in) | (0xFF800000u & ~in));  // masked: -infinity
+    for (int i = 0; i < N; i += 4) {
+      const four w = ((const four*)p)[i / 4];
+      out[i] = w.x, out[i + 1] = w.y, out[i + 2] = w.z, out[i + 3] = w.w;
+    }
   }
-  if (!ADJUST) return ok;
-  if (r.counted) {
+}
+
+// E adjacent columns of a row as they lie in memory, on their way: what is fetched for several groups of columns before
+// the first is looked at waits for the memory once.  FULL: all E columns are in the row, for every lane.
+template <int E>
+struct HeadRaw {
+  unsigned logits[E], allowed[(E + 3) / 4];
+  float bias[E];
+
+  // logits of `type` (null: not wanted) at element `at` of the tensor; columns v0 ... of the row's controls.  (Every path
+  // sets every word: stores to places that differ from path to path would keep the struct out of registers.)
+  template <bool FULL, bool BIAS>
+  __device__ __forceinline__ void fetch(const HeadRow& r, const void* p, int type, long at, int v0, int n) {
+    static_assert(E <= 16, "mask bits of one half word");
+#pragma unroll
+    for (int e = 0; e < E; e++) logits[e] = 0;
+    if (p) {
+      if (type == MG_F32) words<FULL>((const unsigned*)p + at, n, logits);
+      else halves<FULL>((const unsigned short*)p + at, n, logits);
+    }
+#pragma unroll
+    for (int e = 0; e < (E + 3) / 4; e++) allowed[e] = 0;
+    if (r.kind == MG_ALLOWED_BITS) allowed[0] = FULL || n > 0 ? ((const unsigned*)r.allowed)[v0 >> 5] : 0u;
+    if (r.kind == MG_ALLOWED_BOOL) bytes<FULL>((const unsigned char*)r.allowed + v0, n, allowed);
+    if constexpr (BIAS) {
+      unsigned b[E];
+#pragma unroll
+      for (int e = 0; e < E; e++) b[e] = 0;
+      if (r.bias) words<FULL>((const unsigned*)(r.bias + v0), n, b);
+#pragma unroll
+      for (int e = 0; e < E; e++) bias[e] = __uint_as_float(b[e]);
+    }
+  }
+  template <bool FULL>
+  static __device__ __forceinline__ void words(const unsigned* p, int n, unsigned* out) {
+    if (E > 1 && (FULL || n >= E)) {
+      if constexpr (E > 1) head_words<E>(p, out);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; e++) out[e] = e < n ? p[e] : 0u;
+    }
+  }
+  template <bool FULL>
+  static __device__ __forceinline__ void halves(const unsigned short* p, int n, unsigned* out) {
+    if (E > 1 && (FULL || n >= E)) {
+      if constexpr (E > 1) head_words<E / 2>(p, out);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        const unsigned lo = e < n ? p[e] : 0u, hi = e + 1 < n ? p[e + 1] : 0u;
+        out[e / 2] = lo | hi << 16;
+      }
+    }
+  }
+  template <bool FULL>
+  static __device__ __forceinline__ void bytes(const unsigned char* p, int n, unsigned* out) {
+    if (E > 1 && (FULL || n >= E)) {
+      if constexpr (E > 1) head_words<E / 4>(p, out);
+    } else {
+#pragma unroll
+      for (int w = 0; w < (E + 3) / 4; w++) {
+        unsigned b = 0;
+#pragma unroll
+        for (int e = 4 * w; e < E && e < 4 * w + 4; e++) b |= (e < n ? (unsigned)p[e] : 0u) << (8 * (e % 4));
+        out[w] = b;
+      }
+    }
+  }
+
+  __device__ __forceinline__ void values(int type, float* l) const {
+    if (type == MG_F32) {
+#pragma unroll
+      for (int e = 0; e < E; e++) l[e] = __uint_as_float(logits[e]);
+    } else if (type == MG_BF16) {
+#pragma unroll
+      for (int e = 0; e < E; e++) l[e] = __uint_as_float(e % 2 ? logits[e / 2] & 0xFFFF0000u : logits[e / 2] << 16);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; e++) l[e] = (float)__builtin_bit_cast(_Float16, (unsigned short)(e % 2 ? logits[e / 2] >> 16 : logits[e / 2]));
+    }
+  }
+
+  // bit e: column e is in the row (of which n are left) and allowed
+  __device__ __forceinline__ unsigned bits(const HeadRow& r, int v0, int n) const {
+    if (n <= 0) return 0;
+    const unsigned inside = n >= E ? (1u << E) - 1 : (1u << n) - 1;
+    if (r.kind == MG_ALLOWED_BITS) return (allowed[0] >> (v0 & 31)) & inside;  // (E divides 32 and v0)
+    if (r.kind != MG_ALLOWED_BOOL) return inside;
+    unsigned b = 0;
+#pragma unroll
+    for (int e = 0; e < E; e++) b |= (allowed[e / 4] & (0xFFu << (8 * (e % 4)))) ? 1u << e : 0u;
+    return b & inside;
+  }
+
+  // x, and (GRAD) what a gradient of x is multiplied by besides 1 / temperature: 0 where masked, and only where ADJUST,
+  // else the bits tell.  ADJUST: whether there may be a bias or a history at all.  counts: these columns in the history.
+  // Returns bits().
+  template <bool GRAD, bool ADJUST, typename X>
+  __device__ __forceinline__ unsigned columns(const HeadRow& r, int type, int v0, int n, const unsigned* counts, X* x, float* slope) const {
+    float l[E];
+    values(type, l);
+    const unsigned ok = bits(r, v0, n);
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      const unsigned c = counts[e];
-      const X y = (x[e] > 0 ? x[e] * r.inv_rep : x[e] * r.rep) - r.frequency * c - r.presence;
-      if (GRAD) slope[e] = !head_bit(ok, e) ? 0.f : c ? (float)(x[e] > 0 ? r.inv_rep : r.rep) : 1.f;
-      x[e] = c ? y : x[e];
+      const unsigned in = head_bit(ok, e);
+      x[e] = (X)__uint_as_float((__float_as_uint(l[e]) & in) | (0xFF800000u & ~in));  // masked: -infinity
     }
-  } else if (GRAD) {
+    if (!ADJUST) return ok;
+    if (r.counted) {
 #pragma unroll
-    for (int e = 0; e < E; e++) slope[e] = head_bit(ok, e) ? 1.f : 0.f;
-  }
-  if (r.bias) {
-    float b[E];
-    head_load<E>(r.bias, MG_F32, v0, n, b);
+      for (int e = 0; e < E; e++) {
+        const unsigned c = counts[e];
+        const X y = (x[e] > 0 ? x[e] * r.inv_rep : x[e] * r.rep) - r.frequency * c - r.presence;
+        if (GRAD) slope[e] = !head_bit(ok, e) ? 0.f : c ? (float)(x[e] > 0 ? r.inv_rep : r.rep) : 1.f;
+        x[e] = c ? y : x[e];
+      }
+    } else if (GRAD) {
 #pragma unroll
-    for (int e = 0; e < E; e++) x[e] += __uint_as_float(__float_as_uint(b[e]) & head_bit(ok, e));
+      for (int e = 0; e < E; e++) slope[e] = head_bit(ok, e) ? 1.f : 0.f;
+    }
+    if (r.bias) {
+#pragma unroll
+      for (int e = 0; e < E; e++) x[e] += __uint_as_float(__float_as_uint(bias[e]) & head_bit(ok, e));
+    }
+    return ok;
   }
-  return ok;
-}
+};
 
 // ---- lanes ------------------------------------------------------------------------------------------------------------
 
@@ -253,33 +337,45 @@ __device__ __forceinline__ double head_group_before(double x, int lanes, int lan
   return sum - x;
 }
 
-// adjusted logits of E columns, or their gradient
+// adjusted logits of E columns, or their gradient, from what was fetched (for a gradient with a history: the logits and the
+// outer gradient; without: the outer gradient alone, on which the logits have no influence)
 template <int E>
-__device__ __forceinline__ void head_adjust_columns(const mg_logits& a, const HeadRow& r, long row, int v0, int n, const unsigned* counts,
-                                                    void* out, const void* dout, void* dlogits) {
-  double x[E];
-  float slope[E], y[E];
-  if (out) {
-    head_columns<E, false, true>(r, a.logits, a.type, row * a.logits_row, v0, n, counts, x, slope);
+struct HeadAdjust {
+  HeadRaw<E> raw, outer;
+
+  template <bool FULL>
+  __device__ __forceinline__ void fetch(const HeadArgs& a, const HeadRow& r, long row, int v0, int n, const void* dout) {
+    raw.template fetch<FULL, true>(r, !dout || r.counted ? a.logits : nullptr, a.type, row * a.logits_row + v0, v0, n);
+    if (dout) {
+      HeadRow plain = r;
+      plain.kind = 0;
+      outer.template fetch<FULL, false>(plain, dout, a.type, row * a.width + v0, v0, n);
+    }
+  }
+  __device__ __forceinline__ void store(const HeadArgs& a, const HeadRow& r, long row, int v0, int n, const unsigned* counts, void* out,
+                                        const void* dout, void* dlogits) const {
+    double x[E];
+    float slope[E], y[E];
+    if (!dout) {
+      raw.template columns<false, true>(r, a.type, v0, n, counts, x, slope);
 #pragma unroll
-    for (int e = 0; e < E; e++) y[e] = (float)(x[e] * r.inv_temp);
-    head_store<E>(out, a.type, row * a.width + v0, n, y);
-  } else if (r.counted) {
-    float go[E];
-    head_columns<E, true, true>(r, a.logits, a.type, row * a.logits_row, v0, n, counts, x, slope);
-    head_load<E>(dout, a.type, row * a.width + v0, n, go);
+      for (int e = 0; e < E; e++) y[e] = (float)(x[e] * r.inv_temp);
+      head_store<E>(out, a.type, row * a.width + v0, n, y);
+      return;
+    }
+    outer.values(a.type, y);
+    if (r.counted) {
+      raw.template columns<true, true>(r, a.type, v0, n, counts, x, slope);
 #pragma unroll
-    for (int e = 0; e < E; e++) y[e] = slope[e] == 0.f ? 0.f : (float)((double)go[e] * (slope[e] * r.inv_temp));
-    head_store<E>(dlogits, a.type, row * a.width + v0, n, y);
-  } else {  // without penalties the gradient does not depend on the logits: they are not read
-    float go[E];
-    const unsigned ok = head_allowed<E>(r, v0, n);
-    head_load<E>(dout, a.type, row * a.width + v0, n, go);
+      for (int e = 0; e < E; e++) y[e] = slope[e] == 0.f ? 0.f : (float)((double)y[e] * (slope[e] * r.inv_temp));
+    } else {
+      const unsigned ok = raw.bits(r, v0, n);
 #pragma unroll
-    for (int e = 0; e < E; e++) y[e] = __uint_as_float(__float_as_uint((float)(go[e] * r.inv_temp)) & head_bit(ok, e));
+      for (int e = 0; e < E; e++) y[e] = __uint_as_float(__float_as_uint((float)(y[e] * r.inv_temp)) & head_bit(ok, e));
+    }
     head_store<E>(dlogits, a.type, row * a.width + v0, n, y);
   }
-}
+};
 
 // ---- narrow rows ------------------------------------------------------------------------------------------------------
 
@@ -288,7 +384,7 @@ struct HeadNarrow { int lanes, rows; };  // lanes per row, rows per block
 // counts[row * lanes + lane][e] over the block's rows, all threads together, eight entries on their way at a time;
 // barriers inside
 template <int E>
-__device__ __forceinline__ void head_count_rows(const mg_logits& a, const HeadNarrow& g, long row0, unsigned (*counts)[E + 1]) {
+__device__ __forceinline__ void head_count_rows(const HeadArgs& a, const HeadNarrow& g, long row0, unsigned (*counts)[E + 1]) {
   __syncthreads();
 #pragma unroll
   for (int e = 0; e < E; e++) counts[threadIdx.x][e] = 0;
@@ -325,7 +421,7 @@ struct HeadHeld {
   int lane, v0, n;  // this lane's columns, n of them (or fewer than one) in the row
   bool bad, empty, mine;  // mine: the row is this group's own
 
-  __device__ __forceinline__ void place(const mg_logits& a, const HeadNarrow& g, long row0) {
+  __device__ __forceinline__ void place(const HeadArgs& a, const HeadNarrow& g, long row0) {
     const long at = row0 + (ONE ? threadIdx.x : threadIdx.x / g.lanes);
     lane = ONE ? 0 : threadIdx.x % g.lanes;
     mine = at < a.rows && (ONE || (int)threadIdx.x < g.rows * g.lanes);
@@ -335,8 +431,11 @@ struct HeadHeld {
   }
 
   template <bool GRAD>
-  __device__ __forceinline__ void hold(const mg_logits& a, const HeadNarrow& g, const HeadRow& r, const HeadScale<X>& scale, const unsigned* counts) {
-    ok = head_columns<E, GRAD, std::is_same<X, double>::value>(r, a.logits, a.type, row * a.logits_row, v0, n, counts, x, slope);
+  __device__ __forceinline__ void hold(const HeadArgs& a, const HeadNarrow& g, const HeadRow& r, const HeadScale<X>& scale, const unsigned* counts) {
+    constexpr bool adjust = std::is_same<X, double>::value;
+    HeadRaw<E> raw;
+    raw.template fetch<false, adjust>(r, a.logits, a.type, row * a.logits_row + v0, v0, n);
+    ok = raw.template columns<GRAD, adjust>(r, a.type, v0, n, counts, x, slope);
     m = x[0];
 #pragma unroll
     for (int e = 1; e < E; e++) m = head_max(m, x[e]);
@@ -367,7 +466,7 @@ struct HeadHeld {
 };
 
 template <int E>
-__global__ __launch_bounds__(HEAD_THREADS) void mg_adjust_narrow_kernel(mg_logits a, HeadNarrow g, void* __restrict__ out,
+__global__ __launch_bounds__(HEAD_THREADS) void mg_adjust_narrow_kernel(HeadArgs a, HeadNarrow g, void* __restrict__ out,
                                                                        const void* __restrict__ dout, void* __restrict__ dlogits) {
   __shared__ unsigned counts[HEAD_THREADS][E + 1];
   for (long row0 = (long)blockIdx.x * g.rows; row0 < a.rows; row0 += (long)gridDim.x * g.rows) {
@@ -376,12 +475,14 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_adjust_narrow_kernel(mg_logit
     h.place(a, g, row0);
     if (!h.mine) continue;
     const HeadRow r = head_row(a, h.row);
-    head_adjust_columns<E>(a, r, h.row, h.v0, h.n, counts[threadIdx.x], out, dout, dlogits);
+    HeadAdjust<E> it;
+    it.template fetch<false>(a, r, h.row, h.v0, h.n, dout);
+    it.store(a, r, h.row, h.v0, h.n, counts[threadIdx.x], out, dout, dlogits);
   }
 }
 
 template <int E, bool ONE>
-__global__ __launch_bounds__(HEAD_THREADS) void mg_sample_narrow_kernel(mg_logits a, HeadNarrow g, const float* __restrict__ uniforms,
+__global__ __launch_bounds__(HEAD_THREADS) void mg_sample_narrow_kernel(HeadArgs a, HeadNarrow g, const float* __restrict__ uniforms,
                                                                        int* __restrict__ actions, float* __restrict__ log_prob,
                                                                        float* __restrict__ entropy) {
   __shared__ unsigned counts[HEAD_THREADS][E + 1];
@@ -390,7 +491,7 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_sample_narrow_kernel(mg_logit
     HeadHeld<E, ONE, double> h;
     h.place(a, g, row0);
     const HeadRow r = head_row(a, h.row);
-    const HeadScale<double> scale(r.inv_temp);
+    const HeadScale<double> scale(r);
     h.template hold<false>(a, g, r, scale, counts[threadIdx.x]);
     int hit = a.width, last = -1;
     if (uniforms) {
@@ -421,13 +522,13 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_sample_narrow_kernel(mg_logit
       const double log_z = head_log(h.z);
       actions[h.row] = h.bad || h.empty ? -1 : hit;
       log_prob[h.row] = h.bad ? NAN : h.empty ? 0.f : (float)(-t * scale.inv_temp - log_z);
-      entropy[h.row] = h.bad ? NAN : h.empty ? 0.f : (float)(log_z + h.s / h.z);
+      entropy[h.row] = h.bad ? NAN : h.empty ? 0.f : (float)(log_z + h.s * head_inverse(h.z));
     }
   }
 }
 
 template <int E, bool ONE, typename X>
-__global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_kernel(mg_logits a, HeadNarrow g, const int* __restrict__ actions,
+__global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_kernel(HeadArgs a, HeadNarrow g, const int* __restrict__ actions,
                                                                          float* __restrict__ log_prob, float* __restrict__ entropy) {
   __shared__ unsigned counts[HEAD_THREADS][E + 1];
   for (long row0 = (long)blockIdx.x * g.rows; row0 < a.rows; row0 += (long)gridDim.x * g.rows) {
@@ -435,7 +536,7 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_kernel(mg_log
     HeadHeld<E, ONE, X> h;
     h.place(a, g, row0);
     const HeadRow r = head_row(a, h.row);
-    const HeadScale<X> scale(r.inv_temp);
+    const HeadScale<X> scale(r);
     const int act = actions[h.row];
     h.template hold<false>(a, g, r, scale, counts[threadIdx.x]);
     X d = INFINITY;
@@ -445,13 +546,13 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_kernel(mg_log
     if (h.mine && h.lane == 0) {
       const X log_z = head_log(h.z);
       log_prob[h.row] = h.bad ? NAN : h.empty ? 0.f : (float)(-d - log_z);
-      entropy[h.row] = h.bad ? NAN : h.empty ? 0.f : (float)(log_z + h.s / h.z);
+      entropy[h.row] = h.bad ? NAN : h.empty ? 0.f : (float)(log_z + h.s * head_inverse(h.z));
     }
   }
 }
 
 template <int E, bool ONE, typename X>
-__global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_backward_kernel(mg_logits a, HeadNarrow g, const int* __restrict__ actions,
+__global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_backward_kernel(HeadArgs a, HeadNarrow g, const int* __restrict__ actions,
                                                                                   const float* __restrict__ dlog_prob,
                                                                                   const float* __restrict__ dentropy,
                                                                                   void* __restrict__ dlogits) {
@@ -461,7 +562,7 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_backward_kern
     HeadHeld<E, ONE, X> h;
     h.place(a, g, row0);
     const HeadRow r = head_row(a, h.row);
-    const HeadScale<X> scale(r.inv_temp);
+    const HeadScale<X> scale(r);
     const int act = actions[h.row];
     const X gp_row = dlog_prob ? dlog_prob[h.row] : 0.f, gh = (dentropy ? dentropy[h.row] : 0.f) * scale.inv_temp;
     h.template hold<true>(a, g, r, scale, counts[threadIdx.x]);
@@ -469,7 +570,8 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_backward_kern
 #pragma unroll
     for (int e = 0; e < E; e++) left = left || (h.v0 + e == act && e < h.n && h.x[e] > (X)-INFINITY);
     if (!ONE) left = head_group_max((int)left, g.lanes) != 0;
-    const X gp = left ? gp_row * scale.inv_temp : (X)0, inv_z = 1 / h.z;
+    // (a bad row's NaN reaches every token that is left)
+    const X gp = h.bad ? (X)NAN : left ? gp_row * scale.inv_temp : (X)0, inv_z = head_inverse(h.z);
     const X past = h.s * inv_z;  // H - log Z: H + log q = past - t / temperature
     float y[E];
 #pragma unroll
@@ -478,7 +580,7 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_backward_kern
       const X q = h.w[e] * inv_z;
       X d = (h.v0 + e == act ? gp : (X)0) - q * head_fma(gh, past - h.t[e] * scale.inv_temp, gp);
       if (std::is_same<X, double>::value) d *= h.slope[e];
-      y[e] = h.empty || !(h.x[e] != (X)-INFINITY) ? 0.f : h.bad ? NAN : (float)d;
+      y[e] = h.x[e] != (X)-INFINITY ? (float)d : 0.f;
     }
     if (h.mine) head_store<E>(dlogits, a.type, h.row * a.width + h.v0, h.n, y);
   }
@@ -488,7 +590,7 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_backward_kern
 // Thread t of a block holds columns 8 t ... 8 t + 7 of each of its part's chunks.
 
 // counts of the n columns from v0 on, all threads together; barriers inside
-__device__ __forceinline__ void head_count_columns(const mg_logits& a, long row, unsigned* counts, long v0, int n) {
+__device__ __forceinline__ void head_count_columns(const HeadArgs& a, long row, unsigned* counts, long v0, int n) {
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += HEAD_THREADS) counts[i] = 0;
   __syncthreads();
@@ -580,35 +682,56 @@ __device__ __forceinline__ double head_block_before(double x, double* red, doubl
   const int part_n = (int)min((long)CHUNKS * HEAD_CHUNK, a.width - part0);                      \
   if (a.history) head_count_columns(a, row, counts, part0, part_n);
 
+// `fetch` for every chunk c of the part, whose columns of this thread start at `at` with n of them left; FULL says whether
+// the part lies in the row as a whole
+#define HEAD_PART_FETCH(fetch)                                                                  \
+  if (part_n == CHUNKS * HEAD_CHUNK) {                                                          \
+    constexpr bool FULL = true;                                                                 \
+    _Pragma("unroll") for (int c = 0; c < CHUNKS; c++) {                                        \
+      const int at = c * HEAD_CHUNK + threadIdx.x * 8, n = 8;                                   \
+      fetch;                                                                                    \
+    }                                                                                           \
+  } else {                                                                                      \
+    constexpr bool FULL = false;                                                                \
+    _Pragma("unroll") for (int c = 0; c < CHUNKS; c++) {                                        \
+      const int at = c * HEAD_CHUNK + threadIdx.x * 8, n = part_n - at;                         \
+      fetch;                                                                                    \
+    }                                                                                           \
+  }
+
 template <int CHUNKS>
-__global__ __launch_bounds__(HEAD_THREADS) void mg_adjust_wide_kernel(mg_logits a, void* __restrict__ out, const void* __restrict__ dout,
+__global__ __launch_bounds__(HEAD_THREADS) void mg_adjust_wide_kernel(HeadArgs a, void* __restrict__ out, const void* __restrict__ dout,
                                                                      void* __restrict__ dlogits) {
   for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
     HEAD_PART_COUNTS()
     const HeadRow r = head_row(a, row);
+    HeadAdjust<8> it[CHUNKS];
+    HEAD_PART_FETCH(it[c].template fetch<FULL>(a, r, row, (int)(part0 + at), n, dout))
 #pragma unroll
     for (int c = 0; c < CHUNKS; c++) {
       const int at = c * HEAD_CHUNK + threadIdx.x * 8, n = part_n - at;
-      if (n > 0) head_adjust_columns<8>(a, r, row, (int)(part0 + at), n, counts + at, out, dout, dlogits);
+      if (n > 0) it[c].store(a, r, row, (int)(part0 + at), n, counts + at, out, dout, dlogits);
     }
   }
 }
 
 // what a part knows: found[row][part] = M, Z, sum (M - x) exp(-d) / temperature (against its own M), bad, first column of M
 template <int CHUNKS, bool FIRST, typename X>
-__global__ __launch_bounds__(HEAD_THREADS) void mg_head_parts_kernel(mg_logits a, double* __restrict__ found) {
+__global__ __launch_bounds__(HEAD_THREADS) void mg_head_parts_kernel(HeadArgs a, double* __restrict__ found) {
   __shared__ X red[HEAD_THREADS / 64], red_s[HEAD_THREADS / 64];
   __shared__ int red_int[HEAD_THREADS / 64];
   for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
     HEAD_PART_COUNTS()
     const HeadRow r = head_row(a, row);
-    const HeadScale<X> scale(r.inv_temp);
+    const HeadScale<X> scale(r);
+    constexpr bool adjust = std::is_same<X, double>::value;
     X x[CHUNKS][8], m = -INFINITY;
+    HeadRaw<8> raw[CHUNKS];
+    HEAD_PART_FETCH((raw[c].template fetch<FULL, adjust>(r, a.logits, a.type, row * a.logits_row + part0 + at, (int)(part0 + at), n)))
 #pragma unroll
     for (int c = 0; c < CHUNKS; c++) {
       const int at = c * HEAD_CHUNK + threadIdx.x * 8, n = part_n - at;
-      head_columns<8, false, std::is_same<X, double>::value>(r, a.logits, a.type, row * a.logits_row, (int)(part0 + at), n, counts + at, x[c],
-                                                             (float*)nullptr);
+      raw[c].template columns<false, adjust>(r, a.type, (int)(part0 + at), n, counts + at, x[c], (float*)nullptr);
     }
 #pragma unroll
     for (int c = 0; c < CHUNKS; c++) {
@@ -676,7 +799,7 @@ __device__ __forceinline__ HeadJoined head_join(const double* f, int parts, doub
 
 // THREADS * 8 columns are a whole part
 template <int THREADS>
-__global__ __launch_bounds__(THREADS) void mg_sample_join_kernel(mg_logits a, int parts, const double* __restrict__ found,
+__global__ __launch_bounds__(THREADS) void mg_sample_join_kernel(HeadArgs a, int parts, const double* __restrict__ found,
                                                                 const float* __restrict__ uniforms, int* __restrict__ actions,
                                                                 float* __restrict__ log_prob, float* __restrict__ entropy) {
   constexpr int PART = THREADS * 8;
@@ -685,7 +808,7 @@ __global__ __launch_bounds__(THREADS) void mg_sample_join_kernel(mg_logits a, in
   __shared__ int red_int[THREADS / 64], picked;
   for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const HeadRow r = head_row(a, row);
-    const HeadScale<double> scale(r.inv_temp);
+    const HeadScale<double> scale(r);
     const double* f = found + row * parts * HEAD_FOUND;
     const HeadJoined j = head_join(f, parts, r.inv_temp, head_lane());
     int hit = -1;
@@ -725,7 +848,9 @@ __global__ __launch_bounds__(THREADS) void mg_sample_join_kernel(mg_logits a, in
         if (a.history) head_count_columns(a, row, counts, part0, part_n);
         const int at = threadIdx.x * 8, n = part_n - at;
         double x[8], t[8], w[8], mine = 0.0;
-        head_columns<8, false, true>(r, a.logits, a.type, row * a.logits_row, (int)(part0 + at), n, counts + at, x, (float*)nullptr);
+        HeadRaw<8> raw;
+        raw.fetch<false, true>(r, a.logits, a.type, row * a.logits_row + part0 + at, (int)(part0 + at), n);
+        raw.columns<false, true>(r, a.type, (int)(part0 + at), n, counts + at, x, (float*)nullptr);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           t[e] = j.m - x[e];
@@ -764,7 +889,7 @@ __global__ __launch_bounds__(THREADS) void mg_sample_join_kernel(mg_logits a, in
 }
 
 // one wave per row
-__global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_join_kernel(mg_logits a, int parts, const double* __restrict__ found,
+__global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_join_kernel(HeadArgs a, int parts, const double* __restrict__ found,
                                                                        const int* __restrict__ actions, float* __restrict__ log_prob,
                                                                        float* __restrict__ entropy, double* __restrict__ stats) {
   const long row = ((long)blockIdx.x * HEAD_THREADS + threadIdx.x) >> 6;
@@ -780,13 +905,13 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_join_kernel(mg_logit
       for (int i = head_lane(); i < a.history_len; i += 64) count += a.history[row * a.history_row + i] == act;
       count = head_group_sum(count, 64);
     }
-    // (one column, with the bits of its place in a word of the mask)
-    HeadRow one = r;
-    if (r.kind == MG_ALLOWED_BITS) one.kind = 0;
+    HeadRow one = r;  // (one column; its bit of the mask is not at a multiple of anything)
+    one.kind = 0;
+    HeadRaw<1> raw;
     double y[1];
-    head_columns<1, false, true>(one, a.logits, a.type, row * a.logits_row, act, 1, &count, y, (float*)nullptr);
-    const bool ok = r.kind != MG_ALLOWED_BITS || ((((const unsigned*)r.allowed)[act >> 5] >> (act & 31)) & 1);
-    x = ok ? y[0] : -INFINITY;
+    raw.fetch<true, true>(one, a.logits, a.type, row * a.logits_row + act, act, 1);
+    raw.columns<false, true>(one, a.type, act, 1, &count, y, (float*)nullptr);
+    x = head_allowed(r, act) ? y[0] : -INFINITY;
   }
   if (head_lane() == 0) {
     const double log_z = j.bad || j.empty ? 0.0 : head_log(j.z);
@@ -797,7 +922,7 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_join_kernel(mg_logit
 }
 
 template <int CHUNKS, typename X>
-__global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_wide_backward_kernel(mg_logits a, const int* __restrict__ actions,
+__global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_wide_backward_kernel(HeadArgs a, const int* __restrict__ actions,
                                                                                 const float* __restrict__ entropy,
                                                                                 const double* __restrict__ stats,
                                                                                 const float* __restrict__ dlog_prob,
@@ -806,7 +931,7 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_wide_backward_kernel
   for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
     HEAD_PART_COUNTS()
     const HeadRow r = head_row(a, row);
-    const HeadScale<X> scale(r.inv_temp);
+    const HeadScale<X> scale(r);
     const double m = stats[2 * row];
     const X log_z = (X)stats[2 * row + 1], past = (X)((double)entropy[row] - stats[2 * row + 1]);  // H + log q = past - t / temperature
     const bool bad = m != m, empty = m == -INFINITY;
@@ -815,13 +940,17 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_wide_backward_kernel
     X gp = 0;
     const X gh = (dentropy ? dentropy[row] : 0.f) * scale.inv_temp;
     if (dlog_prob && act >= 0 && act < a.width) {  // the action's token is left if it is allowed and not at -infinity
+      HeadRow one = r;
+      one.kind = 0;
+      HeadRaw<1> raw;
       float l[1];
-      head_load<1>(a.logits, a.type, row * a.logits_row + act, 1, l);
-      bool ok = l[0] > -INFINITY && (!r.bias || r.bias[act] > -INFINITY);
-      if (r.kind == MG_ALLOWED_BOOL) ok = ok && ((const unsigned char*)r.allowed)[act];
-      if (r.kind == MG_ALLOWED_BITS) ok = ok && ((((const unsigned*)r.allowed)[act >> 5] >> (act & 31)) & 1);
-      if (ok) gp = dlog_prob[row] * scale.inv_temp;
+      raw.fetch<true, false>(one, a.logits, a.type, row * a.logits_row + act, act, 1);
+      raw.values(a.type, l);
+      if (head_allowed(r, act) && l[0] > -INFINITY && (!r.bias || r.bias[act] > -INFINITY)) gp = dlog_prob[row] * scale.inv_temp;
     }
+    constexpr bool adjust = std::is_same<X, double>::value;
+    HeadRaw<8> raw[CHUNKS];
+    HEAD_PART_FETCH((raw[c].template fetch<FULL, adjust>(r, a.logits, a.type, row * a.logits_row + part0 + at, (int)(part0 + at), n)))
 #pragma unroll
     for (int c = 0; c < CHUNKS; c++) {
       const int at = c * HEAD_CHUNK + threadIdx.x * 8, n = part_n - at;
@@ -829,7 +958,7 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_wide_backward_kernel
       const int v0 = (int)(part0 + at);
       X x[8], g[8];
       float slope[8], y[8];
-      const unsigned ok = head_columns<8, true, std::is_same<X, double>::value>(r, a.logits, a.type, row * a.logits_row, v0, n, counts + at, x, slope);
+      const unsigned ok = raw[c].template columns<true, adjust>(r, a.type, v0, n, counts + at, x, slope);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         const X t = top - x[e];
@@ -868,6 +997,15 @@ static int head_check(const char* who, const mg_logits* a) {
   if (a->history && (a->history_len < 1 || a->history_len > 1 << 30)) return mg_fail_msg(w + ": a history has 1 to 2^30 entries");
   if (a->rows && !a->logits) return mg_fail_msg(w + ": NULL tensor");
   return 0;
+}
+
+static HeadArgs head_args(const mg_logits* a) {
+  HeadArgs g;
+  (mg_logits&)g = *a;
+  g.inv_temp = 1.0 / a->temperature;
+  g.inv_rep = 1.0 / a->repetition;
+  g.weight_scale = (float)(g.inv_temp * -1.4426950408889634);
+  return g;
 }
 
 // A part is four chunks where that leaves enough blocks to fill the GPU, else one.
@@ -928,10 +1066,10 @@ static int head_adjust(const char* who, const mg_logits* a, void* out, const voi
   const hipStream_t s = (hipStream_t)stream;
   if (head_narrow(a)) {
     const HeadNarrow g = head_layout(a, 8, false);
-    hipLaunchKernelGGL(mg_adjust_narrow_kernel<8>, dim3(head_blocks(a->rows, g.rows)), dim3(HEAD_THREADS), 0, s, *a, g, out, dout, dlogits);
+    hipLaunchKernelGGL(mg_adjust_narrow_kernel<8>, dim3(head_blocks(a->rows, g.rows)), dim3(HEAD_THREADS), 0, s, head_args(a), g, out, dout, dlogits);
   } else {
     head_by_chunks(a, [&](auto c) {
-      hipLaunchKernelGGL(mg_adjust_wide_kernel<decltype(c)::value>, head_wide_grid(a), dim3(HEAD_THREADS), 0, s, *a, out, dout, dlogits);
+      hipLaunchKernelGGL(mg_adjust_wide_kernel<decltype(c)::value>, head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), out, dout, dlogits);
     });
   }
   return head_launched(who);
@@ -965,16 +1103,16 @@ extern "C" int mg_sample_actions(const mg_logits* a, const float* uniforms, int3
   const hipStream_t s = (hipStream_t)stream;
   if (head_narrow(a)) {
     head_by_width(a, [&](auto e, auto one, HeadNarrow g) {
-      hipLaunchKernelGGL((mg_sample_narrow_kernel<decltype(e)::value, decltype(one)::value>), dim3(head_blocks(a->rows, g.rows)), dim3(HEAD_THREADS), 0, s, *a, g,
+      hipLaunchKernelGGL((mg_sample_narrow_kernel<decltype(e)::value, decltype(one)::value>), dim3(head_blocks(a->rows, g.rows)), dim3(HEAD_THREADS), 0, s, head_args(a), g,
                          uniforms, actions, log_prob, entropy);
     });
   } else {
     head_by_chunks(a, [&](auto c) {
       constexpr int C = decltype(c)::value;
-      if (uniforms) hipLaunchKernelGGL((mg_head_parts_kernel<C, false, double>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, *a, (double*)a->workspace);
-      else hipLaunchKernelGGL((mg_head_parts_kernel<C, true, double>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, *a, (double*)a->workspace);
+      if (uniforms) hipLaunchKernelGGL((mg_head_parts_kernel<C, false, double>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), (double*)a->workspace);
+      else hipLaunchKernelGGL((mg_head_parts_kernel<C, true, double>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), (double*)a->workspace);
       hipLaunchKernelGGL(mg_sample_join_kernel<C * HEAD_THREADS>, dim3((unsigned)(a->rows < 1 << 20 ? a->rows : 1 << 20)), dim3(C * HEAD_THREADS), 0, s,
-                         *a, head_parts(a), (const double*)a->workspace, uniforms, actions, log_prob, entropy);
+                         head_args(a), head_parts(a), (const double*)a->workspace, uniforms, actions, log_prob, entropy);
     });
   }
   return head_launched(who);
@@ -995,16 +1133,16 @@ extern "C" int mg_evaluate_actions(const mg_logits* a, const int32_t* actions, f
     if (head_narrow(a)) {
       head_by_width(a, [&](auto e, auto one, HeadNarrow g) {
         hipLaunchKernelGGL((mg_evaluate_narrow_kernel<decltype(e)::value, decltype(one)::value, X>), dim3(head_blocks(a->rows, g.rows)), dim3(HEAD_THREADS), 0, s,
-                           *a, g, actions, log_prob, entropy);
+                           head_args(a), g, actions, log_prob, entropy);
       });
     } else {
       head_by_chunks(a, [&](auto c) {
-        hipLaunchKernelGGL((mg_head_parts_kernel<decltype(c)::value, false, X>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, *a, (double*)a->workspace);
+        hipLaunchKernelGGL((mg_head_parts_kernel<decltype(c)::value, false, X>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), (double*)a->workspace);
       });
     }
   });
   if (!head_narrow(a))
-    hipLaunchKernelGGL(mg_evaluate_join_kernel, dim3((unsigned)((a->rows + 3) / 4)), dim3(HEAD_THREADS), 0, s, *a, head_parts(a),
+    hipLaunchKernelGGL(mg_evaluate_join_kernel, dim3((unsigned)((a->rows + 3) / 4)), dim3(HEAD_THREADS), 0, s, head_args(a), head_parts(a),
                        (const double*)a->workspace, actions, log_prob, entropy, stats);
   return head_launched(who);
 } catch (...) {
@@ -1024,11 +1162,11 @@ extern "C" int mg_evaluate_actions_backward(const mg_logits* a, const int32_t* a
     if (head_narrow(a))
       head_by_width(a, [&](auto e, auto one, HeadNarrow g) {
         hipLaunchKernelGGL((mg_evaluate_narrow_backward_kernel<decltype(e)::value, decltype(one)::value, X>), dim3(head_blocks(a->rows, g.rows)), dim3(HEAD_THREADS),
-                           0, s, *a, g, actions, dlog_prob, dentropy, dlogits);
+                           0, s, head_args(a), g, actions, dlog_prob, dentropy, dlogits);
       });
     else
       head_by_chunks(a, [&](auto c) {
-        hipLaunchKernelGGL((mg_evaluate_wide_backward_kernel<decltype(c)::value, X>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, *a, actions,
+        hipLaunchKernelGGL((mg_evaluate_wide_backward_kernel<decltype(c)::value, X>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), actions,
                            entropy, stats, dlog_prob, dentropy, dlogits);
       });
   });
