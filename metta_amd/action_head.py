@@ -157,11 +157,11 @@ class _AdjustLogits(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        head, logits = _saved(ctx)
+        (logits,) = _saved(ctx)
         d = torch.empty(dout.shape, dtype=logits.dtype, device=logits.device)
         if d.numel():
             dout = dout.contiguous()
-            _launch("mg_adjust_logits_backward", d.device, ct.byref(head.args), dout.data_ptr(), d.data_ptr())
+            _launch("mg_adjust_logits_backward", d.device, ct.byref(ctx.args), dout.data_ptr(), d.data_ptr())
         return d, None
 
 
@@ -172,11 +172,8 @@ def _save(ctx, logits, head, *more):
 
 
 def _saved(ctx):
-    class Kept:
-        args = ctx.args
-
     saved = ctx.saved_tensors
-    return (Kept, *saved[:1], *saved[4:])
+    return (saved[0], *saved[4:])
 
 
 class _EvaluateActions(torch.autograd.Function):
@@ -200,11 +197,11 @@ class _EvaluateActions(torch.autograd.Function):
     def backward(ctx, dlogp, dentropy):
         if dlogp is None and dentropy is None:
             return None, None, None
-        head, logits, actions, entropy, stats = _saved(ctx)
+        logits, actions, entropy, stats = _saved(ctx)
         d = torch.empty(ctx.shape, dtype=logits.dtype, device=logits.device)
         if d.numel():
             dlogp, dentropy = (None if g is None else g.contiguous() for g in (dlogp, dentropy))
-            _launch("mg_evaluate_actions_backward", d.device, ct.byref(head.args), actions.data_ptr(), entropy.data_ptr(), None if stats is None else stats.data_ptr(),
+            _launch("mg_evaluate_actions_backward", d.device, ct.byref(ctx.args), actions.data_ptr(), entropy.data_ptr(), None if stats is None else stats.data_ptr(),
                     None if dlogp is None else dlogp.data_ptr(), None if dentropy is None else dentropy.data_ptr(), d.data_ptr())  # fmt: skip
         return d, None, None
 

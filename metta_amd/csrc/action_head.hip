@@ -35,37 +35,6 @@
 
 extern int mg_fail_msg(const std::string& m);  // mettagrid_hip.hip: sets mg_last_error(), returns 1
 
-// ---- elements: the tensors' type is a scalar branch around the loads and stores ---------------------------------------
-
-template <int E>
-__device__ __forceinline__ void head_store(void* p, int type, long at, int n, const float* x) {
-  if (type == MG_F32) {
-    float* q = (float*)p + at;
-    if (n >= E) {
-      __builtin_memcpy(q, x, 4 * E);
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; e++) if (e < n) q[e] = x[e];
-    }
-    return;
-  }
-  unsigned short* q = (unsigned short*)p + at;
-  unsigned short raw[E];
-  if (type == MG_BF16) {
-#pragma unroll
-    for (int e = 0; e < E; e++) raw[e] = __builtin_bit_cast(unsigned short, (__bf16)x[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < E; e++) raw[e] = __builtin_bit_cast(unsigned short, (_Float16)x[e]);
-  }
-  if (n >= E) {
-    __builtin_memcpy(q, raw, 2 * E);
-  } else {
-#pragma unroll
-    for (int e = 0; e < E; e++) if (e < n) q[e] = raw[e];
-  }
-}
-
 // ---- arithmetic -------------------------------------------------------------------------------------------------------
 
 // e^-d for d >= 0 (NaN: NaN).  n = rint(y log2 e) with y = -d, r = y - n ln 2 in two parts, |r| <= 0.347: the series to
@@ -159,21 +128,66 @@ __device__ __forceinline__ bool head_allowed(const HeadRow& r, int v) {
 // bit e of `bits` over a whole word
 __device__ __forceinline__ unsigned head_bit(unsigned bits, int e) { return (unsigned)((int)(bits << (31 - e)) >> 31); }
 
-// N words from an address that is aligned to an element of its tensor only
+// N words from (to) an address that is aligned to an element of its tensor only
+typedef unsigned head_four __attribute__((ext_vector_type(4), aligned(1)));
+typedef unsigned head_two __attribute__((ext_vector_type(2), aligned(1)));
+typedef unsigned head_one __attribute__((aligned(1)));
 template <int N>
 __device__ __forceinline__ void head_words(const void* p, unsigned* out) {
-  typedef unsigned four __attribute__((ext_vector_type(4), aligned(1)));
-  typedef unsigned two __attribute__((ext_vector_type(2), aligned(1)));
-  static_assert(N == 2 || N % 4 == 0, "whole vectors");
-  if constexpr (N == 2) {
-    const two w = *(const two*)p;
-    out[0] = w.x, out[1] = w.y;
+#pragma unroll
+  for (int i = 0; i + 4 <= N; i += 4) {
+    const head_four w = ((const head_four*)p)[i / 4];
+    out[i] = w.x, out[i + 1] = w.y, out[i + 2] = w.z, out[i + 3] = w.w;
+  }
+  constexpr int two = N & ~3, one = N & ~1;
+  if constexpr (N & 2) {
+    const head_two w = *(const head_two*)((const char*)p + 4 * two);
+    out[two] = w.x, out[two + 1] = w.y;
+  }
+  if constexpr (N & 1) out[one] = *(const head_one*)((const char*)p + 4 * one);
+}
+template <int N>
+__device__ __forceinline__ void head_put_words(void* p, const unsigned* in) {
+#pragma unroll
+  for (int i = 0; i + 4 <= N; i += 4) ((head_four*)p)[i / 4] = head_four{in[i], in[i + 1], in[i + 2], in[i + 3]};
+  constexpr int two = N & ~3, one = N & ~1;
+  if constexpr (N & 2) *(head_two*)((char*)p + 4 * two) = head_two{in[two], in[two + 1]};
+  if constexpr (N & 1) *(head_one*)((char*)p + 4 * one) = in[one];
+}
+
+// E adjacent elements, n of them in the row
+template <int E>
+__device__ __forceinline__ void head_store(void* p, int type, long at, int n, const float* x) {
+  unsigned w[E];
+  if (type == MG_F32) {
+    unsigned* q = (unsigned*)p + at;
+#pragma unroll
+    for (int e = 0; e < E; e++) w[e] = __float_as_uint(x[e]);
+    if (n >= E) {
+      head_put_words<E>(q, w);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; e++) if (e < n) q[e] = w[e];
+    }
+    return;
+  }
+  unsigned short* q = (unsigned short*)p + at;
+  if (type == MG_BF16) {
+#pragma unroll
+    for (int e = 0; e < E; e++) w[e] = __builtin_bit_cast(unsigned short, (__bf16)x[e]);
   } else {
 #pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      const four w = ((const four*)p)[i / 4];
-      out[i] = w.x, out[i + 1] = w.y, out[i + 2] = w.z, out[i + 3] = w.w;
-    }
+    for (int e = 0; e < E; e++) w[e] = __builtin_bit_cast(unsigned short, (_Float16)x[e]);
+  }
+  if (n >= E) {
+    unsigned pair[(E + 1) / 2];
+#pragma unroll
+    for (int e = 0; e + 1 < E; e += 2) pair[e / 2] = w[e] | w[e + 1] << 16;
+    head_put_words<E / 2>(q, pair);
+    if constexpr (E & 1) q[E - 1] = (unsigned short)w[E - 1];
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; e++) if (e < n) q[e] = (unsigned short)w[e];
   }
 }
 
@@ -210,8 +224,8 @@ struct HeadRaw {
   }
   template <bool FULL>
   static __device__ __forceinline__ void words(const unsigned* p, int n, unsigned* out) {
-    if (E > 1 && (FULL || n >= E)) {
-      if constexpr (E > 1) head_words<E>(p, out);
+    if (FULL || n >= E) {
+      head_words<E>(p, out);
     } else {
 #pragma unroll
       for (int e = 0; e < E; e++) out[e] = e < n ? p[e] : 0u;
@@ -219,8 +233,9 @@ struct HeadRaw {
   }
   template <bool FULL>
   static __device__ __forceinline__ void halves(const unsigned short* p, int n, unsigned* out) {
-    if (E > 1 && (FULL || n >= E)) {
-      if constexpr (E > 1) head_words<E / 2>(p, out);
+    if (FULL || n >= E) {
+      head_words<E / 2>(p, out);
+      if constexpr (E & 1) out[E / 2] = p[E - 1];
     } else {
 #pragma unroll
       for (int e = 0; e < E; e += 2) {
@@ -231,14 +246,14 @@ struct HeadRaw {
   }
   template <bool FULL>
   static __device__ __forceinline__ void bytes(const unsigned char* p, int n, unsigned* out) {
-    if (E > 1 && (FULL || n >= E)) {
-      if constexpr (E > 1) head_words<E / 4>(p, out);
+    if ((FULL || n >= E) && E % 4 == 0) {
+      head_words<E / 4>(p, out);
     } else {
 #pragma unroll
       for (int w = 0; w < (E + 3) / 4; w++) {
         unsigned b = 0;
 #pragma unroll
-        for (int e = 4 * w; e < E && e < 4 * w + 4; e++) b |= (e < n ? (unsigned)p[e] : 0u) << (8 * (e % 4));
+        for (int e = 4 * w; e < E && e < 4 * w + 4; e++) b |= (FULL || e < n ? (unsigned)p[e] : 0u) << (8 * (e % 4));
         out[w] = b;
       }
     }
@@ -272,16 +287,20 @@ struct HeadRaw {
   // x, and (GRAD) what a gradient of x is multiplied by besides 1 / temperature: 0 where masked, and only where ADJUST,
   // else the bits tell.  ADJUST: whether there may be a bias or a history at all.  counts: these columns in the history.
   // Returns bits().
-  template <bool GRAD, bool ADJUST, typename X>
+  template <bool FULL, bool GRAD, bool ADJUST, typename X>
   __device__ __forceinline__ unsigned columns(const HeadRow& r, int type, int v0, int n, const unsigned* counts, X* x, float* slope) const {
     float l[E];
     values(type, l);
     const unsigned ok = bits(r, v0, n);
+    if (!FULL || r.kind) {  // masked, or behind the row's end: -infinity
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-      const unsigned in = head_bit(ok, e);
-      x[e] = (X)__uint_as_float((__float_as_uint(l[e]) & in) | (0xFF800000u & ~in));  // masked: -infinity
+      for (int e = 0; e < E; e++) {
+        const unsigned in = head_bit(ok, e);
+        l[e] = __uint_as_float((__float_as_uint(l[e]) & in) | (0xFF800000u & ~in));
+      }
     }
+#pragma unroll
+    for (int e = 0; e < E; e++) x[e] = (X)l[e];
     if (!ADJUST) return ok;
     if (r.counted) {
 #pragma unroll
@@ -305,8 +324,6 @@ struct HeadRaw {
 
 // ---- lanes ------------------------------------------------------------------------------------------------------------
 
-__device__ __forceinline__ double head_add(double a, double b) { return a + b; }
-__device__ __forceinline__ float head_add(float a, float b) { return a + b; }
 __device__ __forceinline__ int head_lane() { return threadIdx.x & 63; }
 
 // over the `lanes` (a power of two) lanes of a group; every lane gets the result
@@ -345,9 +362,10 @@ struct HeadAdjust {
 
   template <bool FULL>
   __device__ __forceinline__ void fetch(const HeadArgs& a, const HeadRow& r, long row, int v0, int n, const void* dout) {
-    raw.template fetch<FULL, true>(r, !dout || r.counted ? a.logits : nullptr, a.type, row * a.logits_row + v0, v0, n);
+    HeadRow plain = r;
+    if (dout) plain.bias = nullptr;  // (no gradient depends on it)
+    raw.template fetch<FULL, true>(plain, !dout || r.counted ? a.logits : nullptr, a.type, row * a.logits_row + v0, v0, n);
     if (dout) {
-      HeadRow plain = r;
       plain.kind = 0;
       outer.template fetch<FULL, false>(plain, dout, a.type, row * a.width + v0, v0, n);
     }
@@ -357,7 +375,7 @@ struct HeadAdjust {
     double x[E];
     float slope[E], y[E];
     if (!dout) {
-      raw.template columns<false, true>(r, a.type, v0, n, counts, x, slope);
+      raw.template columns<false, false, true>(r, a.type, v0, n, counts, x, slope);
 #pragma unroll
       for (int e = 0; e < E; e++) y[e] = (float)(x[e] * r.inv_temp);
       head_store<E>(out, a.type, row * a.width + v0, n, y);
@@ -365,7 +383,9 @@ struct HeadAdjust {
     }
     outer.values(a.type, y);
     if (r.counted) {
-      raw.template columns<true, true>(r, a.type, v0, n, counts, x, slope);
+      HeadRow plain = r;
+      plain.bias = nullptr;
+      raw.template columns<false, true, true>(plain, a.type, v0, n, counts, x, slope);
 #pragma unroll
       for (int e = 0; e < E; e++) y[e] = slope[e] == 0.f ? 0.f : (float)((double)y[e] * (slope[e] * r.inv_temp));
     } else {
@@ -411,7 +431,7 @@ __device__ __forceinline__ void head_count_rows(const HeadArgs& a, const HeadNar
   __syncthreads();
 }
 
-// What the lanes of a row know of it.  ONE: a lane per row, so that the number of columns is a scalar.
+// What the lanes of a row know of it.  ONE: a lane per row, of exactly E columns.
 template <int E, bool ONE, typename X>
 struct HeadHeld {
   X x[E], t[E], w[E], m, z, s, z_lane;  // t = M - x, w = its weight; t and w say nothing where the row is bad or empty
@@ -427,15 +447,15 @@ struct HeadHeld {
     mine = at < a.rows && (ONE || (int)threadIdx.x < g.rows * g.lanes);
     row = mine ? at : a.rows - 1;
     v0 = lane * E;
-    n = a.width - v0;
+    n = ONE ? E : a.width - v0;
   }
 
   template <bool GRAD>
   __device__ __forceinline__ void hold(const HeadArgs& a, const HeadNarrow& g, const HeadRow& r, const HeadScale<X>& scale, const unsigned* counts) {
     constexpr bool adjust = std::is_same<X, double>::value;
     HeadRaw<E> raw;
-    raw.template fetch<false, adjust>(r, a.logits, a.type, row * a.logits_row + v0, v0, n);
-    ok = raw.template columns<GRAD, adjust>(r, a.type, v0, n, counts, x, slope);
+    raw.template fetch<ONE, adjust>(r, a.logits, a.type, row * a.logits_row + v0, v0, n);
+    ok = raw.template columns<ONE, GRAD, adjust>(r, a.type, v0, n, counts, x, slope);
     m = x[0];
 #pragma unroll
     for (int e = 1; e < E; e++) m = head_max(m, x[e]);
@@ -444,14 +464,10 @@ struct HeadHeld {
     z = s = 0;
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      if (!ONE || e < n) {
-        t[e] = head_finite(top - x[e]);
-        w[e] = scale.weight(top - x[e]);
-        z += w[e];
-        s = head_fma(t[e], w[e], s);
-      } else {
-        t[e] = w[e] = 0;
-      }
+      t[e] = head_finite(top - x[e]);
+      w[e] = scale.weight(top - x[e]);
+      z += w[e];
+      s = head_fma(t[e], w[e], s);
     }
     z_lane = z;
     if (!ONE) {
@@ -530,15 +546,18 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_sample_narrow_kernel(HeadArgs
 template <int E, bool ONE, typename X>
 __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_kernel(HeadArgs a, HeadNarrow g, const int* __restrict__ actions,
                                                                          float* __restrict__ log_prob, float* __restrict__ entropy) {
-  __shared__ unsigned counts[HEAD_THREADS][E + 1];
+  constexpr bool adjust = std::is_same<X, double>::value;
+  __shared__ unsigned counts[adjust ? HEAD_THREADS : 1][E + 1];
   for (long row0 = (long)blockIdx.x * g.rows; row0 < a.rows; row0 += (long)gridDim.x * g.rows) {
-    if (a.history) head_count_rows<E>(a, g, row0, counts);
+    if constexpr (adjust) {
+      if (a.history) head_count_rows<E>(a, g, row0, counts);
+    }
     HeadHeld<E, ONE, X> h;
     h.place(a, g, row0);
     const HeadRow r = head_row(a, h.row);
     const HeadScale<X> scale(r);
     const int act = actions[h.row];
-    h.template hold<false>(a, g, r, scale, counts[threadIdx.x]);
+    h.template hold<false>(a, g, r, scale, counts[adjust ? threadIdx.x : 0]);
     X d = INFINITY;
 #pragma unroll
     for (int e = 0; e < E; e++) d = h.v0 + e == act && e < h.n ? (h.x[e] == (X)-INFINITY ? (X)INFINITY : h.t[e] * scale.inv_temp) : d;
@@ -556,16 +575,19 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_backward_kern
                                                                                   const float* __restrict__ dlog_prob,
                                                                                   const float* __restrict__ dentropy,
                                                                                   void* __restrict__ dlogits) {
-  __shared__ unsigned counts[HEAD_THREADS][E + 1];
+  constexpr bool adjust = std::is_same<X, double>::value;
+  __shared__ unsigned counts[adjust ? HEAD_THREADS : 1][E + 1];
   for (long row0 = (long)blockIdx.x * g.rows; row0 < a.rows; row0 += (long)gridDim.x * g.rows) {
-    if (a.history) head_count_rows<E>(a, g, row0, counts);
+    if constexpr (adjust) {
+      if (a.history) head_count_rows<E>(a, g, row0, counts);
+    }
     HeadHeld<E, ONE, X> h;
     h.place(a, g, row0);
     const HeadRow r = head_row(a, h.row);
     const HeadScale<X> scale(r);
     const int act = actions[h.row];
     const X gp_row = dlog_prob ? dlog_prob[h.row] : 0.f, gh = (dentropy ? dentropy[h.row] : 0.f) * scale.inv_temp;
-    h.template hold<true>(a, g, r, scale, counts[threadIdx.x]);
+    h.template hold<true>(a, g, r, scale, counts[adjust ? threadIdx.x : 0]);
     bool left = false;  // whether the action is a token that is left
 #pragma unroll
     for (int e = 0; e < E; e++) left = left || (h.v0 + e == act && e < h.n && h.x[e] > (X)-INFINITY);
@@ -576,7 +598,6 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_backward_kern
     float y[E];
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      if (ONE && e >= h.n) continue;
       const X q = h.w[e] * inv_z;
       X d = (h.v0 + e == act ? gp : (X)0) - q * head_fma(gh, past - h.t[e] * scale.inv_temp, gp);
       if (std::is_same<X, double>::value) d *= h.slope[e];
@@ -731,7 +752,7 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_head_parts_kernel(HeadArgs a,
 #pragma unroll
     for (int c = 0; c < CHUNKS; c++) {
       const int at = c * HEAD_CHUNK + threadIdx.x * 8, n = part_n - at;
-      raw[c].template columns<false, adjust>(r, a.type, (int)(part0 + at), n, counts + at, x[c], (float*)nullptr);
+      raw[c].template columns<false, false, adjust>(r, a.type, (int)(part0 + at), n, counts + at, x[c], (float*)nullptr);
     }
 #pragma unroll
     for (int c = 0; c < CHUNKS; c++) {
@@ -850,7 +871,7 @@ __global__ __launch_bounds__(THREADS) void mg_sample_join_kernel(HeadArgs a, int
         double x[8], t[8], w[8], mine = 0.0;
         HeadRaw<8> raw;
         raw.fetch<false, true>(r, a.logits, a.type, row * a.logits_row + part0 + at, (int)(part0 + at), n);
-        raw.columns<false, true>(r, a.type, (int)(part0 + at), n, counts + at, x, (float*)nullptr);
+        raw.columns<false, false, true>(r, a.type, (int)(part0 + at), n, counts + at, x, (float*)nullptr);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           t[e] = j.m - x[e];
@@ -910,7 +931,7 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_join_kernel(HeadArgs
     HeadRaw<1> raw;
     double y[1];
     raw.fetch<true, true>(one, a.logits, a.type, row * a.logits_row + act, act, 1);
-    raw.columns<false, true>(one, a.type, act, 1, &count, y, (float*)nullptr);
+    raw.columns<false, false, true>(one, a.type, act, 1, &count, y, (float*)nullptr);
     x = head_allowed(r, act) ? y[0] : -INFINITY;
   }
   if (head_lane() == 0) {
@@ -921,8 +942,9 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_join_kernel(HeadArgs
   }
 }
 
+// (four waves per SIMD: 69 us on 2048 x 32003 bf16 against 80 with three and more registers each)
 template <int CHUNKS, typename X>
-__global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_wide_backward_kernel(HeadArgs a, const int* __restrict__ actions,
+__global__ __launch_bounds__(HEAD_THREADS, (sizeof(X) == 4 ? 4 : 2)) void mg_evaluate_wide_backward_kernel(HeadArgs a, const int* __restrict__ actions,
                                                                                 const float* __restrict__ entropy,
                                                                                 const double* __restrict__ stats,
                                                                                 const float* __restrict__ dlog_prob,
@@ -958,7 +980,7 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_wide_backward_kernel
       const int v0 = (int)(part0 + at);
       X x[8], g[8];
       float slope[8], y[8];
-      const unsigned ok = raw[c].template columns<true, adjust>(r, a.type, v0, n, counts + at, x, slope);
+      const unsigned ok = raw[c].template columns<false, true, adjust>(r, a.type, v0, n, counts + at, x, slope);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         const X t = top - x[e];
@@ -1031,8 +1053,19 @@ template <int V> using head_int = std::integral_constant<int, V>;
 template <bool V> using head_bool = std::integral_constant<bool, V>;
 template <typename F>
 static void head_by_width(const mg_logits* a, F f) {
-  if (a->width <= 8) f(head_int<8>(), head_bool<true>(), head_layout(a, 8, true));
-  else if (a->width <= 64 * 8) f(head_int<8>(), head_bool<false>(), head_layout(a, 8, true));
+  const head_bool<true> one;
+  const HeadNarrow g{1, HEAD_THREADS};
+  switch (a->width) {
+    case 1: return f(head_int<1>(), one, g);
+    case 2: return f(head_int<2>(), one, g);
+    case 3: return f(head_int<3>(), one, g);
+    case 4: return f(head_int<4>(), one, g);
+    case 5: return f(head_int<5>(), one, g);
+    case 6: return f(head_int<6>(), one, g);
+    case 7: return f(head_int<7>(), one, g);
+    case 8: return f(head_int<8>(), one, g);
+  }
+  if (a->width <= 64 * 8) f(head_int<8>(), head_bool<false>(), head_layout(a, 8, true));
   else f(head_int<16>(), head_bool<false>(), head_layout(a, 16, true));
 }
 template <typename F>
