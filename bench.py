@@ -190,7 +190,7 @@ def rollout_workload(args, wl, rank, local_rank, world, use_dist, saved_stdout, 
     import torch
     import torch.distributed as dist
 
-    from metta_amd.rollout import LSTMPolicy
+    from metta_amd.rollout import ActionControls, GatedRecurrentPolicy, LSTMPolicy
     from metta_amd.vecenv import AsyncDeviceVecEnv, MettaGridDeviceVecEnv
 
     dev = torch.device("cuda", local_rank)
@@ -204,7 +204,9 @@ def rollout_workload(args, wl, rank, local_rank, world, use_dist, saved_stdout, 
         handles = [env.batch]
     env.async_reset(seed0)  # (stats_every = 0: finished episodes are collected without blocking a send)
     n_group = env.agents_per_batch if G > 1 else env.num_agents
-    pol = LSTMPolicy(cfg.game.obs.num_tokens, env.single_action_space.n).to(dev).to(torch.bfloat16)
+    gated = args.policy == "gated"
+    pol = (GatedRecurrentPolicy if gated else LSTMPolicy)(cfg.game.obs.num_tokens, env.single_action_space.n).to(dev).to(torch.bfloat16)
+    controls = ActionControls()
     states = [pol.initial_state(n_group, dev, torch.bfloat16) for _ in range(G)]
     gen = torch.Generator(device=dev).manual_seed(1234 + rank)
     summary = torch.zeros(3 + len(handles[0].compiled.game_slot_names), dtype=torch.float64, device=dev)
@@ -222,6 +224,11 @@ def rollout_workload(args, wl, rank, local_rank, world, use_dist, saved_stdout, 
         for t in range(k):
             for q in range(G):  # one step of the rank = every group once
                 o, r, d, tr, ta, infos, ids, mask = env.recv()
+                if gated:
+                    logits, value, states[q] = pol(o, states[q], d | tr)
+                    acts, _, _ = controls.sample(logits, None, gen)
+                    env.send(acts)
+                    continue
                 logits, value, st = pol(o, states[q])
                 done = (d | tr).to(st[0].dtype).unsqueeze(1)
                 states[q] = (st[0] * (1 - done), st[1] * (1 - done))
@@ -261,7 +268,7 @@ def rollout_workload(args, wl, rank, local_rank, world, use_dist, saved_stdout, 
         step_s = dt / args.steps
         achieved = ALGO_BYTES_PER_AGENT_STEP * E * A / step_s / 1e9
         print(json.dumps({
-            "metric": "agent-steps/sec (node), device-resident rollout with an LSTM policy @1/2/4/8 GPU (BASELINE configs[4]; not the headline metric)",
+            "metric": f"agent-steps/sec (node), device-resident rollout with {'a gated recurrent' if gated else 'an LSTM'} policy @1/2/4/8 GPU (BASELINE configs[4]; not the headline metric)",
             "value": float(world) * E * A * args.steps / dt, "unit": "agent-steps/s", "n_gpus": world, "steps": args.steps,
             "warmup": args.warmup, "ms_per_step": step_s * 1e3, "higher_is_better": True, "scaling": "weak", "vs_baseline": None,
             "dtype": "u8 environment step, bf16 policy", "data": "synthetic",
@@ -288,6 +295,8 @@ def main() -> None:
                     "(bench_shard) and summary all-reduce, for the multi-GPU curves of those configurations")
     ap.add_argument("--envs", type=int, default=None, help="environments per GPU (default: the workload's)")
     ap.add_argument("--groups", type=int, default=None, help="independent environment groups, one HIP stream each (1 = one handle)")
+    ap.add_argument("--policy", choices=("lstm", "gated"), default="lstm",
+                    help="rollout workload: the LSTM policy, or the gated linear recurrence with the action head's kernels")
     ap.add_argument("--no-cpu-baseline", action="store_true")
     ap.add_argument("--no-single", action="store_true", help="skip the one-handle comparison run (profiling passes: one launch shape only)")
     ap.add_argument("--no-obs-pass", action="store_true", help="skip the observation-kernel pass (metric 2) after the timed region")

@@ -1,0 +1,177 @@
+"""The recurrent core and the action head as they are used together: a rollout with `GatedRecurrentPolicy` under
+`ActionControls`, the stored segments re-evaluated with gradients, against a plain 64-bit loop over time."""
+
+import numpy as np
+import pytest
+import torch
+
+from metta_amd.rollout import ActionControls, GatedRecurrentPolicy, LSTMPolicy, reset_state
+from metta_amd.training import DeviceExperience, evaluate_experience, experience_spec
+
+
+def test_action_controls_history():
+    """One column per step in turn, cleared where an episode ended, separate for every slice of agents."""
+    c = ActionControls(history_length=3, repetition=1.5)
+    h = c.history("a", 2, "cpu")
+    assert h.shape == (2, 3) and h.dtype == torch.int32 and bool((h == -1).all())
+    for t in range(4):
+        c.took("a", torch.tensor([t, 10 + t], dtype=torch.int32))
+    assert c.history("a", 2, "cpu") is h and h.tolist() == [[3, 1, 2], [13, 11, 12]]
+    c.ended("a", torch.tensor([True, False]))
+    assert h.tolist() == [[-1, -1, -1], [13, 11, 12]]
+    assert bool((c.history("b", 4, "cpu") == -1).all())
+    none = ActionControls(temperature=0.5)
+    assert none.history("a", 2, "cpu") is None
+    none.took("a", torch.zeros(2)), none.ended("a", torch.zeros(2, dtype=torch.bool))
+    with pytest.raises(ValueError, match="history_length"):
+        ActionControls(history=h)
+
+
+def test_segment_state_is_kept_at_the_first_step():
+    ex = DeviceExperience(4, 8 * 3, 3, {"x": ((), torch.float32)}, "cpu", state_width=2)
+    for t in range(6):
+        for sl in (slice(0, 2), slice(2, 4)):
+            ex.store_state(torch.full((2, 2), float(10 * t + sl.start)), sl)
+            ex.store({"x": torch.zeros(2)}, sl)
+    want = [0, 0, 2, 2, 30, 30, 32, 32]
+    assert ex.segment_state[:, 0].tolist() == want and ex.segment_state[:, 1].tolist() == want
+    assert DeviceExperience(4, 8 * 3, 3, {}, "cpu").segment_state is None
+
+
+def test_reset_state_and_refusals():
+    done = torch.tensor([True, False])
+    s = (torch.ones(2, 3), torch.full((2, 3), 2.0))
+    out = reset_state(LSTMPolicy(4, 5, 3), s, done)
+    assert out[0].tolist() == [[0] * 3, [1] * 3] and out[1].tolist() == [[0] * 3, [2] * 3]
+    p = GatedRecurrentPolicy(4, 5, 3)
+    assert reset_state(p, s, done) is s
+    assert p.initial_state(7, "cpu")[0].shape == (7, 3) and p.bfloat16().initial_state(2, "cpu")[0].dtype == torch.float32
+    ex = DeviceExperience(2, 8, 4, experience_spec(4), "cpu")
+    with pytest.raises(ValueError, match="action_history"):
+        evaluate_experience(p, ex, ActionControls(history_length=2, presence=0.5))
+    assert experience_spec(4, history_length=6)["action_history"] == ((6,), torch.int32)
+
+
+def _plain(policy, obs, state, resets, actions, history, controls):
+    """The policy and the action head in float64, step by step; returns (log_prob, entropy, values)."""
+    x = policy.core(policy.enc(obs.flatten(-2).double() / 255.0))
+    cand, gate = x.chunk(2, -1)
+    h, out = state, []
+    for t in range(x.shape[1]):
+        h = torch.where(resets[:, t, None], torch.zeros_like(h), h)
+        a = torch.sigmoid(gate[:, t])
+        h = a * h + (1 - a) * cand[:, t]
+        out.append(h)
+    h = torch.stack(out, 1)
+    l = policy.pi(h)
+    if history is not None:
+        v = torch.arange(l.shape[-1])
+        c = (history.unsqueeze(-1) == v).sum(-2)
+        l = torch.where(c > 0, torch.where(l > 0, l / controls["repetition"], l * controls["repetition"]), l)
+        l = l - controls["frequency"] * c - controls["presence"] * (c > 0)
+    if "bias" in controls:
+        l = l + controls["bias"].double()
+    l = l / controls["temperature"]
+    if "allowed" in controls:
+        l = l.masked_fill(~controls["allowed"], -1e30)
+    logq = torch.log_softmax(l, -1)
+    return logq.gather(-1, actions.long().unsqueeze(-1)).squeeze(-1), -(logq.exp() * logq).sum(-1), policy.v(h).squeeze(-1)
+
+
+@pytest.mark.gpu
+def test_rollout_and_evaluation_together():
+    """24 agents x 4 environments in two groups, episodes of 9 steps inside segments of 16: masked actions are never taken,
+    nothing reads the device, the re-evaluated log-probabilities are the stored ones, and the gradients of a loss over
+    log-probabilities, entropies and values are those of the plain loop."""
+    from metta_amd.builder import make_arena
+    from metta_amd.training import compute_rollout_advantages, rollout_phase
+    from metta_amd.vecenv import DeviceTrainingEnvironment
+    from tests.helpers import load_map_pool
+    from tests.test_training_seam import _SyncCounter
+
+    cfg = make_arena(24)
+    cfg.game.max_steps = 9
+    env = DeviceTrainingEnvironment(cfg, num_envs=4, device=0, seed=5, async_factor=2, maps=load_map_pool()[:2], early_reset=False)
+    n, T, L = env.total_parallel_agents, 16, 6
+    torch.manual_seed(3)
+    policy = GatedRecurrentPolicy(200, 5, hidden=48).cuda()
+    with torch.no_grad():
+        policy.pi.weight.mul_(8.0)  # logits that differ
+        policy.core.bias[48:] += 1.0
+    allowed = torch.tensor([True, True, False, True, True]).cuda()
+    bias = torch.tensor([0.5, 0.0, 3.0, -0.25, 0.0]).cuda()
+    settings = dict(allowed=allowed, bias=bias, temperature=0.8, repetition=1.25, presence=0.3, frequency=0.1)
+    controls = ActionControls(history_length=L, **settings)
+    ex = DeviceExperience(n, 2 * n * T, T, experience_spec(200, history_length=L), device="cuda", state_width=48)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    states: dict = {}
+    torch.cuda.synchronize()
+    with _SyncCounter() as sc:
+        res = rollout_phase(env, policy, ex, policy_state=states, generator=g, controls=controls)
+        reads = sc.count
+    assert reads == 0 and ex.ready_for_training and res.agent_steps == 2 * n * T
+    b = ex.buffer
+    acts = b["actions"]
+    assert bool(((acts >= 0) & (acts < 5) & (acts != 2)).all())
+    ended = (b["dones"] + b["truncateds"]) > 0
+    assert bool(ended.any()) and not bool(ended.all())
+    # a step's history holds the actions before it, back to the episode's start
+    hist, a_np, e_np = b["action_history"].cpu().numpy(), acts.cpu().numpy(), ended.cpu().numpy()
+    for row in (0, 31, n - 1):
+        t0 = 0
+        for t in range(T):
+            if e_np[row, t]:
+                t0 = t
+            want = sorted(a_np[row, max(t0, t - L) : t].tolist())
+            assert sorted(hist[row, t][hist[row, t] >= 0].tolist()) == want, (row, t)
+
+    logp, entropy, values = evaluate_experience(policy, ex, controls)
+    assert logp.shape == (2 * n, T) and logp.requires_grad
+    # the products of 600 and 48 terms are summed in another order: sqrt(600) * 2^-24 * (sum of |w x| up to 12) * (8-fold
+    # logits over a temperature of 0.8) is some 2e-4 at the most
+    assert float((logp.detach() - b["act_log_prob"]).abs().max()) < 1e-3
+    assert float((values.detach() - b["values"]).abs().max()) < 1e-3
+    adv = compute_rollout_advantages(ex)
+    loss = -(adv * logp).mean() - 0.01 * entropy.mean() + 0.5 * (values - adv).pow(2).mean()
+    params = dict(policy.named_parameters())
+    got = dict(zip(params, torch.autograd.grad(loss, params.values())))
+
+    twin = GatedRecurrentPolicy(200, 5, hidden=48).double()
+    twin.load_state_dict({k: v.double().cpu() for k, v in policy.state_dict().items()})
+    c64 = {k: v.cpu() if torch.is_tensor(v) else v for k, v in settings.items()}
+    lp, en, va = _plain(twin, b["env_obs"].cpu(), ex.segment_state.double().cpu(), ended.cpu(), acts.cpu(), b["action_history"].cpu(), c64)
+    a64 = adv.double().cpu()
+    want = torch.autograd.grad(-(a64 * lp).mean() - 0.01 * en.mean() + 0.5 * (va - a64).pow(2).mean(), list(twin.parameters()))
+    assert float((logp.detach().double().cpu() - lp.detach()).abs().max()) < 1e-3
+    assert float((entropy.detach().double().cpu() - en.detach()).abs().max()) < 1e-3
+    for (name, d), w in zip(got.items(), want):
+        off = float((d.double().cpu() - w).norm() / w.norm())
+        assert off < 1e-3, (name, off)  # sums of 6144 x 16 terms in 32 bits
+    # the next rollout goes on from the states and histories that this one left
+    rollout_phase(env, policy, ex, policy_state=states, generator=g, controls=controls)
+    logp, _, _ = evaluate_experience(policy, ex, controls, rows=slice(3, 77))
+    assert float((logp.detach() - ex.buffer["act_log_prob"][3:77]).abs().max()) < 1e-3
+    env.vecenv.flush_infos()
+    env.close()
+
+
+@pytest.mark.gpu
+def test_plain_rollout_with_controls():
+    from metta_amd.builder import make_arena
+    from metta_amd.rollout import rollout
+    from metta_amd.vecenv import MettaGridDeviceVecEnv
+    from tests.helpers import load_map_pool
+
+    env = MettaGridDeviceVecEnv(make_arena(24), 3, maps=load_map_pool()[:2], device=0, seed=2)
+    env.async_reset(2)
+    g = torch.Generator(device="cuda").manual_seed(0)
+    torch.manual_seed(0)
+    for policy in (GatedRecurrentPolicy(200, 5).cuda().bfloat16(), LSTMPolicy(200, 5).cuda()):
+        controls = ActionControls(history_length=4, presence=1.0, temperature=1.5)
+        steps, seconds, state, _ = rollout(env, policy, 12, generator=g, controls=controls)
+        assert steps == 12 * 72 and bool(torch.isfinite(state[0]).all())
+        h = controls.history(0, 72, "cuda")
+        assert bool(((h >= -1) & (h < 5)).all()) and bool((h >= 0).any())
+        steps, _, state, _ = rollout(env, policy, 3, state=state, generator=g)
+        assert steps == 3 * 72
+    env.close()
