@@ -271,6 +271,8 @@ def _own(s):
         h, last = recurrence.gated_recurrence(s["x"], s["gate"], s["state"], s["resets"])
         leaves = [s["x"], s["state"]] + ([] if s["gate"] is None else [s["gate"]])
         grads = torch.autograd.grad([h, last], leaves, [s["dh"], s["dlast"]])
+        if s["dh"].dtype == torch.float32:  # the plain form adds dlast to a 32-bit dh where it lies: a state called again is
+            s["dh"][:, -1] += s["dlast"]  # the same on both sides only if this one does so too, after its own pass
         out = {"h": h.detach(), "last": last.detach(), "dstate": grads[1], "dx": grads[0]}
         return out if s["gate"] is None else out | {"dgate": grads[2]}
     if op == "adjust":
