@@ -366,8 +366,8 @@ int mg_gated_recurrence_backward(const mg_recurrence* r, const float* marks, int
  * i32, entries outside [0, width) count for nothing.  A row stride of 0 shares a control among all rows; NULL: none. */
 #define MG_ALLOWED_BOOL 1
 #define MG_ALLOWED_BITS 2
-/* Rows up to this many tokens stay in registers: their backward pass wants neither stats nor entropy back. */
-#define MG_EVALUATE_STATS_WIDTH 1024
+/* Rows up to this many tokens are held in registers: their backward pass wants neither stats nor entropy back. */
+#define MG_EVALUATE_STATS_WIDTH 8192
 typedef struct mg_logits {
   const void* logits;
   const float* bias;

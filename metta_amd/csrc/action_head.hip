@@ -12,14 +12,14 @@
 // or +infinity among its allowed tokens has action -1 and NaN.
 //
 // Rows of up to HEAD_NARROW columns are held in registers, E adjacent columns per lane, by as many lanes as that takes
-// (one lane for five actions, a wave for a thousand), so logits are read once.  Wider rows are cut into parts of one or
-// four times HEAD_CHUNK columns, a block each; what a part found (maximum, sum, ...) goes to a workspace and a second launch joins
+// (one lane for five actions, a wave for five hundred); rows of up to HEAD_ROW columns by a block, eight columns per
+// thread.  Their logits are read once.  Wider rows are cut into parts of one or four chunks, a block each; what a part found (maximum, sum, ...) goes to a workspace and a second launch joins
 // the parts of a row.  A history is counted in LDS by the block that needs it, for the columns that it holds.
 //
 // Sampling is done in 64 bits from the exponential on: an action that falls next to a border of the distribution is then
 // the definition's whatever the order of the sums, and a 64-bit multiply-add costs what a 32-bit one costs here.
-// Log-probabilities and entropies of given actions need no more than 32 bits, and are computed in 32 unless a bias or a
-// penalty could cancel large logits (HeadX = double).
+// Log-probabilities and entropies of given actions need no more than 32 bits; there only the logits themselves are held in 64
+// where a bias or a penalty could cancel large ones.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -29,8 +29,10 @@
 #include "../../include/mettagrid_hip.h"
 
 #define HEAD_THREADS 256
-#define HEAD_NARROW MG_EVALUATE_STATS_WIDTH
+#define HEAD_NARROW (64 * 8)  // the widest row that lanes of one wave hold
 #define HEAD_CHUNK (HEAD_THREADS * 8)  // columns that a block holds as 8 per thread
+#define HEAD_ROW (4 * HEAD_CHUNK)  // the widest row that a block holds
+static_assert(HEAD_ROW == MG_EVALUATE_STATS_WIDTH, "what a backward pass computes again, it need not be given");
 #define HEAD_FOUND 5  // doubles per part in the workspace: M, Z, sum d exp(-d), bad, first column of M
 
 extern int mg_fail_msg(const std::string& m);  // mettagrid_hip.hip: sets mg_last_error(), returns 1
@@ -326,10 +328,28 @@ struct HeadRaw {
 
 __device__ __forceinline__ int head_lane() { return threadIdx.x & 63; }
 
-// over the `lanes` (a power of two) lanes of a group; every lane gets the result
+// x of the lane that DPP control C names (within 16 lanes, or from one row of 16 to others); `none` where there is none
+template <int C, typename V>
+__device__ __forceinline__ V head_dpp(V x, V none) {
+  if constexpr (sizeof(V) == 4) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, x), C, 0xF, 0xF, false));
+  } else {
+    const long long xs = __builtin_bit_cast(long long, x), ns = __builtin_bit_cast(long long, none);
+    const unsigned lo = __builtin_amdgcn_update_dpp((int)ns, (int)xs, C, 0xF, 0xF, false);
+    const unsigned hi = __builtin_amdgcn_update_dpp((int)(ns >> 32), (int)(xs >> 32), C, 0xF, 0xF, false);
+    return __builtin_bit_cast(V, (long long)hi << 32 | lo);
+  }
+}
+// over the `lanes` (a power of two) lanes of a group; every lane gets the result.  (Pairs, quads, then mirrors within 8 and
+// 16 lanes: what is mirrored is the same in each half by then.)
 template <typename V, typename F>
 __device__ __forceinline__ V head_group(V x, int lanes, F f) {
-  for (int o = 1; o < lanes; o <<= 1) x = f(x, __shfl_xor(x, o));
+  if (lanes > 1) x = f(x, head_dpp<0xB1>(x, x));
+  if (lanes > 2) x = f(x, head_dpp<0x4E>(x, x));
+  if (lanes > 4) x = f(x, head_dpp<0x141>(x, x));
+  if (lanes > 8) x = f(x, head_dpp<0x140>(x, x));
+  if (lanes > 16) x = f(x, __shfl_xor(x, 16));
+  if (lanes > 32) x = f(x, __shfl_xor(x, 32));
   return x;
 }
 template <typename V>
@@ -347,9 +367,19 @@ __device__ __forceinline__ V head_group_sum(V x, int lanes) {
 // the sum of the lanes before this one in its group
 __device__ __forceinline__ double head_group_before(double x, int lanes, int lane) {
   double sum = x;
-  for (int o = 1; o < lanes; o <<= 1) {
-    const double up = __shfl_up(sum, o);
-    if (lane >= o) sum += up;
+  auto add = [&](double up, int o) { sum += lane >= o ? up : 0.0; };
+  if (lanes > 1) add(head_dpp<0x111>(sum, 0.0), 1);
+  if (lanes > 2) add(head_dpp<0x112>(sum, 0.0), 2);
+  if (lanes > 4) add(head_dpp<0x114>(sum, 0.0), 4);
+  if (lanes > 8) add(head_dpp<0x118>(sum, 0.0), 8);
+  // (so far within rows of 16 lanes: now the whole of the rows before)
+  if (lanes > 16) {
+    const double row = __shfl(sum, (head_lane() & 48) - 1);  // (read by all lanes: those that are off hold nothing to read)
+    sum += lane & 16 ? row : 0.0;
+  }
+  if (lanes > 32) {
+    const double half = __shfl(sum, 31);
+    sum += lane & 32 ? half : 0.0;
   }
   return sum - x;
 }
@@ -431,10 +461,12 @@ __device__ __forceinline__ void head_count_rows(const HeadArgs& a, const HeadNar
   __syncthreads();
 }
 
-// What the lanes of a row know of it.  ONE: a lane per row, of exactly E columns.
-template <int E, bool ONE, typename X>
+// What the lanes of a row know of it.  ONE: a lane per row, of exactly E columns.  X: the type of x, W: of what comes after
+// the difference from the largest (64 bits for x alone are enough where large logits and biases or penalties could cancel).
+template <int E, bool ONE, typename X, typename W>
 struct HeadHeld {
-  X x[E], t[E], w[E], m, z, s, z_lane;  // t = M - x, w = its weight; t and w say nothing where the row is bad or empty
+  X x[E], m;
+  W t[E], w[E], z, s, z_lane;  // t = M - x, w = its weight; t and w say nothing where the row is bad or empty
   float slope[E];
   unsigned ok;
   long row;         // clamped: the groups behind the last row do that row's work once more
@@ -451,7 +483,7 @@ struct HeadHeld {
   }
 
   template <bool GRAD>
-  __device__ __forceinline__ void hold(const HeadArgs& a, const HeadNarrow& g, const HeadRow& r, const HeadScale<X>& scale, const unsigned* counts) {
+  __device__ __forceinline__ void hold(const HeadArgs& a, const HeadNarrow& g, const HeadRow& r, const HeadScale<W>& scale, const unsigned* counts) {
     constexpr bool adjust = std::is_same<X, double>::value;
     HeadRaw<E> raw;
     raw.template fetch<ONE, adjust>(r, a.logits, a.type, row * a.logits_row + v0, v0, n);
@@ -464,15 +496,16 @@ struct HeadHeld {
     z = s = 0;
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      t[e] = head_finite(top - x[e]);
-      w[e] = scale.weight(top - x[e]);
+      const W far = (W)(top - x[e]);
+      t[e] = head_finite(far);
+      w[e] = scale.weight(far);
       z += w[e];
       s = head_fma(t[e], w[e], s);
     }
     z_lane = z;
     if (!ONE) {
-      z = head_group(z, g.lanes, [](X p, X q) { return p + q; });
-      s = head_group(s, g.lanes, [](X p, X q) { return p + q; });
+      z = head_group_sum(z, g.lanes);
+      s = head_group_sum(s, g.lanes);
     }
     s *= scale.inv_temp;
     // +infinity is the largest, NaN has lost to everything but makes the sum NaN
@@ -487,7 +520,7 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_adjust_narrow_kernel(HeadArgs
   __shared__ unsigned counts[HEAD_THREADS][E + 1];
   for (long row0 = (long)blockIdx.x * g.rows; row0 < a.rows; row0 += (long)gridDim.x * g.rows) {
     if (a.history) head_count_rows<E>(a, g, row0, counts);
-    HeadHeld<E, false, double> h;
+    HeadHeld<E, false, double, double> h;
     h.place(a, g, row0);
     if (!h.mine) continue;
     const HeadRow r = head_row(a, h.row);
@@ -504,7 +537,7 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_sample_narrow_kernel(HeadArgs
   __shared__ unsigned counts[HEAD_THREADS][E + 1];
   for (long row0 = (long)blockIdx.x * g.rows; row0 < a.rows; row0 += (long)gridDim.x * g.rows) {
     if (a.history) head_count_rows<E>(a, g, row0, counts);
-    HeadHeld<E, ONE, double> h;
+    HeadHeld<E, ONE, double, double> h;
     h.place(a, g, row0);
     const HeadRow r = head_row(a, h.row);
     const HeadScale<double> scale(r);
@@ -552,18 +585,18 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_kernel(HeadAr
     if constexpr (adjust) {
       if (a.history) head_count_rows<E>(a, g, row0, counts);
     }
-    HeadHeld<E, ONE, X> h;
+    HeadHeld<E, ONE, X, float> h;
     h.place(a, g, row0);
     const HeadRow r = head_row(a, h.row);
-    const HeadScale<X> scale(r);
+    const HeadScale<float> scale(r);
     const int act = actions[h.row];
     h.template hold<false>(a, g, r, scale, counts[adjust ? threadIdx.x : 0]);
-    X d = INFINITY;
+    float d = INFINITY;
 #pragma unroll
-    for (int e = 0; e < E; e++) d = h.v0 + e == act && e < h.n ? (h.x[e] == (X)-INFINITY ? (X)INFINITY : h.t[e] * scale.inv_temp) : d;
+    for (int e = 0; e < E; e++) d = h.v0 + e == act && e < h.n ? (h.x[e] == (X)-INFINITY ? (float)INFINITY : h.t[e] * scale.inv_temp) : d;
     if (!ONE) d = head_group_min(d, g.lanes);
     if (h.mine && h.lane == 0) {
-      const X log_z = head_log(h.z);
+      const float log_z = head_log(h.z);
       log_prob[h.row] = h.bad ? NAN : h.empty ? 0.f : (float)(-d - log_z);
       entropy[h.row] = h.bad ? NAN : h.empty ? 0.f : (float)(log_z + h.s * head_inverse(h.z));
     }
@@ -581,27 +614,27 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_backward_kern
     if constexpr (adjust) {
       if (a.history) head_count_rows<E>(a, g, row0, counts);
     }
-    HeadHeld<E, ONE, X> h;
+    HeadHeld<E, ONE, X, float> h;
     h.place(a, g, row0);
     const HeadRow r = head_row(a, h.row);
-    const HeadScale<X> scale(r);
+    const HeadScale<float> scale(r);
     const int act = actions[h.row];
-    const X gp_row = dlog_prob ? dlog_prob[h.row] : 0.f, gh = (dentropy ? dentropy[h.row] : 0.f) * scale.inv_temp;
+    const float gp_row = dlog_prob ? dlog_prob[h.row] : 0.f, gh = (dentropy ? dentropy[h.row] : 0.f) * scale.inv_temp;
     h.template hold<true>(a, g, r, scale, counts[adjust ? threadIdx.x : 0]);
     bool left = false;  // whether the action is a token that is left
 #pragma unroll
     for (int e = 0; e < E; e++) left = left || (h.v0 + e == act && e < h.n && h.x[e] > (X)-INFINITY);
     if (!ONE) left = head_group_max((int)left, g.lanes) != 0;
     // (a bad row's NaN reaches every token that is left)
-    const X gp = h.bad ? (X)NAN : left ? gp_row * scale.inv_temp : (X)0, inv_z = head_inverse(h.z);
-    const X past = h.s * inv_z;  // H - log Z: H + log q = past - t / temperature
+    const float gp = h.bad ? NAN : left ? gp_row * scale.inv_temp : 0.f, inv_z = head_inverse(h.z);
+    const float past = h.s * inv_z;  // H - log Z: H + log q = past - t / temperature
     float y[E];
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      const X q = h.w[e] * inv_z;
-      X d = (h.v0 + e == act ? gp : (X)0) - q * head_fma(gh, past - h.t[e] * scale.inv_temp, gp);
-      if (std::is_same<X, double>::value) d *= h.slope[e];
-      y[e] = h.x[e] != (X)-INFINITY ? (float)d : 0.f;
+      const float q = h.w[e] * inv_z;
+      float d = (h.v0 + e == act ? gp : 0.f) - q * head_fma(gh, past - h.t[e] * scale.inv_temp, gp);
+      if (adjust) d *= h.slope[e];
+      y[e] = h.x[e] != (X)-INFINITY ? d : 0.f;
     }
     if (h.mine) head_store<E>(dlogits, a.type, h.row * a.width + h.v0, h.n, y);
   }
@@ -613,29 +646,16 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_backward_kern
 // counts of the n columns from v0 on, all threads together; barriers inside
 __device__ __forceinline__ void head_count_columns(const HeadArgs& a, long row, unsigned* counts, long v0, int n) {
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += HEAD_THREADS) counts[i] = 0;
+  for (int i = threadIdx.x; i < n; i += blockDim.x) counts[i] = 0;
   __syncthreads();
   const int* h = a.history + row * a.history_row;
-  for (int i = threadIdx.x; i < a.history_len; i += HEAD_THREADS) {
+  for (int i = threadIdx.x; i < a.history_len; i += blockDim.x) {
     const long v = (long)h[i] - v0;
     if (h[i] >= 0 && v >= 0 && v < n) atomicAdd(&counts[v], 1u);
   }
   __syncthreads();
 }
 
-// x of the lane that DPP control C names (row_shr 1 ... 8 within 16 lanes, then the last lane of a row of 16 to the next
-// row, and of the first 32 lanes to the others); `none` where there is none
-template <int C, typename V>
-__device__ __forceinline__ V head_dpp(V x, V none) {
-  if constexpr (sizeof(V) == 4) {
-    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, x), C, 0xF, 0xF, false));
-  } else {
-    const long long xs = __builtin_bit_cast(long long, x), ns = __builtin_bit_cast(long long, none);
-    const unsigned lo = __builtin_amdgcn_update_dpp((int)ns, (int)xs, C, 0xF, 0xF, false);
-    const unsigned hi = __builtin_amdgcn_update_dpp((int)(ns >> 32), (int)(xs >> 32), C, 0xF, 0xF, false);
-    return __builtin_bit_cast(V, (long long)hi << 32 | lo);
-  }
-}
 // lane l: f over lanes 0 ... l
 template <typename V, typename F>
 __device__ __forceinline__ V head_scan(V x, V none, F f) {
@@ -699,6 +719,7 @@ __device__ __forceinline__ double head_block_before(double x, double* red, doubl
 // A part is CHUNKS * HEAD_CHUNK columns.
 #define HEAD_PART_COUNTS()                                                                      \
   __shared__ unsigned counts[CHUNKS * HEAD_CHUNK];                                              \
+  constexpr int THREADS [[maybe_unused]] = HEAD_THREADS;                                        \
   const long part0 = (long)blockIdx.x * (CHUNKS * HEAD_CHUNK);                                  \
   const int part_n = (int)min((long)CHUNKS * HEAD_CHUNK, a.width - part0);                      \
   if (a.history) head_count_columns(a, row, counts, part0, part_n);
@@ -706,16 +727,16 @@ __device__ __forceinline__ double head_block_before(double x, double* red, doubl
 // `fetch` for every chunk c of the part, whose columns of this thread start at `at` with n of them left; FULL says whether
 // the part lies in the row as a whole
 #define HEAD_PART_FETCH(fetch)                                                                  \
-  if (part_n == CHUNKS * HEAD_CHUNK) {                                                          \
+  if (part_n == CHUNKS * THREADS * 8) {                                                         \
     constexpr bool FULL = true;                                                                 \
     _Pragma("unroll") for (int c = 0; c < CHUNKS; c++) {                                        \
-      const int at = c * HEAD_CHUNK + threadIdx.x * 8, n = 8;                                   \
+      const int at = (c * THREADS + threadIdx.x) * 8, n = 8;                                    \
       fetch;                                                                                    \
     }                                                                                           \
   } else {                                                                                      \
     constexpr bool FULL = false;                                                                \
     _Pragma("unroll") for (int c = 0; c < CHUNKS; c++) {                                        \
-      const int at = c * HEAD_CHUNK + threadIdx.x * 8, n = part_n - at;                         \
+      const int at = (c * THREADS + threadIdx.x) * 8, n = part_n - at;                          \
       fetch;                                                                                    \
     }                                                                                           \
   }
@@ -736,56 +757,200 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_adjust_wide_kernel(HeadArgs a
   }
 }
 
-// what a part knows: found[row][part] = M, Z, sum (M - x) exp(-d) / temperature (against its own M), bad, first column of M
-template <int CHUNKS, bool FIRST, typename X>
-__global__ __launch_bounds__(HEAD_THREADS) void mg_head_parts_kernel(HeadArgs a, double* __restrict__ found) {
-  __shared__ X red[HEAD_THREADS / 64], red_s[HEAD_THREADS / 64];
-  __shared__ int red_int[HEAD_THREADS / 64];
-  for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
-    HEAD_PART_COUNTS()
-    const HeadRow r = head_row(a, row);
-    const HeadScale<X> scale(r);
-    constexpr bool adjust = std::is_same<X, double>::value;
-    X x[CHUNKS][8], m = -INFINITY;
+// What a block of THREADS knows of a part of CHUNKS * THREADS * 8 columns (X, W: as for narrow rows).
+struct HeadRed {
+  double d[2][16];
+  int i[16];
+};
+template <int CHUNKS, int THREADS, typename X, typename W>
+struct HeadPart {
+  static constexpr bool adjust = std::is_same<X, double>::value;
+  X x[CHUNKS][8], m;
+  W w[CHUNKS][8], z, s;  // s = sum (M - x) exp(-d) / temperature
+  float slope[CHUNKS][8];
+  unsigned ok[CHUNKS];
+  bool bad, empty;
+
+  __device__ __forceinline__ W far(int c, int e) const { return (W)(top() - x[c][e]); }
+  __device__ __forceinline__ X top() const { return m < (X)INFINITY && m > (X)-INFINITY ? m : (X)0; }
+  static __device__ __forceinline__ int at(int c) { return (c * THREADS + threadIdx.x) * 8; }
+
+  template <bool GRAD>
+  __device__ __forceinline__ void hold(const HeadArgs& a, const HeadRow& r, const HeadScale<W>& scale, long row, long part0, int part_n,
+                                       const unsigned* counts, HeadRed& red) {
     HeadRaw<8> raw[CHUNKS];
     HEAD_PART_FETCH((raw[c].template fetch<FULL, adjust>(r, a.logits, a.type, row * a.logits_row + part0 + at, (int)(part0 + at), n)))
+    m = -INFINITY;
 #pragma unroll
     for (int c = 0; c < CHUNKS; c++) {
-      const int at = c * HEAD_CHUNK + threadIdx.x * 8, n = part_n - at;
-      raw[c].template columns<false, false, adjust>(r, a.type, (int)(part0 + at), n, counts + at, x[c], (float*)nullptr);
-    }
-#pragma unroll
-    for (int c = 0; c < CHUNKS; c++) {
+      ok[c] = raw[c].template columns<false, GRAD, adjust>(r, a.type, (int)(part0 + at(c)), part_n - at(c), counts + at(c), x[c], slope[c]);
 #pragma unroll
       for (int e = 0; e < 8; e++) m = head_max(m, x[c][e]);
     }
-    const X most = head_block<X>(m, -INFINITY, red, [](X p, X q) { return head_max(p, q); });
-    const X top = most < (X)INFINITY && most > (X)-INFINITY ? most : (X)0;
-    X z = 0, s = 0;
-    int first = 0x7FFFFFFF;
+    m = head_block<X>(m, -INFINITY, (X*)red.d[0], [](X p, X q) { return head_max(p, q); });
+    z = s = 0;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; c++) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        w[c][e] = scale.weight(far(c, e));
+        z += w[c][e];
+        s = head_fma(head_finite(far(c, e)), w[c][e], s);
+      }
+    }
+    auto add = [](W p, W q) { return p + q; };
+    z = head_lane_of(head_scan<W>(z, 0, add), 63);
+    s = head_lane_of(head_scan<W>(s, 0, add), 63);
+    __syncthreads();
+    if (head_lane() == 0) red.d[0][threadIdx.x >> 6] = z, red.d[1][threadIdx.x >> 6] = s;
+    __syncthreads();
+    z = s = 0;
+    for (int k = 0; k < THREADS / 64; k++) z += (W)red.d[0][k], s += (W)red.d[1][k];
+    s *= scale.inv_temp;
+    // +infinity is the largest, NaN has lost to everything but makes the sum NaN
+    bad = !(m < (X)INFINITY) || z != z;
+    empty = !bad && m == (X)-INFINITY;
+  }
+  // the first column of the largest
+  __device__ __forceinline__ int first(long part0, HeadRed& red) const {
+    int v = 0x7FFFFFFF;
 #pragma unroll
     for (int c = CHUNKS - 1; c >= 0; c--) {
 #pragma unroll
-      for (int e = 7; e >= 0; e--) {
-        const X t = top - x[c][e], w = scale.weight(t);
-        z += w;
-        s = head_fma(head_finite(t), w, s);
-        if (FIRST && x[c][e] == most) first = (int)(part0 + c * HEAD_CHUNK + threadIdx.x * 8 + e);
-      }
+      for (int e = 7; e >= 0; e--)
+        if (x[c][e] == m) v = (int)(part0 + at(c) + e);
     }
-    auto add = [](X p, X q) { return p + q; };
-    z = head_lane_of(head_scan<X>(z, 0, add), 63);
-    s = head_lane_of(head_scan<X>(s, 0, add), 63);
-    __syncthreads();
-    if (head_lane() == 0) red[threadIdx.x >> 6] = z, red_s[threadIdx.x >> 6] = s;
-    if (FIRST) first = head_block_min(first, red_int);
-    else __syncthreads();
+    return head_block_min(v, red.i);
+  }
+};
+
+// ---- rows of up to HEAD_ROW columns: a block holds the row, eight columns per thread ------------------------------------
+
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void mg_sample_row_kernel(HeadArgs a, const float* __restrict__ uniforms, int* __restrict__ actions,
+                                                                    float* __restrict__ log_prob, float* __restrict__ entropy) {
+  __shared__ unsigned counts[THREADS * 8];
+  __shared__ HeadRed red;
+  __shared__ double picked;
+  for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    if (a.history) head_count_columns(a, row, counts, 0, a.width);
+    const HeadRow r = head_row(a, row);
+    const HeadScale<double> scale(r);
+    HeadPart<1, THREADS, double, double> h;
+    h.template hold<false>(a, r, scale, row, 0, a.width, counts, red);
+    int hit = -1;
+    double t = 0.0;
+    if (!h.bad && !h.empty && !uniforms) hit = h.first(0, red);
+    if (!h.bad && !h.empty && uniforms) {
+      const double target = fmax((double)uniforms[row], 0.0) * h.z;
+      int over = a.width, last = -1;  // this thread's first above the target, its last with any weight
+      double mine = 0.0, all;
+#pragma unroll
+      for (int e = 0; e < 8; e++) mine += h.w[0][e];
+      double run = head_block_before(mine, red.d[0], all);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        run += h.w[0][e];
+        if (run > target && over == a.width && h.at(0) + e < a.width) over = h.at(0) + e;
+        if (h.w[0][e] > 0.0) last = h.at(0) + e;
+      }
+      hit = head_block_min(over, red.i);
+      if (hit == a.width) hit = head_block_max(last, red.i);  // a uniform of 1 or more
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        if (h.at(0) + e == hit) picked = h.far(0, e);
+      __syncthreads();
+      t = picked;
+    }
     if (threadIdx.x == 0) {
-      double zz = 0.0, ss = 0.0;
-      for (int w = 0; w < HEAD_THREADS / 64; w++) zz += red[w], ss += red_s[w];
+      const double log_z = head_log(h.z);
+      actions[row] = h.bad || h.empty ? -1 : hit;
+      log_prob[row] = h.bad ? NAN : h.empty ? 0.f : (float)(-t * scale.inv_temp - log_z);
+      entropy[row] = h.bad ? NAN : h.empty ? 0.f : (float)(log_z + h.s * head_inverse(h.z));
+    }
+    __syncthreads();
+  }
+}
+
+template <int THREADS, typename X>
+__global__ __launch_bounds__(THREADS) void mg_evaluate_row_kernel(HeadArgs a, const int* __restrict__ actions, float* __restrict__ log_prob,
+                                                                      float* __restrict__ entropy) {
+  __shared__ unsigned counts[std::is_same<X, double>::value ? THREADS * 8 : 1];
+  __shared__ HeadRed red;
+  __shared__ float picked;
+  for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    if (std::is_same<X, double>::value && a.history) head_count_columns(a, row, counts, 0, a.width);
+    const HeadRow r = head_row(a, row);
+    const HeadScale<float> scale(r);
+    const int act = actions[row];
+    if (threadIdx.x == 0) picked = INFINITY;
+    HeadPart<1, THREADS, X, float> h;
+    h.template hold<false>(a, r, scale, row, 0, a.width, counts, red);
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      if (h.at(0) + e == act && act < a.width && h.x[0][e] != (X)-INFINITY) picked = h.far(0, e) * scale.inv_temp;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      const float log_z = head_log(h.z);
+      log_prob[row] = h.bad ? NAN : h.empty ? 0.f : -picked - log_z;
+      entropy[row] = h.bad ? NAN : h.empty ? 0.f : log_z + h.s * head_inverse(h.z);
+    }
+    __syncthreads();
+  }
+}
+
+template <int THREADS, typename X>
+__global__ __launch_bounds__(THREADS) void mg_evaluate_row_backward_kernel(HeadArgs a, const int* __restrict__ actions,
+                                                                               const float* __restrict__ dlog_prob,
+                                                                               const float* __restrict__ dentropy, void* __restrict__ dlogits) {
+  constexpr bool adjust = std::is_same<X, double>::value;
+  __shared__ unsigned counts[adjust ? THREADS * 8 : 1];
+  __shared__ HeadRed red;
+  __shared__ int left;  // whether the action is a token that is left
+  for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    if (adjust && a.history) head_count_columns(a, row, counts, 0, a.width);
+    const HeadRow r = head_row(a, row);
+    const HeadScale<float> scale(r);
+    const int act = actions[row];
+    const float gp_row = dlog_prob ? dlog_prob[row] : 0.f, gh = (dentropy ? dentropy[row] : 0.f) * scale.inv_temp;
+    if (threadIdx.x == 0) left = 0;
+    HeadPart<1, THREADS, X, float> h;
+    h.template hold<true>(a, r, scale, row, 0, a.width, counts, red);
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      if (h.at(0) + e == act && act < a.width && h.x[0][e] > (X)-INFINITY) left = 1;
+    __syncthreads();
+    // (a bad row's NaN reaches every token that is left)
+    const float gp = h.bad ? NAN : left ? gp_row * scale.inv_temp : 0.f, inv_z = head_inverse(h.z), past = h.s * inv_z;
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const float q = h.w[0][e] * inv_z;
+      float d = (h.at(0) + e == act ? gp : 0.f) - q * head_fma(gh, past - head_finite(h.far(0, e)) * scale.inv_temp, gp);
+      if (adjust) d *= h.slope[0][e];
+      y[e] = h.x[0][e] != (X)-INFINITY ? d : 0.f;
+    }
+    if (h.at(0) < a.width) head_store<8>(dlogits, a.type, row * a.width + h.at(0), a.width - h.at(0), y);
+    __syncthreads();
+  }
+}
+
+// ---- wider rows: parts, and a second launch that joins them ------------------------------------------------------------
+
+// found[row][part] = M, Z, sum (M - x) exp(-d) / temperature (against the part's own M), bad, first column of M
+template <int CHUNKS, bool FIRST, typename X, typename W>
+__global__ __launch_bounds__(HEAD_THREADS) void mg_head_parts_kernel(HeadArgs a, double* __restrict__ found) {
+  __shared__ HeadRed red;
+  for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    HEAD_PART_COUNTS()
+    const HeadRow r = head_row(a, row);
+    const HeadScale<W> scale(r);
+    HeadPart<CHUNKS, HEAD_THREADS, X, W> h;
+    h.template hold<false>(a, r, scale, row, part0, part_n, counts, red);
+    const int first = FIRST ? h.first(part0, red) : 0;
+    if (threadIdx.x == 0) {
       double* f = found + (row * gridDim.x + blockIdx.x) * HEAD_FOUND;
-      // +infinity is the largest, NaN has lost to everything but makes the sum NaN
-      f[0] = most; f[1] = zz; f[2] = ss * scale.inv_temp; f[3] = !(most < (X)INFINITY) || zz != zz ? 1.0 : 0.0; f[4] = first;
+      f[0] = h.m; f[1] = h.z; f[2] = h.s; f[3] = h.bad ? 1.0 : 0.0; f[4] = first;
     }
     __syncthreads();
   }
@@ -953,14 +1118,14 @@ __global__ __launch_bounds__(HEAD_THREADS, (sizeof(X) == 4 ? 4 : 2)) void mg_eva
   for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
     HEAD_PART_COUNTS()
     const HeadRow r = head_row(a, row);
-    const HeadScale<X> scale(r);
+    const HeadScale<float> scale(r);
     const double m = stats[2 * row];
-    const X log_z = (X)stats[2 * row + 1], past = (X)((double)entropy[row] - stats[2 * row + 1]);  // H + log q = past - t / temperature
+    const float log_z = (float)stats[2 * row + 1], past = (float)((double)entropy[row] - stats[2 * row + 1]);  // H + log q = past - t / temperature
     const bool bad = m != m, empty = m == -INFINITY;
     const X top = bad || empty ? (X)0 : (X)m;
     const int act = actions[row];
-    X gp = 0;
-    const X gh = (dentropy ? dentropy[row] : 0.f) * scale.inv_temp;
+    float gp = 0;
+    const float gh = (dentropy ? dentropy[row] : 0.f) * scale.inv_temp;
     if (dlog_prob && act >= 0 && act < a.width) {  // the action's token is left if it is allowed and not at -infinity
       HeadRow one = r;
       one.kind = 0;
@@ -978,12 +1143,12 @@ __global__ __launch_bounds__(HEAD_THREADS, (sizeof(X) == 4 ? 4 : 2)) void mg_eva
       const int at = c * HEAD_CHUNK + threadIdx.x * 8, n = part_n - at;
       if (n <= 0) continue;
       const int v0 = (int)(part0 + at);
-      X x[8], g[8];
-      float slope[8], y[8];
+      X x[8];
+      float g[8], slope[8], y[8];
       const unsigned ok = raw[c].template columns<false, true, adjust>(r, a.type, v0, n, counts + at, x, slope);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        const X t = top - x[e];
+        const float t = (float)(top - x[e]);
         g[e] = -scale.weight(t, log_z) * head_fma(gh, past - head_finite(t) * scale.inv_temp, gp);
       }
       if ((unsigned)(act - v0) < 8u) {
@@ -996,8 +1161,8 @@ __global__ __launch_bounds__(HEAD_THREADS, (sizeof(X) == 4 ? 4 : 2)) void mg_eva
       }
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        if (std::is_same<X, double>::value) g[e] *= slope[e];
-        y[e] = __uint_as_float(__float_as_uint((float)g[e]) & head_bit(ok, e));
+        if (adjust) g[e] *= slope[e];
+        y[e] = __uint_as_float(__float_as_uint(g[e]) & head_bit(ok, e));
       }
       head_store<8>(dlogits, a.type, row * a.width + v0, n, y);
     }
@@ -1032,11 +1197,13 @@ static HeadArgs head_args(const mg_logits* a) {
 
 // A part is four chunks where that leaves enough blocks to fill the GPU, else one.
 static int head_chunks(const mg_logits* a) {
-  return (int64_t)((a->width - 1) / (4 * HEAD_CHUNK) + 1) * a->rows >= 2048 ? 4 : 1;
+  return a->width > 2 * HEAD_CHUNK && (int64_t)((a->width - 1) / (4 * HEAD_CHUNK) + 1) * a->rows >= 2048 ? 4 : 1;
 }
 static int head_parts(const mg_logits* a) { return (a->width - 1) / (head_chunks(a) * HEAD_CHUNK) + 1; }
 static dim3 head_wide_grid(const mg_logits* a) { return dim3(head_parts(a), (unsigned)(a->rows < 32768 ? a->rows : 32768)); }
 static bool head_narrow(const mg_logits* a) { return a->width <= HEAD_NARROW; }
+static bool head_wide(const mg_logits* a) { return a->width > HEAD_ROW; }
+static unsigned head_row_blocks(const mg_logits* a) { return (unsigned)(a->rows < 1 << 20 ? a->rows : 1 << 20); }
 
 // lanes per row: as many as hold the row with E columns each; a power of two where they work on it together
 static HeadNarrow head_layout(const mg_logits* a, int e, bool together) {
@@ -1065,8 +1232,15 @@ static void head_by_width(const mg_logits* a, F f) {
     case 7: return f(head_int<7>(), one, g);
     case 8: return f(head_int<8>(), one, g);
   }
-  if (a->width <= 64 * 8) f(head_int<8>(), head_bool<false>(), head_layout(a, 8, true));
-  else f(head_int<16>(), head_bool<false>(), head_layout(a, 16, true));
+  f(head_int<8>(), head_bool<false>(), head_layout(a, 8, true));
+}
+// the threads of a block that holds a row
+template <typename F>
+static void head_by_row(const mg_logits* a, F f) {
+  if (a->width <= HEAD_CHUNK / 2) f(head_int<HEAD_THREADS / 2>());
+  else if (a->width <= HEAD_CHUNK) f(head_int<HEAD_THREADS>());
+  else if (a->width <= 2 * HEAD_CHUNK) f(head_int<2 * HEAD_THREADS>());
+  else f(head_int<4 * HEAD_THREADS>());
 }
 template <typename F>
 static void head_by_chunks(const mg_logits* a, F f) {
@@ -1085,13 +1259,13 @@ static int head_launched(const char* who) {
   return err == hipSuccess ? 0 : mg_fail_msg(std::string(who) + ": " + hipGetErrorString(err));
 }
 static int head_workspace(const char* who, const mg_logits* a) {
-  if (!head_narrow(a) && (!a->workspace || a->workspace_bytes < mg_logits_workspace(a)))
+  if (head_wide(a) && (!a->workspace || a->workspace_bytes < mg_logits_workspace(a)))
     return mg_fail_msg(std::string(who) + ": workspace smaller than mg_logits_workspace says");
   return 0;
 }
 
 extern "C" int64_t mg_logits_workspace(const mg_logits* a) {
-  if (!a || a->rows <= 0 || a->width < 1 || head_narrow(a)) return 0;
+  if (!a || a->rows <= 0 || a->width < 1 || !head_wide(a)) return 0;
   return a->rows * head_parts(a) * HEAD_FOUND * (int64_t)sizeof(double);
 }
 
@@ -1139,12 +1313,17 @@ extern "C" int mg_sample_actions(const mg_logits* a, const float* uniforms, int3
       hipLaunchKernelGGL((mg_sample_narrow_kernel<decltype(e)::value, decltype(one)::value>), dim3(head_blocks(a->rows, g.rows)), dim3(HEAD_THREADS), 0, s, head_args(a), g,
                          uniforms, actions, log_prob, entropy);
     });
+  } else if (!head_wide(a)) {
+    head_by_row(a, [&](auto c) {
+      hipLaunchKernelGGL(mg_sample_row_kernel<decltype(c)::value>, dim3(head_row_blocks(a)), dim3(decltype(c)::value), 0, s, head_args(a), uniforms,
+                         actions, log_prob, entropy);
+    });
   } else {
     head_by_chunks(a, [&](auto c) {
       constexpr int C = decltype(c)::value;
-      if (uniforms) hipLaunchKernelGGL((mg_head_parts_kernel<C, false, double>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), (double*)a->workspace);
-      else hipLaunchKernelGGL((mg_head_parts_kernel<C, true, double>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), (double*)a->workspace);
-      hipLaunchKernelGGL(mg_sample_join_kernel<C * HEAD_THREADS>, dim3((unsigned)(a->rows < 1 << 20 ? a->rows : 1 << 20)), dim3(C * HEAD_THREADS), 0, s,
+      if (uniforms) hipLaunchKernelGGL((mg_head_parts_kernel<C, false, double, double>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), (double*)a->workspace);
+      else hipLaunchKernelGGL((mg_head_parts_kernel<C, true, double, double>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), (double*)a->workspace);
+      hipLaunchKernelGGL(mg_sample_join_kernel<C * HEAD_THREADS>, dim3(head_row_blocks(a)), dim3(C * HEAD_THREADS), 0, s,
                          head_args(a), head_parts(a), (const double*)a->workspace, uniforms, actions, log_prob, entropy);
     });
   }
@@ -1168,13 +1347,18 @@ extern "C" int mg_evaluate_actions(const mg_logits* a, const int32_t* actions, f
         hipLaunchKernelGGL((mg_evaluate_narrow_kernel<decltype(e)::value, decltype(one)::value, X>), dim3(head_blocks(a->rows, g.rows)), dim3(HEAD_THREADS), 0, s,
                            head_args(a), g, actions, log_prob, entropy);
       });
+    } else if (!head_wide(a)) {
+      head_by_row(a, [&](auto c) {
+        hipLaunchKernelGGL((mg_evaluate_row_kernel<decltype(c)::value, X>), dim3(head_row_blocks(a)), dim3(decltype(c)::value), 0, s, head_args(a),
+                           actions, log_prob, entropy);
+      });
     } else {
       head_by_chunks(a, [&](auto c) {
-        hipLaunchKernelGGL((mg_head_parts_kernel<decltype(c)::value, false, X>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), (double*)a->workspace);
+        hipLaunchKernelGGL((mg_head_parts_kernel<decltype(c)::value, false, X, float>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), (double*)a->workspace);
       });
     }
   });
-  if (!head_narrow(a))
+  if (head_wide(a))
     hipLaunchKernelGGL(mg_evaluate_join_kernel, dim3((unsigned)((a->rows + 3) / 4)), dim3(HEAD_THREADS), 0, s, head_args(a), head_parts(a),
                        (const double*)a->workspace, actions, log_prob, entropy, stats);
   return head_launched(who);
@@ -1188,7 +1372,7 @@ extern "C" int mg_evaluate_actions_backward(const mg_logits* a, const int32_t* a
   static const char who[] = "mg_evaluate_actions_backward";
   if (const int rc = head_check(who, a)) return rc;
   if (!a->rows) return 0;
-  if (!actions || !dlogits || (!head_narrow(a) && (!entropy || !stats))) return mg_fail_msg(std::string(who) + ": NULL tensor");
+  if (!actions || !dlogits || (head_wide(a) && (!entropy || !stats))) return mg_fail_msg(std::string(who) + ": NULL tensor");
   const hipStream_t s = (hipStream_t)stream;
   head_by_controls(a, [&](auto* null) {
     using X = std::remove_pointer_t<decltype(null)>;
@@ -1196,6 +1380,11 @@ extern "C" int mg_evaluate_actions_backward(const mg_logits* a, const int32_t* a
       head_by_width(a, [&](auto e, auto one, HeadNarrow g) {
         hipLaunchKernelGGL((mg_evaluate_narrow_backward_kernel<decltype(e)::value, decltype(one)::value, X>), dim3(head_blocks(a->rows, g.rows)), dim3(HEAD_THREADS),
                            0, s, head_args(a), g, actions, dlog_prob, dentropy, dlogits);
+      });
+    else if (!head_wide(a))
+      head_by_row(a, [&](auto c) {
+        hipLaunchKernelGGL((mg_evaluate_row_backward_kernel<decltype(c)::value, X>), dim3(head_row_blocks(a)), dim3(decltype(c)::value), 0, s,
+                           head_args(a), actions, dlog_prob, dentropy, dlogits);
       });
     else
       head_by_chunks(a, [&](auto c) {

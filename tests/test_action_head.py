@@ -110,7 +110,8 @@ def _cuda(c):
     return {k: t.cuda() if torch.is_tensor(t) else t for k, t in c.items()}
 
 
-SHAPES = [(1, 1), (3, 2), (24, 5), (1000, 5), (65, 8), (33, 63), (17, 64), (9, 65), (40, 157), (7, 1000), (3, 4097), (2, 20001), (1, 131072), (300, 33)]  # fmt: skip
+SHAPES = [(1, 1), (3, 2), (24, 5), (1000, 5), (65, 8), (11, 9), (33, 63), (17, 64), (9, 65), (40, 157), (5, 512), (7, 513), (7, 1000), (3, 1025), (3, 2049),
+          (3, 4097), (2, 8192), (2, 8193), (2, 20001), (1, 131072), (300, 33), (257, 3), (130, 6), (64, 7), (65, 4)]  # fmt: skip
 
 # ---- refusals ------------------------------------------------------------------------------------------------------
 
@@ -281,6 +282,39 @@ def test_evaluate(shape, dtype):
             tol = err * slope + (fi.eps / 2 + 4 * U) * np.abs(want) + fi.smallest_normal * fi.eps / 2 + 1e-37
             off = np.abs(_np(d) - want)
             assert d.dtype == dtype and np.all(off <= tol), (which, k, np.max(off - tol))
+
+
+@pytest.mark.gpu
+def test_many_wide_rows():
+    """Enough rows beyond 8192 tokens that a block takes four times as many columns of each."""
+    n, v = 1030, 8300
+    logits, c, u = _case(n, v, torch.bfloat16, seed=7, length=40, scale=3.0)
+    l, slope = _adjusted(logits, **c)
+    dev = _cuda(c)
+    a, logp, h = sample_actions(logits.cuda(), u.cuda(), **dev)
+    want = _picked(l, _np(u))
+    assert np.array_equal(a.cpu().numpy(), want)
+    _check_rows(logp, h, l, want)
+    greedy, logp, h = sample_actions(logits.cuda(), **dev)
+    most = _picked(l, None)
+    assert np.array_equal(greedy.cpu().numpy(), most)
+    _check_rows(logp, h, l, most)
+    x = logits.cuda().requires_grad_()
+    logp, h = evaluate_actions(x, a, **dev)
+    _check_rows(logp, h, l, want)
+    (d,) = torch.autograd.grad(logp.sum() + h.sum(), x)
+    s = _stats(l)
+    logz, tol_h = _tol(s)
+    q = s["e"] / s["z"][:, None]
+    lq = np.where(q > 0, -np.where(np.isinf(s["d"]), 0, s["d"]) - np.log(s["z"])[:, None], 0.0)
+    hit = np.zeros_like(q)
+    hit[np.arange(n), np.clip(want, 0, v - 1)] = want >= 0
+    value = np.where(s["empty"][:, None], 0.0, (hit - q - q * (lq + s["h"][:, None])) * slope)
+    relq = 5 * U * np.abs(lq) + logz[:, None] + 8 * U
+    err = q * relq + 4 * U * hit + q * (relq * np.abs(lq + s["h"][:, None]) + 5 * U * np.abs(lq) + (logz + tol_h)[:, None] + 8 * U * (np.abs(lq) + s["h"][:, None]))
+    assert np.all(np.abs(_np(d) - value) <= err * slope + (2.0**-8 + 4 * U) * np.abs(value) + 1e-37)
+    out = adjust_logits(x, **dev)
+    _rounded(out, l, torch.bfloat16)
 
 
 @pytest.mark.gpu
