@@ -367,7 +367,7 @@ int mg_gated_recurrence_backward(const mg_recurrence* r, const float* marks, int
 #define MG_ALLOWED_BOOL 1
 #define MG_ALLOWED_BITS 2
 /* Rows up to this many tokens are held in registers: their backward pass wants neither stats nor entropy back. */
-#define MG_EVALUATE_STATS_WIDTH 8192
+#define MG_EVALUATE_STATS_WIDTH 1024
 typedef struct mg_logits {
   const void* logits;
   const float* bias;
@@ -381,7 +381,7 @@ typedef struct mg_logits {
   int32_t width, history_len, allowed_kind, type;
 } mg_logits;
 
-/* Bytes of workspace that mg_sample_actions and mg_evaluate_actions need (0 up to MG_EVALUATE_STATS_WIDTH tokens). */
+/* Bytes of workspace that mg_sample_actions and mg_evaluate_actions need (0 up to 8192 tokens). */
 int64_t mg_logits_workspace(const mg_logits* a);
 
 /* Adjusted logits, contiguous and of `type`; backward: dlogits = dout * d adjusted / d logits (0 where masked). */

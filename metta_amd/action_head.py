@@ -127,9 +127,9 @@ class _Head:
 
 def _workspace(args: native.MgLogits, device: torch.device) -> Optional[Tensor]:
     """Memory of this call's own (torch's allocator keeps it for the stream, and for a captured graph), set in `args`."""
-    if args.width <= native.STATS_WIDTH:
+    size = native.load().mg_logits_workspace(ct.byref(args)) if args.width > native.STATS_WIDTH else 0
+    if not size:
         return None
-    size = native.load().mg_logits_workspace(ct.byref(args))
     w = torch.empty(size, dtype=torch.uint8, device=device)
     args.workspace, args.workspace_bytes = w.data_ptr(), size
     return w

@@ -32,7 +32,7 @@
 #define HEAD_NARROW (64 * 8)  // the widest row that lanes of one wave hold
 #define HEAD_CHUNK (HEAD_THREADS * 8)  // columns that a block holds as 8 per thread
 #define HEAD_ROW (4 * HEAD_CHUNK)  // the widest row that a block holds
-static_assert(HEAD_ROW == MG_EVALUATE_STATS_WIDTH, "what a backward pass computes again, it need not be given");
+static_assert(HEAD_CHUNK / 2 == MG_EVALUATE_STATS_WIDTH, "a backward pass computes again what half a block holds");
 #define HEAD_FOUND 5  // doubles per part in the workspace: M, Z, sum d exp(-d), bad, first column of M
 
 extern int mg_fail_msg(const std::string& m);  // mettagrid_hip.hip: sets mg_last_error(), returns 1
@@ -872,10 +872,10 @@ __global__ __launch_bounds__(THREADS) void mg_sample_row_kernel(HeadArgs a, cons
   }
 }
 
-template <int THREADS, typename X>
+template <int CHUNKS, int THREADS, typename X>
 __global__ __launch_bounds__(THREADS) void mg_evaluate_row_kernel(HeadArgs a, const int* __restrict__ actions, float* __restrict__ log_prob,
-                                                                      float* __restrict__ entropy) {
-  __shared__ unsigned counts[std::is_same<X, double>::value ? THREADS * 8 : 1];
+                                                                 float* __restrict__ entropy, double* __restrict__ stats) {
+  __shared__ unsigned counts[std::is_same<X, double>::value ? CHUNKS * THREADS * 8 : 1];
   __shared__ HeadRed red;
   __shared__ float picked;
   for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -884,25 +884,30 @@ __global__ __launch_bounds__(THREADS) void mg_evaluate_row_kernel(HeadArgs a, co
     const HeadScale<float> scale(r);
     const int act = actions[row];
     if (threadIdx.x == 0) picked = INFINITY;
-    HeadPart<1, THREADS, X, float> h;
+    HeadPart<CHUNKS, THREADS, X, float> h;
     h.template hold<false>(a, r, scale, row, 0, a.width, counts, red);
 #pragma unroll
-    for (int e = 0; e < 8; e++)
-      if (h.at(0) + e == act && act < a.width && h.x[0][e] != (X)-INFINITY) picked = h.far(0, e) * scale.inv_temp;
+    for (int c = 0; c < CHUNKS; c++) {
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        if (h.at(c) + e == act && act < a.width && h.x[c][e] != (X)-INFINITY) picked = h.far(c, e) * scale.inv_temp;
+    }
     __syncthreads();
     if (threadIdx.x == 0) {
       const float log_z = head_log(h.z);
       log_prob[row] = h.bad ? NAN : h.empty ? 0.f : -picked - log_z;
       entropy[row] = h.bad ? NAN : h.empty ? 0.f : log_z + h.s * head_inverse(h.z);
+      if (stats) stats[2 * row] = h.bad ? NAN : (double)h.m, stats[2 * row + 1] = h.bad ? NAN : h.empty ? 0.0 : (double)log_z;
     }
     __syncthreads();
   }
 }
 
-template <int THREADS, typename X>
-__global__ __launch_bounds__(THREADS) void mg_evaluate_row_backward_kernel(HeadArgs a, const int* __restrict__ actions,
+template <typename X>
+__global__ __launch_bounds__(HEAD_THREADS / 2) void mg_evaluate_row_backward_kernel(HeadArgs a, const int* __restrict__ actions,
                                                                                const float* __restrict__ dlog_prob,
                                                                                const float* __restrict__ dentropy, void* __restrict__ dlogits) {
+  constexpr int CHUNKS = 1, THREADS = HEAD_THREADS / 2;
   constexpr bool adjust = std::is_same<X, double>::value;
   __shared__ unsigned counts[adjust ? THREADS * 8 : 1];
   __shared__ HeadRed red;
@@ -914,23 +919,29 @@ __global__ __launch_bounds__(THREADS) void mg_evaluate_row_backward_kernel(HeadA
     const int act = actions[row];
     const float gp_row = dlog_prob ? dlog_prob[row] : 0.f, gh = (dentropy ? dentropy[row] : 0.f) * scale.inv_temp;
     if (threadIdx.x == 0) left = 0;
-    HeadPart<1, THREADS, X, float> h;
+    HeadPart<CHUNKS, THREADS, X, float> h;
     h.template hold<true>(a, r, scale, row, 0, a.width, counts, red);
 #pragma unroll
-    for (int e = 0; e < 8; e++)
-      if (h.at(0) + e == act && act < a.width && h.x[0][e] > (X)-INFINITY) left = 1;
+    for (int c = 0; c < CHUNKS; c++) {
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        if (h.at(c) + e == act && act < a.width && h.x[c][e] > (X)-INFINITY) left = 1;
+    }
     __syncthreads();
     // (a bad row's NaN reaches every token that is left)
     const float gp = h.bad ? NAN : left ? gp_row * scale.inv_temp : 0.f, inv_z = head_inverse(h.z), past = h.s * inv_z;
-    float y[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const float q = h.w[0][e] * inv_z;
-      float d = (h.at(0) + e == act ? gp : 0.f) - q * head_fma(gh, past - head_finite(h.far(0, e)) * scale.inv_temp, gp);
-      if (adjust) d *= h.slope[0][e];
-      y[e] = h.x[0][e] != (X)-INFINITY ? d : 0.f;
+    for (int c = 0; c < CHUNKS; c++) {
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float q = h.w[c][e] * inv_z;
+        float d = (h.at(c) + e == act ? gp : 0.f) - q * head_fma(gh, past - head_finite(h.far(c, e)) * scale.inv_temp, gp);
+        if (adjust) d *= h.slope[c][e];
+        y[e] = h.x[c][e] != (X)-INFINITY ? d : 0.f;
+      }
+      if (h.at(c) < a.width) head_store<8>(dlogits, a.type, row * a.width + h.at(c), a.width - h.at(c), y);
     }
-    if (h.at(0) < a.width) head_store<8>(dlogits, a.type, row * a.width + h.at(0), a.width - h.at(0), y);
     __syncthreads();
   }
 }
@@ -1195,13 +1206,14 @@ static HeadArgs head_args(const mg_logits* a) {
   return g;
 }
 
-// A part is four chunks where that leaves enough blocks to fill the GPU, else one.
+// A part is four chunks where the row has more than two and that leaves enough blocks to fill the GPU, else one.
 static int head_chunks(const mg_logits* a) {
   return a->width > 2 * HEAD_CHUNK && (int64_t)((a->width - 1) / (4 * HEAD_CHUNK) + 1) * a->rows >= 2048 ? 4 : 1;
 }
 static int head_parts(const mg_logits* a) { return (a->width - 1) / (head_chunks(a) * HEAD_CHUNK) + 1; }
 static dim3 head_wide_grid(const mg_logits* a) { return dim3(head_parts(a), (unsigned)(a->rows < 32768 ? a->rows : 32768)); }
 static bool head_narrow(const mg_logits* a) { return a->width <= HEAD_NARROW; }
+static bool head_remembers(const mg_logits* a) { return a->width > MG_EVALUATE_STATS_WIDTH; }  // what the forward pass found
 static bool head_wide(const mg_logits* a) { return a->width > HEAD_ROW; }
 static unsigned head_row_blocks(const mg_logits* a) { return (unsigned)(a->rows < 1 << 20 ? a->rows : 1 << 20); }
 
@@ -1242,6 +1254,15 @@ static void head_by_row(const mg_logits* a, F f) {
   else if (a->width <= 2 * HEAD_CHUNK) f(head_int<2 * HEAD_THREADS>());
   else f(head_int<4 * HEAD_THREADS>());
 }
+// the chunks of a row that each thread of a smaller block holds: fewer threads to wait for, where 32 bits leave the registers
+// (4096 x 8192 bf16: 33 us with 256 threads, 56 with 1024)
+template <typename F>
+static void head_by_row_chunks(const mg_logits* a, F f) {
+  if (a->width <= HEAD_CHUNK / 2) f(head_int<1>(), head_int<HEAD_THREADS / 2>());
+  else if (a->width <= HEAD_CHUNK) f(head_int<1>(), head_int<HEAD_THREADS>());
+  else if (a->width <= 2 * HEAD_CHUNK) f(head_int<2>(), head_int<HEAD_THREADS>());
+  else f(head_int<4>(), head_int<HEAD_THREADS>());
+}
 template <typename F>
 static void head_by_chunks(const mg_logits* a, F f) {
   if (head_chunks(a) == 4) f(head_int<4>());
@@ -1271,7 +1292,7 @@ extern "C" int64_t mg_logits_workspace(const mg_logits* a) {
 
 static int head_adjust(const char* who, const mg_logits* a, void* out, const void* dout, void* dlogits, void* stream) {
   const hipStream_t s = (hipStream_t)stream;
-  if (head_narrow(a)) {
+  if (a->width <= HEAD_CHUNK / 2) {
     const HeadNarrow g = head_layout(a, 8, false);
     hipLaunchKernelGGL(mg_adjust_narrow_kernel<8>, dim3(head_blocks(a->rows, g.rows)), dim3(HEAD_THREADS), 0, s, head_args(a), g, out, dout, dlogits);
   } else {
@@ -1348,9 +1369,9 @@ extern "C" int mg_evaluate_actions(const mg_logits* a, const int32_t* actions, f
                            head_args(a), g, actions, log_prob, entropy);
       });
     } else if (!head_wide(a)) {
-      head_by_row(a, [&](auto c) {
-        hipLaunchKernelGGL((mg_evaluate_row_kernel<decltype(c)::value, X>), dim3(head_row_blocks(a)), dim3(decltype(c)::value), 0, s, head_args(a),
-                           actions, log_prob, entropy);
+      head_by_row_chunks(a, [&](auto c, auto t) {
+        hipLaunchKernelGGL((mg_evaluate_row_kernel<decltype(c)::value, decltype(t)::value, X>), dim3(head_row_blocks(a)), dim3(decltype(t)::value), 0,
+                           s, head_args(a), actions, log_prob, entropy, stats);
       });
     } else {
       head_by_chunks(a, [&](auto c) {
@@ -1372,7 +1393,7 @@ extern "C" int mg_evaluate_actions_backward(const mg_logits* a, const int32_t* a
   static const char who[] = "mg_evaluate_actions_backward";
   if (const int rc = head_check(who, a)) return rc;
   if (!a->rows) return 0;
-  if (!actions || !dlogits || (head_wide(a) && (!entropy || !stats))) return mg_fail_msg(std::string(who) + ": NULL tensor");
+  if (!actions || !dlogits || (head_remembers(a) && (!entropy || !stats))) return mg_fail_msg(std::string(who) + ": NULL tensor");
   const hipStream_t s = (hipStream_t)stream;
   head_by_controls(a, [&](auto* null) {
     using X = std::remove_pointer_t<decltype(null)>;
@@ -1381,11 +1402,9 @@ extern "C" int mg_evaluate_actions_backward(const mg_logits* a, const int32_t* a
         hipLaunchKernelGGL((mg_evaluate_narrow_backward_kernel<decltype(e)::value, decltype(one)::value, X>), dim3(head_blocks(a->rows, g.rows)), dim3(HEAD_THREADS),
                            0, s, head_args(a), g, actions, dlog_prob, dentropy, dlogits);
       });
-    else if (!head_wide(a))
-      head_by_row(a, [&](auto c) {
-        hipLaunchKernelGGL((mg_evaluate_row_backward_kernel<decltype(c)::value, X>), dim3(head_row_blocks(a)), dim3(decltype(c)::value), 0, s,
-                           head_args(a), actions, dlog_prob, dentropy, dlogits);
-      });
+    else if (!head_remembers(a))
+      hipLaunchKernelGGL(mg_evaluate_row_backward_kernel<X>, dim3(head_row_blocks(a)), dim3(HEAD_THREADS / 2), 0, s, head_args(a), actions,
+                         dlog_prob, dentropy, dlogits);
     else
       head_by_chunks(a, [&](auto c) {
         hipLaunchKernelGGL((mg_evaluate_wide_backward_kernel<decltype(c)::value, X>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), actions,

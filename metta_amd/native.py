@@ -96,7 +96,7 @@ class MgLogits(ct.Structure):
 
 
 MARK_STEPS = 16  # MG_RECURRENCE_MARK_STEPS
-STATS_WIDTH = 8192  # MG_EVALUATE_STATS_WIDTH
+STATS_WIDTH = 1024  # MG_EVALUATE_STATS_WIDTH
 ALLOWED_BOOL, ALLOWED_BITS = 1, 2  # MG_ALLOWED_*
 
 # name -> (restype, argtypes); every symbol include/mettagrid_hip.h declares
