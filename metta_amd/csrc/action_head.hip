@@ -114,6 +114,12 @@ template <> struct HeadScale<float> {
   __device__ __forceinline__ float weight(float t) const { return __builtin_amdgcn_exp2f(t * k); }
   __device__ __forceinline__ float weight(float t, float log_z) const { return __builtin_amdgcn_exp2f(fmaf(t, k, log_z * -1.44269504f)); }
 };
+// M - x in W, from values in X: in the wider of the two
+template <typename W, typename X>
+__device__ __forceinline__ W head_far(X m, X x) {
+  if constexpr (sizeof(W) > sizeof(X)) return (W)m - (W)x;
+  else return (W)(m - x);
+}
 __device__ __forceinline__ double head_fma(double a, double b, double c) { return fma(a, b, c); }
 __device__ __forceinline__ float head_fma(float a, float b, float c) { return fmaf(a, b, c); }
 __device__ __forceinline__ double head_max(double a, double b) { return fmax(a, b); }  // (a NaN loses)
@@ -496,7 +502,7 @@ struct HeadHeld {
     z = s = 0;
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      const W far = (W)(top - x[e]);
+      const W far = head_far<W, X>(top, x[e]);
       t[e] = head_finite(far);
       w[e] = scale.weight(far);
       z += w[e];
@@ -530,18 +536,21 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_adjust_narrow_kernel(HeadArgs
   }
 }
 
-template <int E, bool ONE>
+template <int E, bool ONE, typename X>
 __global__ __launch_bounds__(HEAD_THREADS) void mg_sample_narrow_kernel(HeadArgs a, HeadNarrow g, const float* __restrict__ uniforms,
                                                                        int* __restrict__ actions, float* __restrict__ log_prob,
                                                                        float* __restrict__ entropy) {
-  __shared__ unsigned counts[HEAD_THREADS][E + 1];
+  constexpr bool adjust = std::is_same<X, double>::value;
+  __shared__ unsigned counts[adjust ? HEAD_THREADS : 1][E + 1];
   for (long row0 = (long)blockIdx.x * g.rows; row0 < a.rows; row0 += (long)gridDim.x * g.rows) {
-    if (a.history) head_count_rows<E>(a, g, row0, counts);
-    HeadHeld<E, ONE, double, double> h;
+    if constexpr (adjust) {
+      if (a.history) head_count_rows<E>(a, g, row0, counts);
+    }
+    HeadHeld<E, ONE, X, double> h;
     h.place(a, g, row0);
     const HeadRow r = head_row(a, h.row);
     const HeadScale<double> scale(r);
-    h.template hold<false>(a, g, r, scale, counts[threadIdx.x]);
+    h.template hold<false>(a, g, r, scale, counts[adjust ? threadIdx.x : 0]);
     int hit = a.width, last = -1;
     if (uniforms) {
       const double target = fmax((double)uniforms[h.row], 0.0) * h.z;
@@ -718,11 +727,11 @@ __device__ __forceinline__ double head_block_before(double x, double* red, doubl
 
 // A part is CHUNKS * HEAD_CHUNK columns.
 #define HEAD_PART_COUNTS()                                                                      \
-  __shared__ unsigned counts[CHUNKS * HEAD_CHUNK];                                              \
+  __shared__ unsigned counts[ADJUST ? CHUNKS * HEAD_CHUNK : 1];                                 \
   constexpr int THREADS [[maybe_unused]] = HEAD_THREADS;                                        \
   const long part0 = (long)blockIdx.x * (CHUNKS * HEAD_CHUNK);                                  \
   const int part_n = (int)min((long)CHUNKS * HEAD_CHUNK, a.width - part0);                      \
-  if (a.history) head_count_columns(a, row, counts, part0, part_n);
+  if (ADJUST && a.history) head_count_columns(a, row, counts, part0, part_n);
 
 // `fetch` for every chunk c of the part, whose columns of this thread start at `at` with n of them left; FULL says whether
 // the part lies in the row as a whole
@@ -744,6 +753,7 @@ __device__ __forceinline__ double head_block_before(double x, double* red, doubl
 template <int CHUNKS>
 __global__ __launch_bounds__(HEAD_THREADS) void mg_adjust_wide_kernel(HeadArgs a, void* __restrict__ out, const void* __restrict__ dout,
                                                                      void* __restrict__ dlogits) {
+  constexpr bool ADJUST = true;
   for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
     HEAD_PART_COUNTS()
     const HeadRow r = head_row(a, row);
@@ -771,7 +781,7 @@ struct HeadPart {
   unsigned ok[CHUNKS];
   bool bad, empty;
 
-  __device__ __forceinline__ W far(int c, int e) const { return (W)(top() - x[c][e]); }
+  __device__ __forceinline__ W far(int c, int e) const { return head_far<W, X>(top(), x[c][e]); }
   __device__ __forceinline__ X top() const { return m < (X)INFINITY && m > (X)-INFINITY ? m : (X)0; }
   static __device__ __forceinline__ int at(int c) { return (c * THREADS + threadIdx.x) * 8; }
 
@@ -826,17 +836,18 @@ struct HeadPart {
 
 // ---- rows of up to HEAD_ROW columns: a block holds the row, eight columns per thread ------------------------------------
 
-template <int THREADS>
+template <int THREADS, typename X>
 __global__ __launch_bounds__(THREADS) void mg_sample_row_kernel(HeadArgs a, const float* __restrict__ uniforms, int* __restrict__ actions,
                                                                     float* __restrict__ log_prob, float* __restrict__ entropy) {
-  __shared__ unsigned counts[THREADS * 8];
+  constexpr bool adjust = std::is_same<X, double>::value;
+  __shared__ unsigned counts[adjust ? THREADS * 8 : 1];
   __shared__ HeadRed red;
   __shared__ double picked;
   for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    if (a.history) head_count_columns(a, row, counts, 0, a.width);
+    if (adjust && a.history) head_count_columns(a, row, counts, 0, a.width);
     const HeadRow r = head_row(a, row);
     const HeadScale<double> scale(r);
-    HeadPart<1, THREADS, double, double> h;
+    HeadPart<1, THREADS, X, double> h;
     h.template hold<false>(a, r, scale, row, 0, a.width, counts, red);
     int hit = -1;
     double t = 0.0;
@@ -951,6 +962,7 @@ __global__ __launch_bounds__(HEAD_THREADS / 2) void mg_evaluate_row_backward_ker
 // found[row][part] = M, Z, sum (M - x) exp(-d) / temperature (against the part's own M), bad, first column of M
 template <int CHUNKS, bool FIRST, typename X, typename W>
 __global__ __launch_bounds__(HEAD_THREADS) void mg_head_parts_kernel(HeadArgs a, double* __restrict__ found) {
+  constexpr bool ADJUST = std::is_same<X, double>::value;
   __shared__ HeadRed red;
   for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
     HEAD_PART_COUNTS()
@@ -995,12 +1007,13 @@ __device__ __forceinline__ HeadJoined head_join(const double* f, int parts, doub
 }
 
 // THREADS * 8 columns are a whole part
-template <int THREADS>
+template <int THREADS, typename X>
 __global__ __launch_bounds__(THREADS) void mg_sample_join_kernel(HeadArgs a, int parts, const double* __restrict__ found,
                                                                 const float* __restrict__ uniforms, int* __restrict__ actions,
                                                                 float* __restrict__ log_prob, float* __restrict__ entropy) {
   constexpr int PART = THREADS * 8;
-  __shared__ unsigned counts[PART];
+  constexpr bool adjust = std::is_same<X, double>::value;
+  __shared__ unsigned counts[adjust ? PART : 1];
   __shared__ double red[THREADS / 64], picked_t, picked_run;
   __shared__ int red_int[THREADS / 64], picked;
   for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -1042,15 +1055,16 @@ __global__ __launch_bounds__(THREADS) void mg_sample_join_kernel(HeadArgs a, int
       } else {
         const long part0 = (long)picked * PART;
         const int part_n = (int)min((long)PART, a.width - part0);
-        if (a.history) head_count_columns(a, row, counts, part0, part_n);
+        if (adjust && a.history) head_count_columns(a, row, counts, part0, part_n);
         const int at = threadIdx.x * 8, n = part_n - at;
-        double x[8], t[8], w[8], mine = 0.0;
+        X x[8];
+        double t[8], w[8], mine = 0.0;
         HeadRaw<8> raw;
-        raw.fetch<false, true>(r, a.logits, a.type, row * a.logits_row + part0 + at, (int)(part0 + at), n);
-        raw.columns<false, false, true>(r, a.type, (int)(part0 + at), n, counts + at, x, (float*)nullptr);
+        raw.template fetch<false, adjust>(r, a.logits, a.type, row * a.logits_row + part0 + at, (int)(part0 + at), n);
+        raw.template columns<false, false, adjust>(r, a.type, (int)(part0 + at), n, counts + at, x, (float*)nullptr);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-          t[e] = j.m - x[e];
+          t[e] = j.m - (double)x[e];
           w[e] = scale.weight(t[e]);
           mine += w[e];
         }
@@ -1126,6 +1140,7 @@ __global__ __launch_bounds__(HEAD_THREADS, (sizeof(X) == 4 ? 4 : 2)) void mg_eva
                                                                                 const float* __restrict__ dlog_prob,
                                                                                 const float* __restrict__ dentropy,
                                                                                 void* __restrict__ dlogits) {
+  constexpr bool ADJUST = std::is_same<X, double>::value;
   for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
     HEAD_PART_COUNTS()
     const HeadRow r = head_row(a, row);
@@ -1146,7 +1161,7 @@ __global__ __launch_bounds__(HEAD_THREADS, (sizeof(X) == 4 ? 4 : 2)) void mg_eva
       raw.values(a.type, l);
       if (head_allowed(r, act) && l[0] > -INFINITY && (!r.bias || r.bias[act] > -INFINITY)) gp = dlog_prob[row] * scale.inv_temp;
     }
-    constexpr bool adjust = std::is_same<X, double>::value;
+    constexpr bool adjust = ADJUST;
     HeadRaw<8> raw[CHUNKS];
     HEAD_PART_FETCH((raw[c].template fetch<FULL, adjust>(r, a.logits, a.type, row * a.logits_row + part0 + at, (int)(part0 + at), n)))
 #pragma unroll
@@ -1268,7 +1283,7 @@ static void head_by_chunks(const mg_logits* a, F f) {
   if (head_chunks(a) == 4) f(head_int<4>());
   else f(head_int<1>());
 }
-// the arithmetic of given actions: 64 bits where a bias or a penalty could cancel large logits
+// the type of the logits' values: 64 bits where there is a bias or a penalty, which could cancel large logits
 template <typename F>
 static void head_by_controls(const mg_logits* a, F f) {
   if (a->bias || a->history) f((double*)nullptr);
@@ -1329,25 +1344,30 @@ extern "C" int mg_sample_actions(const mg_logits* a, const float* uniforms, int3
   if (!actions || !log_prob || !entropy) return mg_fail_msg(std::string(who) + ": NULL tensor");
   if (const int rc = head_workspace(who, a)) return rc;
   const hipStream_t s = (hipStream_t)stream;
-  if (head_narrow(a)) {
-    head_by_width(a, [&](auto e, auto one, HeadNarrow g) {
-      hipLaunchKernelGGL((mg_sample_narrow_kernel<decltype(e)::value, decltype(one)::value>), dim3(head_blocks(a->rows, g.rows)), dim3(HEAD_THREADS), 0, s, head_args(a), g,
-                         uniforms, actions, log_prob, entropy);
-    });
-  } else if (!head_wide(a)) {
-    head_by_row(a, [&](auto c) {
-      hipLaunchKernelGGL(mg_sample_row_kernel<decltype(c)::value>, dim3(head_row_blocks(a)), dim3(decltype(c)::value), 0, s, head_args(a), uniforms,
-                         actions, log_prob, entropy);
-    });
-  } else {
-    head_by_chunks(a, [&](auto c) {
-      constexpr int C = decltype(c)::value;
-      if (uniforms) hipLaunchKernelGGL((mg_head_parts_kernel<C, false, double, double>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), (double*)a->workspace);
-      else hipLaunchKernelGGL((mg_head_parts_kernel<C, true, double, double>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), (double*)a->workspace);
-      hipLaunchKernelGGL(mg_sample_join_kernel<C * HEAD_THREADS>, dim3(head_row_blocks(a)), dim3(C * HEAD_THREADS), 0, s,
-                         head_args(a), head_parts(a), (const double*)a->workspace, uniforms, actions, log_prob, entropy);
-    });
-  }
+  head_by_controls(a, [&](auto* null) {
+    using X = std::remove_pointer_t<decltype(null)>;
+    if (head_narrow(a)) {
+      head_by_width(a, [&](auto e, auto one, HeadNarrow g) {
+        hipLaunchKernelGGL((mg_sample_narrow_kernel<decltype(e)::value, decltype(one)::value, X>), dim3(head_blocks(a->rows, g.rows)),
+                           dim3(HEAD_THREADS), 0, s, head_args(a), g, uniforms, actions, log_prob, entropy);
+      });
+    } else if (!head_wide(a)) {
+      head_by_row(a, [&](auto c) {
+        hipLaunchKernelGGL((mg_sample_row_kernel<decltype(c)::value, X>), dim3(head_row_blocks(a)), dim3(decltype(c)::value), 0, s, head_args(a),
+                           uniforms, actions, log_prob, entropy);
+      });
+    } else {
+      head_by_chunks(a, [&](auto c) {
+        constexpr int C = decltype(c)::value;
+        if (uniforms)
+          hipLaunchKernelGGL((mg_head_parts_kernel<C, false, X, double>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), (double*)a->workspace);
+        else
+          hipLaunchKernelGGL((mg_head_parts_kernel<C, true, X, double>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), (double*)a->workspace);
+        hipLaunchKernelGGL((mg_sample_join_kernel<C * HEAD_THREADS, X>), dim3(head_row_blocks(a)), dim3(C * HEAD_THREADS), 0, s, head_args(a),
+                           head_parts(a), (const double*)a->workspace, uniforms, actions, log_prob, entropy);
+      });
+    }
+  });
   return head_launched(who);
 } catch (...) {
   return 1;
