@@ -39,26 +39,24 @@ extern int mg_fail_msg(const std::string& m);  // mettagrid_hip.hip: sets mg_las
 
 // ---- arithmetic -------------------------------------------------------------------------------------------------------
 
-// e^-d for d >= 0 (NaN: NaN).  n = rint(y log2 e) with y = -d, r = y - n ln 2 in two parts, |r| <= 0.347: the series to
-// r^12 / 12! leaves 2e-16; 18 instructions, where the library's takes 40.
-__device__ __forceinline__ double head_exp(double d) {
-  const double n = rint(d * -1.4426950408889634);
-  double r = fma(n, -0.69314718055994529, -d);  // ln 2 = 0.69314718055994529 + 2.3190468138462996e-17
-  r = fma(n, -2.3190468138462996e-17, r);
-  double p = 1.0 / 479001600.0;
-  p = fma(p, r, 1.0 / 39916800.0);
-  p = fma(p, r, 1.0 / 3628800.0);
-  p = fma(p, r, 1.0 / 362880.0);
-  p = fma(p, r, 1.0 / 40320.0);
-  p = fma(p, r, 1.0 / 5040.0);
-  p = fma(p, r, 1.0 / 720.0);
-  p = fma(p, r, 1.0 / 120.0);
-  p = fma(p, r, 1.0 / 24.0);
-  p = fma(p, r, 1.0 / 6.0);
-  p = fma(p, r, 0.5);
+// 2^y for y <= 0: n = rint(y), and the series in (y - n) ln 2, |y - n| <= 1/2, to its 12th term, which leaves 2e-16.  (y of
+// less than -1075 gives 0.)  15 instructions, where the library's e^x takes 40.
+__device__ __forceinline__ double head_exp_two(double y) {
+  const double n = rint(y), r = y - n;
+  double p = 2.5678435993488196e-11;
+  p = fma(p, r, 4.44553827187081e-10);
+  p = fma(p, r, 7.054911620801121e-09);
+  p = fma(p, r, 1.0178086009239696e-07);
+  p = fma(p, r, 1.3215486790144305e-06);
+  p = fma(p, r, 1.5252733804059838e-05);
+  p = fma(p, r, 0.00015403530393381606);
+  p = fma(p, r, 0.0013333558146428441);
+  p = fma(p, r, 0.009618129107628477);
+  p = fma(p, r, 0.055504108664821576);
+  p = fma(p, r, 0.2402265069591007);
+  p = fma(p, r, 0.6931471805599453);
   p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
-  return d > 746.0 ? 0.0 : ldexp(p, (int)n);  // (the smallest denormal is e^-745)
+  return ldexp(p, (int)n);
 }
 
 // 1 / z; in 32 bits by the hardware's reciprocal and one Newton step
@@ -73,7 +71,7 @@ __device__ __forceinline__ float head_log(float z) { return logf(z); }
 // The call's arguments, with the quotients that every row wants (a 64-bit division costs a wave as much as a dozen tokens).
 struct HeadArgs : mg_logits {
   double inv_temp, inv_rep;
-  float weight_scale;  // -log2 e / temperature
+  double weight_scale;  // -log2 e / temperature
 };
 
 // One row's controls.
@@ -82,8 +80,7 @@ struct HeadRow {
   const void* allowed;
   int kind;
   bool counted;
-  double inv_rep, rep, presence, frequency, inv_temp;
-  float weight_scale;
+  double inv_rep, rep, presence, frequency, inv_temp, weight_scale;
 };
 
 __device__ __forceinline__ HeadRow head_row(const HeadArgs& a, long row) {
@@ -98,21 +95,26 @@ __device__ __forceinline__ HeadRow head_row(const HeadArgs& a, long row) {
   return r;
 }
 
-// What a row's exponentials and gradients are scaled by: weight(t) = exp(-t / temperature) for t = M - x.  In 32 bits the
-// scale and log2 e are one factor, and the hardware's exp2 does the rest: the difference, the factor and the product
-// round once each, 3 u t / temperature relative, plus the 2 u of exp2.
+// What a row's exponentials and gradients are scaled by.  weight(t) = exp(-t / temperature) for t = M - x: the scale and
+// log2 e are one factor.  In 32 bits the difference, the factor and the product round once each, 3 u t / temperature
+// relative, plus the 2 u of the hardware's exp2.  In 64 bits a NaN is not handed on (the caller looks for it).
+// sum() adds t / temperature times the weight, in units that finish() turns into those of the entropy; it stays finite
+// where t does not (its weight is 0 there).
 template <typename X> struct HeadScale;
 template <> struct HeadScale<double> {
-  double inv_temp;
-  __device__ explicit HeadScale(const HeadRow& r) : inv_temp(r.inv_temp) {}
-  __device__ __forceinline__ double weight(double t) const { return head_exp(t * inv_temp); }
-  __device__ __forceinline__ double weight(double t, double log_z) const { return head_exp(t * inv_temp + log_z); }
+  double inv_temp, k;
+  __device__ explicit HeadScale(const HeadRow& r) : inv_temp(r.inv_temp), k(r.weight_scale) {}
+  __device__ __forceinline__ double weight(double t) const { return head_exp_two(fmax(t * k, -2000.0)); }
+  __device__ __forceinline__ double sum(double t, double w, double s) const { return fma(fmax(t * k, -2000.0), w, s); }
+  __device__ __forceinline__ double finish(double s) const { return s * -0.69314718055994529; }
 };
 template <> struct HeadScale<float> {
   float inv_temp, k;
-  __device__ explicit HeadScale(const HeadRow& r) : inv_temp((float)r.inv_temp), k(r.weight_scale) {}
+  __device__ explicit HeadScale(const HeadRow& r) : inv_temp((float)r.inv_temp), k((float)r.weight_scale) {}
   __device__ __forceinline__ float weight(float t) const { return __builtin_amdgcn_exp2f(t * k); }
   __device__ __forceinline__ float weight(float t, float log_z) const { return __builtin_amdgcn_exp2f(fmaf(t, k, log_z * -1.44269504f)); }
+  __device__ __forceinline__ float sum(float t, float w, float s) const { return fmaf(fminf(t, 1e37f), w, s); }
+  __device__ __forceinline__ float finish(float s) const { return s * inv_temp; }
 };
 // M - x in W, from values in X: in the wider of the two
 template <typename W, typename X>
@@ -500,20 +502,23 @@ struct HeadHeld {
     if (!ONE) m = head_group(m, g.lanes, [](X p, X q) { return head_max(p, q); });
     const X top = m < (X)INFINITY && m > (X)-INFINITY ? m : (X)0;
     z = s = 0;
+    bool lost = false;  // a NaN
 #pragma unroll
     for (int e = 0; e < E; e++) {
       const W far = head_far<W, X>(top, x[e]);
       t[e] = head_finite(far);
       w[e] = scale.weight(far);
       z += w[e];
-      s = head_fma(t[e], w[e], s);
+      s = scale.sum(far, w[e], s);
+      if (sizeof(W) == 8) lost = lost || far != far;
     }
+    if (lost) z = NAN;
     z_lane = z;
     if (!ONE) {
       z = head_group_sum(z, g.lanes);
       s = head_group_sum(s, g.lanes);
     }
-    s *= scale.inv_temp;
+    s = scale.finish(s);
     // +infinity is the largest, NaN has lost to everything but makes the sum NaN
     bad = !(m < (X)INFINITY) || z != z;
     empty = !bad && m == (X)-INFINITY;
@@ -799,15 +804,19 @@ struct HeadPart {
     }
     m = head_block<X>(m, -INFINITY, (X*)red.d[0], [](X p, X q) { return head_max(p, q); });
     z = s = 0;
+    bool lost = false;  // a NaN
 #pragma unroll
     for (int c = 0; c < CHUNKS; c++) {
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        w[c][e] = scale.weight(far(c, e));
+        const W t = far(c, e);
+        w[c][e] = scale.weight(t);
         z += w[c][e];
-        s = head_fma(head_finite(far(c, e)), w[c][e], s);
+        s = scale.sum(t, w[c][e], s);
+        if (sizeof(W) == 8) lost = lost || t != t;
       }
     }
+    if (lost) z = NAN;
     auto add = [](W p, W q) { return p + q; };
     z = head_lane_of(head_scan<W>(z, 0, add), 63);
     s = head_lane_of(head_scan<W>(s, 0, add), 63);
@@ -816,7 +825,7 @@ struct HeadPart {
     __syncthreads();
     z = s = 0;
     for (int k = 0; k < THREADS / 64; k++) z += (W)red.d[0][k], s += (W)red.d[1][k];
-    s *= scale.inv_temp;
+    s = scale.finish(s);
     // +infinity is the largest, NaN has lost to everything but makes the sum NaN
     bad = !(m < (X)INFINITY) || z != z;
     empty = !bad && m == (X)-INFINITY;
@@ -982,7 +991,7 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_head_parts_kernel(HeadArgs a,
 struct HeadJoined { double m, z, s; bool bad, empty; };
 
 // the parts of a row, by all lanes of a wave
-__device__ __forceinline__ HeadJoined head_join(const double* f, int parts, double inv_temp, int lane) {
+__device__ __forceinline__ HeadJoined head_join(const double* f, int parts, const HeadScale<double>& scale, int lane) {
   HeadJoined j;
   double m = -INFINITY, bad = 0.0;
   for (int i = lane; i < parts; i += 64) {
@@ -997,7 +1006,7 @@ __device__ __forceinline__ HeadJoined head_join(const double* f, int parts, doub
     for (int i = lane; i < parts; i += 64) {
       const double mi = f[i * HEAD_FOUND];
       if (mi == -INFINITY) continue;
-      const double d = (j.m - mi) * inv_temp, w = head_exp(d), zi = f[i * HEAD_FOUND + 1];
+      const double d = (j.m - mi) * scale.inv_temp, w = scale.weight(j.m - mi), zi = f[i * HEAD_FOUND + 1];
       z += w * zi;
       s += w > 0.0 ? w * (f[i * HEAD_FOUND + 2] + d * zi) : 0.0;
     }
@@ -1020,7 +1029,7 @@ __global__ __launch_bounds__(THREADS) void mg_sample_join_kernel(HeadArgs a, int
     const HeadRow r = head_row(a, row);
     const HeadScale<double> scale(r);
     const double* f = found + row * parts * HEAD_FOUND;
-    const HeadJoined j = head_join(f, parts, r.inv_temp, head_lane());
+    const HeadJoined j = head_join(f, parts, scale, head_lane());
     int hit = -1;
     double t_hit = 0.0;
     if (!j.bad && !j.empty) {
@@ -1106,7 +1115,7 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_join_kernel(HeadArgs
   const long row = ((long)blockIdx.x * HEAD_THREADS + threadIdx.x) >> 6;
   if (row >= a.rows) return;
   const HeadRow r = head_row(a, row);
-  const HeadJoined j = head_join(found + row * parts * HEAD_FOUND, parts, r.inv_temp, head_lane());
+  const HeadJoined j = head_join(found + row * parts * HEAD_FOUND, parts, HeadScale<double>(r), head_lane());
   const int act = actions[row];
   const bool inside = act >= 0 && act < a.width;
   double x = -INFINITY;
@@ -1217,7 +1226,7 @@ static HeadArgs head_args(const mg_logits* a) {
   (mg_logits&)g = *a;
   g.inv_temp = 1.0 / a->temperature;
   g.inv_rep = 1.0 / a->repetition;
-  g.weight_scale = (float)(g.inv_temp * -1.4426950408889634);
+  g.weight_scale = g.inv_temp * -1.4426950408889634;
   return g;
 }
 
