@@ -166,8 +166,7 @@ __global__ __launch_bounds__(256) void mg_recurrence_kernel(RecArgs a, T* __rest
       *(rec_vec<float, VEC>*)(mark + (t / REC_L - 1) * a.width) = m;
     }
     RecTile<T, VEC> o;
-#pragma unroll
-    for (int i = 0; i < REC_L; i++) {
+    auto step = [&](int i) {
 #pragma unroll
       for (int j = 0; j < VEC; j++) {
         float ga, gw;
@@ -176,6 +175,14 @@ __global__ __launch_bounds__(256) void mg_recurrence_kernel(RecArgs a, T* __rest
         s[j] = (rt[k] >> i) & 1 ? q : fmaf(ga, s[j], q);
         o.v[i][j] = (T)s[j];
       }
+    };
+    if (n == REC_L) {
+#pragma unroll
+      for (int i = 0; i < REC_L; i++) step(i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < REC_L; i++)
+        if (i < n) step(i);
     }
     if (out) rec_store<T, VEC>(o, out + t * a.width, a.width, n);
   };
@@ -578,17 +585,24 @@ static int rec_check(const char* who, const mg_recurrence* r) {
 }
 
 // How the work is laid out; a function of the shape alone, so that results do not depend on addresses.
-struct RecPlan { bool shared; unsigned tiles, tiles_each, splits; int vec; };
+struct RecPlan { bool shared; unsigned tiles, tiles_each, splits; };
 
 static RecPlan rec_plan(const mg_recurrence* r) {
-  RecPlan p{false, (unsigned)((r->steps + REC_TILE - 1) / REC_TILE), 0, 1, 2};
-  const int64_t waves = (r->rows * r->width + 127) / (r->type == MG_F32 ? 64 : 128);
-  p.shared = waves < 2048 && r->steps > REC_L;
-  if (p.shared && p.tiles >= 4) {
-    const int64_t want = (512 + waves - 1) / waves;
+  // 4 bytes per lane and step whatever the type: with two f32 columns per lane a block's registers leave room for no second
+  // one on a CU (1 x 65536 x 128: 45 us backward against 39; 2500 x 100 x 128: 154 against 138)
+  const bool f32 = r->type == MG_F32;
+  RecPlan p{false, (unsigned)((r->steps + REC_TILE - 1) / REC_TILE), 0, 1};
+  const int64_t each = f32 ? 64 : 128, waves = (r->rows * r->width + each - 1) / each;
+  // a walk through time needs five waves per CU (eight with f32's smaller loads) to keep the memory busy: 1500 x 170 x 128
+  // bf16 takes 55 us that way and 66 in tiles, 1024 x 256 x 128 53 and 54
+  p.shared = waves < (f32 ? 2048 : 1280) && r->steps > REC_L;
+  // time is cut only where there is less than a block per CU, since the pairs are the price of reading the inputs again
+  // (256 x 1024 x 128 bf16: 50 us in one launch, 87 cut in two), into as many blocks as are resident at a time: two per
+  // CU (f32) or one (1 x 65536 x 128 bf16: 30 us, with two 42)
+  if (p.shared && p.tiles >= 4 && waves < 256) {
+    const int64_t want = ((f32 ? 512 : 256) + waves - 1) / waves;
     p.splits = (unsigned)(want < p.tiles ? want : p.tiles);
   }
-  if (p.shared && r->type == MG_F32) p.vec = 1;
   p.tiles_each = (p.tiles + p.splits - 1) / p.splits;
   p.splits = (p.tiles + p.tiles_each - 1) / p.tiles_each;
   return p;
@@ -645,12 +659,24 @@ extern "C" int mg_gated_recurrence(const mg_recurrence* r, void* h, float* last,
   const hipStream_t s = (hipStream_t)stream;
   return rec_by_type(r->type, [&](auto* null) {
     using T = std::remove_pointer_t<decltype(null)>;
+    const int64_t e = sizeof(T);
+    auto fits = [&](int vec) {
+      return rec_fits(vec, e, r->width, {r->x, r->gate, h}, {r->state, last, marks}, {r->x_row, r->x_step, r->gate_row, r->gate_step});
+    };
+    auto step = [&](auto vec) {
+      constexpr int VEC = decltype(vec)::value;
+      const RecArgs a = rec_args(r, p, VEC);
+      hipLaunchKernelGGL((mg_recurrence_step_kernel<T, VEC>), dim3((a.groups + 255) / 256), dim3(256), 0, s, a, (T*)h, last);
+      return rec_launched(who);
+    };
+    if (r->steps == 1) {  // with fewer columns than that, rather more threads
+      if (r->rows * r->width >= 1 << 20 && fits(4)) return step(rec_int<4>());
+      return fits(2) ? step(rec_int<2>()) : step(rec_int<1>());
+    }
     auto with = [&](auto vec) {
       constexpr int VEC = decltype(vec)::value;
       const RecArgs a = rec_args(r, p, VEC);
-      if (r->steps == 1) {
-        hipLaunchKernelGGL((mg_recurrence_step_kernel<T, VEC>), dim3((a.groups + 255) / 256), dim3(256), 0, s, a, (T*)h, last);
-      } else if (!p.shared) {
+      if (!p.shared) {
         hipLaunchKernelGGL((mg_recurrence_kernel<T, VEC>), dim3((a.groups + 255) / 256), dim3(256), 0, s, a, (T*)h, last, marks);
       } else {
         const dim3 grid((a.groups + 63) / 64, p.splits);
@@ -660,9 +686,9 @@ extern "C" int mg_gated_recurrence(const mg_recurrence* r, void* h, float* last,
       }
       return rec_launched(who);
     };
-    const int64_t e = sizeof(T);
-    if (p.vec == 2 && rec_fits(2, e, r->width, {r->x, r->gate, h}, {r->state, last, marks}, {r->x_row, r->x_step, r->gate_row, r->gate_step}))
-      return with(rec_int<2>());
+    if constexpr (sizeof(T) == 2) {
+      if (fits(2)) return with(rec_int<2>());
+    }
     return with(rec_int<1>());
   });
 } catch (...) {
@@ -696,10 +722,11 @@ extern "C" int mg_gated_recurrence_backward(const mg_recurrence* r, const float*
       }
       return rec_launched(who);
     };
-    const int64_t e = sizeof(T);
-    if (p.vec == 2 && rec_fits(2, e, r->width, {r->x, r->gate, d->dh, d->dx, d->dgate}, {},
-                 {r->x_row, r->x_step, r->gate_row, r->gate_step, d->dh_row, d->dh_step, d->dx_row, d->dx_step, d->dgate_row, d->dgate_step}))
-      return with(rec_int<2>());
+    if constexpr (sizeof(T) == 2) {
+      if (rec_fits(2, 2, r->width, {r->x, r->gate, d->dh, d->dx, d->dgate}, {},
+                   {r->x_row, r->x_step, r->gate_row, r->gate_step, d->dh_row, d->dh_step, d->dx_row, d->dx_step, d->dgate_row, d->dgate_step}))
+        return with(rec_int<2>());
+    }
     return with(rec_int<1>());
   });
 } catch (...) {

@@ -127,7 +127,7 @@ def test_library_refuses_bad_arguments_before_any_launch():
 # ---- GPU ----------------------------------------------------------------------------------------------------------
 
 SHAPES = [(1, 1, 1), (3, 1, 5), (2, 15, 7), (2, 16, 8), (2, 17, 2), (5, 33, 33), (1, 1000, 3), (7, 65, 128), (300, 40, 100),
-          (1, 4100, 64), (2, 2049, 130), (1, 129, 1000), (700, 48, 256)]  # fmt: skip
+          (1, 4100, 64), (2, 2049, 130), (1, 129, 1000), (700, 48, 256), (300, 300, 64), (130, 600, 128), (1, 70000, 3)]  # fmt: skip
 
 
 @pytest.mark.gpu
@@ -280,7 +280,7 @@ def test_empty():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows,width", [(1, 1), (24, 128), (5, 33), (1000, 100), (3, 2050)])
+@pytest.mark.parametrize("rows,width", [(1, 1), (24, 128), (5, 33), (1000, 100), (3, 2050), (4100, 256)])
 def test_step(rows, width, dtype):
     x, gate, state, resets, _, _ = (t.cuda() for t in _inputs(rows, 1, width, dtype, seed=rows, resets=0.3))
     want = _definition(*map(_np, (x, gate, state, resets)))
