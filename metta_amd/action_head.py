@@ -58,6 +58,8 @@ class _Head:
         if logits.dtype not in TYPES:
             raise RuntimeError("logits must be float32, bfloat16 or float16")
         lead, v = logits.shape[:-1], logits.size(-1)
+        if v >= 1 << 31:
+            raise RuntimeError("logits must have fewer than 2^31 tokens")
         device = logits.device
         for name, x in (("temperature", temperature), ("repetition", repetition)):
             if not 0.0 < x < math.inf:
@@ -145,51 +147,73 @@ def _per_row(name: str, t: Tensor, dtypes, lead, device) -> Tensor:
     return t.detach().contiguous()
 
 
+def _adjust(shape, head: _Head) -> Tensor:
+    out = torch.empty(shape, dtype=head.logits.dtype, device=head.logits.device)
+    if out.numel():
+        _launch("mg_adjust_logits", out.device, ct.byref(head.args), out.data_ptr())
+    return out
+
+
+def _evaluate(head: _Head, actions: Tensor, train: bool):
+    device = head.logits.device
+    logp = torch.empty(head.lead, dtype=torch.float32, device=device)
+    entropy = torch.empty_like(logp)
+    wide = train and head.args.width > native.STATS_WIDTH
+    stats = torch.empty(*head.lead, 2, dtype=torch.float64, device=device) if wide else None
+    if logp.numel():
+        w = _workspace(head.args, device)
+        _launch("mg_evaluate_actions", device, ct.byref(head.args), actions.data_ptr(), logp.data_ptr(), entropy.data_ptr(),
+                None if stats is None else stats.data_ptr())  # fmt: skip
+        del w
+    return logp, entropy, stats
+
+
+def _save(ctx, head: _Head, shape, *more) -> None:
+    # through save_for_backward, so that a tensor changed in between is noticed
+    ctx.save_for_backward(head.logits, head.bias, head.allowed, head.history, *more)
+    ctx.args, ctx.shape = head.args, shape
+
+
+def _saved(ctx):
+    """The arguments, pointing at what was saved (which a hook may have moved: it may lie elsewhere and otherwise), and the
+    rest of what was saved."""
+    logits, bias, allowed, history, *more = ctx.saved_tensors
+    a = native.MgLogits.from_buffer_copy(ctx.args)
+    kept = []
+    for name, t in (("logits", logits), ("bias", bias), ("allowed", allowed), ("history", history)):
+        if t is None:
+            continue
+        if t.stride(-1) != 1 and t.size(-1) != 1:
+            t = t.contiguous()
+        kept.append(t)
+        setattr(a, name, t.data_ptr())
+        setattr(a, name + "_row", t.stride(0) if t.dim() == 2 else 0)
+    return a, kept, more
+
+
 class _AdjustLogits(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, head):
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        if out.numel():
-            _launch("mg_adjust_logits", logits.device, ct.byref(head.args), out.data_ptr())
-        _save(ctx, logits, head)
-        return out
+        _save(ctx, head, logits.shape)
+        return _adjust(logits.shape, head)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        (logits,) = _saved(ctx)
-        d = torch.empty(dout.shape, dtype=logits.dtype, device=logits.device)
+        d = torch.empty(ctx.shape, dtype=dout.dtype, device=dout.device)
         if d.numel():
+            args, kept, _ = _saved(ctx)
             dout = dout.contiguous()
-            _launch("mg_adjust_logits_backward", d.device, ct.byref(ctx.args), dout.data_ptr(), d.data_ptr())
+            _launch("mg_adjust_logits_backward", d.device, ct.byref(args), dout.data_ptr(), d.data_ptr())
         return d, None
-
-
-def _save(ctx, logits, head, *more):
-    # through save_for_backward, so that a tensor changed in between is noticed; the structure points at the same memory
-    ctx.save_for_backward(head.logits, head.bias, head.allowed, head.history, *more)
-    ctx.args, ctx.shape = head.args, logits.shape
-
-
-def _saved(ctx):
-    saved = ctx.saved_tensors
-    return (saved[0], *saved[4:])
 
 
 class _EvaluateActions(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, head, actions):
         ctx.set_materialize_grads(False)
-        logp = torch.empty(head.lead, dtype=torch.float32, device=logits.device)
-        entropy = torch.empty_like(logp)
-        wide = ctx.needs_input_grad[0] and logits.size(-1) > native.STATS_WIDTH
-        stats = torch.empty(*head.lead, 2, dtype=torch.float64, device=logits.device) if wide else None
-        if logp.numel():
-            w = _workspace(head.args, logits.device)
-            _launch("mg_evaluate_actions", logits.device, ct.byref(head.args), actions.data_ptr(), logp.data_ptr(), entropy.data_ptr(),
-                    None if stats is None else stats.data_ptr())  # fmt: skip
-            del w
-        _save(ctx, logits, head, actions, entropy, stats)
+        logp, entropy, stats = _evaluate(head, actions, True)
+        _save(ctx, head, logits.shape, actions, entropy, stats)
         return logp, entropy
 
     @staticmethod
@@ -197,12 +221,13 @@ class _EvaluateActions(torch.autograd.Function):
     def backward(ctx, dlogp, dentropy):
         if dlogp is None and dentropy is None:
             return None, None, None
-        logits, actions, entropy, stats = _saved(ctx)
-        d = torch.empty(ctx.shape, dtype=logits.dtype, device=logits.device)
+        args, kept, (actions, entropy, stats) = _saved(ctx)
+        d = torch.empty(ctx.shape, dtype=kept[0].dtype, device=kept[0].device)
         if d.numel():
-            dlogp, dentropy = (None if g is None else g.contiguous() for g in (dlogp, dentropy))
-            _launch("mg_evaluate_actions_backward", d.device, ct.byref(ctx.args), actions.data_ptr(), entropy.data_ptr(), None if stats is None else stats.data_ptr(),
-                    None if dlogp is None else dlogp.data_ptr(), None if dentropy is None else dentropy.data_ptr(), d.data_ptr())  # fmt: skip
+            dlogp, dentropy, actions, entropy, stats = (None if t is None else t.contiguous() for t in (dlogp, dentropy, actions, entropy, stats))
+            _launch("mg_evaluate_actions_backward", d.device, ct.byref(args), actions.data_ptr(), entropy.data_ptr(),
+                    None if stats is None else stats.data_ptr(), None if dlogp is None else dlogp.data_ptr(),
+                    None if dentropy is None else dentropy.data_ptr(), d.data_ptr())  # fmt: skip
         return d, None, None
 
 
@@ -219,7 +244,10 @@ def adjust_logits(
 ) -> Tensor:
     """The adjusted logits (shape and type of `logits`, -infinity where masked), computed in 64 bits and rounded once.
     Differentiable once in `logits`."""
-    return _AdjustLogits.apply(logits, _Head(logits, allowed, bias, history, temperature, repetition, presence, frequency))
+    head = _Head(logits, allowed, bias, history, temperature, repetition, presence, frequency)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _AdjustLogits.apply(logits, head)
+    return _adjust(logits.shape, head)
 
 
 def sample_actions(
@@ -273,4 +301,6 @@ def evaluate_actions(
     actions = _per_row("actions", actions, (torch.int32, torch.int64), head.lead, logits.device)
     if actions.dtype == torch.int64:  # kept outside [0, V) where it is outside
         actions = actions.clamp(-1, 2**31 - 1).to(torch.int32)
-    return _EvaluateActions.apply(logits, head, actions)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _EvaluateActions.apply(logits, head, actions)
+    return _evaluate(head, actions, False)[:2]

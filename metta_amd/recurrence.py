@@ -9,7 +9,7 @@ element by element along the last dimension.  `gated_recurrence` runs `[rows, st
 Types: `x` and `gate` float32, bfloat16 or float16 (one type), `state` always float32; the state, the products along time
 and the running gradient are kept in 32 bits, outputs and gradients are rounded once.  `x` and `gate` may be strided
 views whose last dimension is adjacent (halves of one projection, a time-major tensor transposed); others are copied.
-A padded tail is held by a gate of +infinity: the state passes such a step unchanged.
+A padded tail is held by a gate of +infinity: the state passes such a step unchanged (with any finite x).
 """
 
 from __future__ import annotations
@@ -38,6 +38,13 @@ def _launch(name: str, device: torch.device, *args) -> None:
         native.check(rc, L)
 
 
+def _halves(x: Tensor, gate: Optional[Tensor]) -> Tuple[Tensor, Tensor]:
+    if gate is not None:
+        return x, gate
+    width = x.size(-1) // 2
+    return x[..., :width], x[..., width:]
+
+
 def _checked(x: Tensor, gate: Optional[Tensor], state: Optional[Tensor], resets: Optional[Tensor], dims: int) -> Tuple[Tensor, Tensor]:
     """The two inputs, after the checks that all entry points share."""
     if x.dim() != dims:
@@ -45,7 +52,7 @@ def _checked(x: Tensor, gate: Optional[Tensor], state: Optional[Tensor], resets:
     if gate is None:
         if x.size(-1) % 2:
             raise RuntimeError("without a gate, x holds candidates and gates side by side: its last dimension must be even")
-        x, gate = x.chunk(2, -1)
+        x, gate = _halves(x, None)
     if gate.shape != x.shape:
         raise RuntimeError("x and gate must have the same shape")
     if x.dtype not in TYPES or gate.dtype != x.dtype:
@@ -93,44 +100,44 @@ def _workspace(args: native.MgRecurrence, device: torch.device) -> Optional[Tens
     return w
 
 
+def _forward(x: Tensor, gate: Optional[Tensor], state: Optional[Tensor], resets: Optional[Tensor], train: bool):
+    xs, gs = _halves(x, gate)
+    rows, steps, width = xs.shape
+    h = torch.empty(rows, steps, width, dtype=x.dtype, device=x.device)
+    last = torch.empty(rows, width, dtype=torch.float32, device=x.device)
+    marks = None
+    if train and x.dtype != torch.float32:
+        marks = torch.empty(rows, (steps - 1) // native.MARK_STEPS, width, dtype=torch.float32, device=x.device)
+    args = _args(xs, gs, state, resets, steps)
+    w = _workspace(args, x.device)
+    _launch("mg_gated_recurrence", x.device, ct.byref(args), h.data_ptr(), last.data_ptr(), None if marks is None else marks.data_ptr())
+    del w
+    return h, last, marks
+
+
 class _GatedRecurrence(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, gate, state, resets, packed):
+    def forward(ctx, x, gate, state, resets):
         ctx.set_materialize_grads(False)
-        rows, steps, width = x.shape
-        if packed:
-            width //= 2
-        xs, gs = (x[..., :width], x[..., width:]) if packed else (x, gate)
-        h = torch.empty(rows, steps, width, dtype=x.dtype, device=x.device)
-        last = torch.empty(rows, width, dtype=torch.float32, device=x.device)
-        marks = None
-        if x.dtype != torch.float32 and any(ctx.needs_input_grad):
-            marks = torch.empty(rows, (steps - 1) // native.MARK_STEPS, width, dtype=torch.float32, device=x.device)
-        args = _args(xs, gs, state, resets, steps)
-        w = _workspace(args, x.device)
-        _launch("mg_gated_recurrence", x.device, ct.byref(args), h.data_ptr(), last.data_ptr(), None if marks is None else marks.data_ptr())
-        del w
+        h, last, marks = _forward(x, gate, state, resets, True)
         # an f32 output holds the states itself, in shorter types they are kept apart
         ctx.save_for_backward(x, gate, state, resets, h if marks is None else marks)
-        ctx.packed = packed
         return h, last
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dh, dlast):
-        x, gate, state, resets, marks = ctx.saved_tensors
         if dh is None and dlast is None:
-            return None, None, None, None, None
-        rows, steps, width = x.shape
-        if ctx.packed:
-            width //= 2
-            xs, gs = x[..., :width], x[..., width:]
-            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            d1, d2, dgate = dx[..., :width], dx[..., width:], None
-        else:
-            xs, gs = x, gate
-            d1 = dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            d2 = dgate = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            return None, None, None, None
+        # (what comes back may lie elsewhere and otherwise than what was saved: a hook may have moved it)
+        x, gate, state, resets, marks = ctx.saved_tensors
+        x, gate = _adjacent(x), None if gate is None else _adjacent(gate)
+        state, resets, marks = (None if t is None else t.contiguous() for t in (state, resets, marks))
+        xs, gs = _halves(x, gate)
+        rows, steps, width = xs.shape
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dgate = None if gate is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        d1, d2 = _halves(dx, dgate)
         dstate = torch.empty_like(state) if ctx.needs_input_grad[2] else None
         if dh is not None:
             dh = _adjacent(dh)
@@ -147,7 +154,7 @@ class _GatedRecurrence(torch.autograd.Function):
         w = _workspace(args, x.device)
         _launch("mg_gated_recurrence_backward", x.device, ct.byref(args), at, *strides, ct.byref(grads))
         del w
-        return dx, dgate, dstate, None, None
+        return dx, dgate, dstate, None
 
 
 def gated_recurrence(x: Tensor, gate: Optional[Tensor] = None, state: Optional[Tensor] = None, resets: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
@@ -156,7 +163,6 @@ def gated_recurrence(x: Tensor, gate: Optional[Tensor] = None, state: Optional[T
     Without `gate`, `x` is `[rows, steps, 2 * width]`: candidates, then gates (one projection; its gradient comes back as
     one tensor).  `state` float32 `[rows, width]` enters step 0 (None: zeros); where `resets` (bool or uint8
     `[rows, steps]`) is set, the state entering that step is zero.  Differentiable once in x, gate and state."""
-    packed = gate is None
     xs, gs = _checked(x, gate, state, resets, 3)
     if state is not None:
         state = state.contiguous()
@@ -165,7 +171,10 @@ def gated_recurrence(x: Tensor, gate: Optional[Tensor] = None, state: Optional[T
         return torch.empty_like(xs) + gs, last  # nothing to compute; part of the graph all the same
     if resets is not None:
         resets = resets.contiguous()
-    return _GatedRecurrence.apply(_adjacent(x), None if packed else _adjacent(gate), state, resets, packed)
+    x, gate = _adjacent(x), None if gate is None else _adjacent(gate)
+    if torch.is_grad_enabled() and (x.requires_grad or (gate is not None and gate.requires_grad) or (state is not None and state.requires_grad)):
+        return _GatedRecurrence.apply(x, gate, state, resets)
+    return _forward(x, gate, state, resets, False)[:2]
 
 
 def gated_recurrence_step(x: Tensor, gate: Optional[Tensor], state: Tensor, resets: Optional[Tensor] = None, out_state: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
@@ -183,6 +192,8 @@ def gated_recurrence_step(x: Tensor, gate: Optional[Tensor], state: Tensor, rese
         raise RuntimeError("out_state must be contiguous float32 [rows, width] on x's device")
     elif out_state.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("out_state is written in place and must not require a gradient")
+    elif 0 < abs(out_state.data_ptr() - state.data_ptr()) < 4 * state.numel():
+        raise RuntimeError("out_state may be state itself, but not overlap it otherwise")
     h = out_state if xs.dtype == torch.float32 else torch.empty(xs.shape, dtype=xs.dtype, device=xs.device)
     if xs.numel():
         xs, gs, state = _adjacent(xs), _adjacent(gs), state.contiguous()

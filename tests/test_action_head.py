@@ -537,3 +537,75 @@ def test_offsets_past_32_bits():
     a, logp, h = sample_actions(x, u.cuda(), **_cuda(c))
     assert np.array_equal(a.cpu().numpy(), _picked(l, _np(u)))
     _check_rows(logp, h, l, _picked(l, _np(u)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v", [5, 300, 9000])
+def test_training_in_a_captured_graph(v):
+    """Forward and backward captured once, replayed on new inputs with eager work in between; other leaves do the eager part."""
+    logits, c, u = _case(60, v, torch.bfloat16, seed=v)
+    dev, x, gp = _cuda(c), logits.cuda().requires_grad_(), u.cuda()
+    actions, _, _ = sample_actions(x, gp, **dev)
+
+    def once(t):
+        logp, h = evaluate_actions(t, actions, **dev)
+        adj = adjust_logits(t, **dev)
+        return [logp, h, adj, *torch.autograd.grad([logp, h], [t], [gp, gp]), *torch.autograd.grad(adj, t, adj.detach().clamp(-1, 1))]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            once(x)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = once(x)
+    for k in range(4):
+        with torch.no_grad():
+            x.mul_(0.5).add_(0.1 * k)
+        gp.uniform_()
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, once(x.detach().clone().requires_grad_())):
+            assert torch.equal(a, b), k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v", [7, 700, 9000])
+def test_saved_tensors_that_move(v):
+    """Hooks that take what was saved to the host and back give the same gradients, for sliced logits too."""
+    logits, c, u = _case(20, v, torch.float16, seed=v)
+    dev, gp = _cuda(c), u.cuda()
+    wide = torch.zeros(20, v + 9, dtype=torch.float16, device="cuda")
+    wide[:, 3 : 3 + v] = logits.cuda()
+    actions, _, _ = sample_actions(wide[:, 3 : 3 + v], gp, **dev)
+
+    def once():
+        leaf = wide.clone().requires_grad_()
+        view = (leaf * 1.0)[:, 3 : 3 + v]
+        return leaf, [*evaluate_actions(view, actions, **dev), adjust_logits(view, **dev)]
+
+    grads = [gp, gp, torch.ones(20, v, dtype=torch.float16, device="cuda")]
+    leaf, out = once()
+    (want,) = torch.autograd.grad(out, leaf, grads)
+    with torch.autograd.graph.save_on_cpu():
+        leaf, out = once()
+    junk = [torch.randn_like(wide) for _ in range(8)]  # memory that was free is written over
+    (got,) = torch.autograd.grad(out, leaf, grads)
+    assert len(junk) == 8 and torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_saved_tensors_are_watched_and_second_derivatives_refused():
+    x = torch.randn(4, 9, device="cuda", requires_grad=True)
+    y = x * 1.0
+    logp, _ = evaluate_actions(y, torch.zeros(4, dtype=torch.int32, device="cuda"))
+    y.detach().add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        logp.sum().backward()
+    for out in (evaluate_actions(x, torch.zeros(4, dtype=torch.int64, device="cuda"))[0], adjust_logits(x)):
+        (d,) = torch.autograd.grad(out.sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable|does not require grad"):
+            d.sum().backward()

@@ -389,3 +389,78 @@ def test_saved_tensors_are_watched():
     y.detach().add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         h.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_training_in_a_captured_graph(dtype):
+    """Forward and backward captured once, replayed on new inputs with eager work in between; other leaves do the eager part."""
+    x, gate, state, resets, dh, dlast = (t.cuda() for t in _inputs(3, 700, 40, dtype, seed=12))
+    leaves = [t.clone().requires_grad_() for t in (x, gate, state)]
+
+    def once(a, b, s):
+        h, last = gated_recurrence(a, b, s, resets)
+        return [h, last, *torch.autograd.grad([h, last], [a, b, s], [dh, dlast])]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            once(*leaves)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = once(*leaves)
+    for k in range(4):
+        with torch.no_grad():
+            for t in leaves:
+                t.mul_(0.9).add_(0.1 * k)
+        g.replay()
+        torch.cuda.synchronize()
+        want = once(*(t.detach().clone().requires_grad_() for t in leaves))
+        for a, b in zip(out, want):
+            assert torch.equal(a, b), k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_saved_tensors_that_move(packed, dtype):
+    """Hooks that take what was saved to the host and back give the same gradients."""
+    x, gate, state, resets, dh, dlast = (t.cuda() for t in _inputs(4, 90, 24, dtype, seed=17))
+
+    def once():
+        leaf = torch.cat([x, gate], -1).requires_grad_() if packed else x.clone().requires_grad_()
+        other = [] if packed else [gate.transpose(0, 1).contiguous().transpose(0, 1).requires_grad_()]
+        s = state.clone().requires_grad_()
+        out = gated_recurrence(leaf * 1.0, None if packed else other[0] * 1.0, s, resets)
+        return out, [leaf, s, *other]
+
+    out, leaves = once()
+    want = torch.autograd.grad(out, leaves, [dh, dlast])
+    with torch.autograd.graph.save_on_cpu():
+        out, leaves = once()
+    junk = [torch.randn_like(x) for _ in range(8)]  # memory that was free is written over
+    got = torch.autograd.grad(out, leaves, [dh, dlast])
+    assert len(junk) == 8
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused():
+    x = torch.randn(2, 20, 4, device="cuda", requires_grad=True)
+    (d,) = torch.autograd.grad(gated_recurrence(x, x)[0].sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable|does not require grad"):
+        d.sum().backward()
+
+
+@pytest.mark.gpu
+def test_overlapping_states_are_refused():
+    flat = torch.zeros(100, device="cuda")
+    x = torch.zeros(2, 8, device="cuda")
+    for at in (4, 12):
+        with pytest.raises(RuntimeError, match="overlap"):
+            gated_recurrence_step(x, x, flat[8:24].view(2, 8), out_state=flat[at : at + 16].view(2, 8))
+    gated_recurrence_step(x, x, flat[8:24].view(2, 8), out_state=flat[24:40].view(2, 8))
