@@ -363,7 +363,8 @@ int mg_gated_recurrence_backward(const mg_recurrence* r, const float* marks, int
  *   l1 = c > 0 ? (l > 0 ? l / repetition : l * repetition) : l;   l2 = l1 - frequency * c - presence * (c > 0)
  *   adjusted = allowed ? (l2 + bias) / temperature : -infinity
  * allowed: one byte per token (MG_ALLOWED_BOOL) or bit v % 32 of i32 word v / 32 (MG_ALLOWED_BITS); bias f32; history
- * i32, entries outside [0, width) count for nothing.  A row stride of 0 shares a control among all rows; NULL: none. */
+ * i32, entries outside [0, width) count for nothing.  temperature and repetition: 1e-30 to 1e30.  A row stride of 0
+ * shares a control among all rows; NULL: none. */
 #define MG_ALLOWED_BOOL 1
 #define MG_ALLOWED_BITS 2
 /* Rows up to this many tokens are held in registers: their backward pass wants neither stats nor entropy back. */

@@ -14,7 +14,7 @@ They share these controls, all keyword arguments, for logits `[..., V]` of float
 * `history`: int32 `[..., L]`, recent tokens of the row; entries outside `[0, V)` (-1) are empty.  A token that stands in
   it c > 0 times has its logit divided by `repetition` if it is positive and multiplied otherwise, and then lowered by
   `frequency * c + presence`;
-* `temperature`: what the result is divided by.
+* `temperature`: what the result is divided by (it and `repetition`: from 1e-30 to 1e30).
 
     adjusted = allowed ? (penalised + bias) / temperature : -infinity
 
@@ -39,11 +39,12 @@ from metta_amd.recurrence import TYPES, _launch
 
 def pack_allowed(allowed: Tensor) -> Tensor:
     """bool `[..., V]` -> int32 `[..., ceil(V / 32)]`: bit v % 32 of word v // 32 is token v's."""
-    if allowed.dtype != torch.bool or allowed.dim() < 1:
+    if allowed.dtype != torch.bool or allowed.dim() < 1 or allowed.size(-1) < 1:
         raise RuntimeError("allowed must be a bool tensor [..., V]")
     v = allowed.size(-1)
     bits = torch.nn.functional.pad(allowed, (0, -v % 32)).unflatten(-1, (-1, 32))
-    weights = torch.tensor([1 << i if i < 31 else -(1 << 31) for i in range(32)], dtype=torch.int32, device=allowed.device)
+    weights = 1 << torch.arange(32, dtype=torch.int64, device=allowed.device)  # (made where they are used: also in a captured graph)
+    weights = torch.where(weights > 0x7FFFFFFF, weights - (1 << 32), weights).to(torch.int32)
     return torch.where(bits, weights, 0).sum(-1, dtype=torch.int32)
 
 
@@ -62,8 +63,8 @@ class _Head:
             raise RuntimeError("logits must have fewer than 2^31 tokens")
         device = logits.device
         for name, x in (("temperature", temperature), ("repetition", repetition)):
-            if not 0.0 < x < math.inf:
-                raise RuntimeError(f"{name} must be positive and finite")
+            if not 1e-30 <= x <= 1e30:
+                raise RuntimeError(f"{name} must be from 1e-30 to 1e30")
         if not (math.isfinite(presence) and math.isfinite(frequency)):
             raise RuntimeError("presence and frequency must be finite")
         for t in (allowed, bias, history):

@@ -98,14 +98,15 @@ __device__ __forceinline__ HeadRow head_row(const HeadArgs& a, long row) {
 // What a row's exponentials and gradients are scaled by.  weight(t) = exp(-t / temperature) for t = M - x: the scale and
 // log2 e are one factor.  In 32 bits the difference, the factor and the product round once each, 3 u t / temperature
 // relative, plus the 2 u of the hardware's exp2.  In 64 bits a NaN is not handed on (the caller looks for it).
-// sum() adds t / temperature times the weight, in units that finish() turns into those of the entropy; it stays finite
-// where t does not (its weight is 0 there).
+// log2() is the weight's logarithm, kept finite where t is infinite or far: the weight is 0 there (from -150 on in 32 bits, from
+// -1075 on in 64), and 0 times it has to be 0.  sum() adds it times the weight; finish() turns that into sum t / temperature.
 template <typename X> struct HeadScale;
 template <> struct HeadScale<double> {
   double inv_temp, k;
   __device__ explicit HeadScale(const HeadRow& r) : inv_temp(r.inv_temp), k(r.weight_scale) {}
-  __device__ __forceinline__ double weight(double t) const { return head_exp_two(fmax(t * k, -2000.0)); }
-  __device__ __forceinline__ double sum(double t, double w, double s) const { return fma(fmax(t * k, -2000.0), w, s); }
+  __device__ __forceinline__ double weight(double t) const { return head_exp_two(log2(t)); }
+  __device__ __forceinline__ double log2(double t) const { return fmax(t * k, -2000.0); }
+  __device__ __forceinline__ double sum(double t, double w, double s) const { return fma(log2(t), w, s); }
   __device__ __forceinline__ double finish(double s) const { return s * -0.69314718055994529; }
 };
 template <> struct HeadScale<float> {
@@ -113,8 +114,11 @@ template <> struct HeadScale<float> {
   __device__ explicit HeadScale(const HeadRow& r) : inv_temp((float)r.inv_temp), k((float)r.weight_scale) {}
   __device__ __forceinline__ float weight(float t) const { return __builtin_amdgcn_exp2f(t * k); }
   __device__ __forceinline__ float weight(float t, float log_z) const { return __builtin_amdgcn_exp2f(fmaf(t, k, log_z * -1.44269504f)); }
-  __device__ __forceinline__ float sum(float t, float w, float s) const { return fmaf(fminf(t, 1e37f), w, s); }
-  __device__ __forceinline__ float finish(float s) const { return s * inv_temp; }
+  __device__ __forceinline__ float log2(float t) const { return fmaxf(t * k, -160.f); }
+  __device__ __forceinline__ float sum(float t, float w, float s) const { return fmaf(log2(t), w, s); }
+  __device__ __forceinline__ float finish(float s) const { return s * -0.693147182f; }
+  // H + log q of a token, from `past` = H - log Z
+  __device__ __forceinline__ float surprise(float t, float past) const { return fmaf(log2(t), 0.693147182f, past); }
 };
 // M - x in W, from values in X: in the wider of the two
 template <typename W, typename X>
@@ -122,13 +126,8 @@ __device__ __forceinline__ W head_far(X m, X x) {
   if constexpr (sizeof(W) > sizeof(X)) return (W)m - (W)x;
   else return (W)(m - x);
 }
-__device__ __forceinline__ double head_fma(double a, double b, double c) { return fma(a, b, c); }
-__device__ __forceinline__ float head_fma(float a, float b, float c) { return fmaf(a, b, c); }
 __device__ __forceinline__ double head_max(double a, double b) { return fmax(a, b); }  // (a NaN loses)
 __device__ __forceinline__ float head_max(float a, float b) { return fmaxf(a, b); }
-// t kept finite: its weight is 0 long before, and 0 * t has to be 0
-__device__ __forceinline__ double head_finite(double t) { return fmin(t, 1e300); }
-__device__ __forceinline__ float head_finite(float t) { return fminf(t, 1e37f); }
 
 __device__ __forceinline__ bool head_allowed(const HeadRow& r, int v) {
   if (r.kind == MG_ALLOWED_BITS) return (((const unsigned*)r.allowed)[v >> 5] >> (v & 31)) & 1;
@@ -506,7 +505,7 @@ struct HeadHeld {
 #pragma unroll
     for (int e = 0; e < E; e++) {
       const W far = head_far<W, X>(top, x[e]);
-      t[e] = head_finite(far);
+      t[e] = far;
       w[e] = scale.weight(far);
       z += w[e];
       s = scale.sum(far, w[e], s);
@@ -565,7 +564,8 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_sample_narrow_kernel(HeadArgs
 #pragma unroll
       for (int e = 0; e < E; e++) {
         run += h.w[e];
-        if (run > target && hit == a.width && e < h.n) hit = h.v0 + e;
+        // (a token without weight is never picked, also where a lane's sum of what came before is rounded up over the target)
+        if (run > target && hit == a.width && h.w[e] > 0.0) hit = h.v0 + e;
       }
     } else {
 #pragma unroll
@@ -605,10 +605,11 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_kernel(HeadAr
     const HeadScale<float> scale(r);
     const int act = actions[h.row];
     h.template hold<false>(a, g, r, scale, counts[adjust ? threadIdx.x : 0]);
-    float d = INFINITY;
+    X at = -INFINITY;  // (behind the row's end, where an action outside of it could lie, too)
 #pragma unroll
-    for (int e = 0; e < E; e++) d = h.v0 + e == act && e < h.n ? (h.x[e] == (X)-INFINITY ? (float)INFINITY : h.t[e] * scale.inv_temp) : d;
-    if (!ONE) d = head_group_min(d, g.lanes);
+    for (int e = 0; e < E; e++) at = h.v0 + e == act ? h.x[e] : at;
+    if (!ONE) at = head_group_max(at, g.lanes);
+    const float d = at == (X)-INFINITY ? INFINITY : head_far<float, X>(h.m, at) * scale.inv_temp;
     if (h.mine && h.lane == 0) {
       const float log_z = head_log(h.z);
       log_prob[h.row] = h.bad ? NAN : h.empty ? 0.f : (float)(-d - log_z);
@@ -641,12 +642,12 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_backward_kern
     if (!ONE) left = head_group_max((int)left, g.lanes) != 0;
     // (a bad row's NaN reaches every token that is left)
     const float gp = h.bad ? NAN : left ? gp_row * scale.inv_temp : 0.f, inv_z = head_inverse(h.z);
-    const float past = h.s * inv_z;  // H - log Z: H + log q = past - t / temperature
+    const float past = h.s * inv_z;  // H - log Z
     float y[E];
 #pragma unroll
     for (int e = 0; e < E; e++) {
       const float q = h.w[e] * inv_z;
-      float d = (h.v0 + e == act ? gp : 0.f) - q * head_fma(gh, past - h.t[e] * scale.inv_temp, gp);
+      float d = (h.v0 + e == act ? gp : 0.f) - q * fmaf(gh, scale.surprise(h.t[e], past), gp);
       if (adjust) d *= h.slope[e];
       y[e] = h.x[e] != (X)-INFINITY ? d : 0.f;
     }
@@ -871,7 +872,7 @@ __global__ __launch_bounds__(THREADS) void mg_sample_row_kernel(HeadArgs a, cons
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         run += h.w[0][e];
-        if (run > target && over == a.width && h.at(0) + e < a.width) over = h.at(0) + e;
+        if (run > target && over == a.width && h.w[0][e] > 0.0) over = h.at(0) + e;
         if (h.w[0][e] > 0.0) last = h.at(0) + e;
       }
       hit = head_block_min(over, red.i);
@@ -956,7 +957,7 @@ __global__ __launch_bounds__(HEAD_THREADS / 2) void mg_evaluate_row_backward_ker
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         const float q = h.w[c][e] * inv_z;
-        float d = (h.at(c) + e == act ? gp : 0.f) - q * head_fma(gh, past - head_finite(h.far(c, e)) * scale.inv_temp, gp);
+        float d = (h.at(c) + e == act ? gp : 0.f) - q * fmaf(gh, scale.surprise(h.far(c, e), past), gp);
         if (adjust) d *= h.slope[c][e];
         y[e] = h.x[c][e] != (X)-INFINITY ? d : 0.f;
       }
@@ -1084,7 +1085,7 @@ __global__ __launch_bounds__(THREADS) void mg_sample_join_kernel(HeadArgs a, int
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           run += w[e];
-          if (run > target && over == a.width && e < n) over = (int)(part0 + at + e), t_over = t[e];
+          if (run > target && over == a.width && w[e] > 0.0) over = (int)(part0 + at + e), t_over = t[e];
           if (w[e] > 0.0) last = (int)(part0 + at + e), t_last = t[e];
         }
         hit = head_block_min(over, red_int);
@@ -1155,7 +1156,7 @@ __global__ __launch_bounds__(HEAD_THREADS, (sizeof(X) == 4 ? 4 : 2)) void mg_eva
     const HeadRow r = head_row(a, row);
     const HeadScale<float> scale(r);
     const double m = stats[2 * row];
-    const float log_z = (float)stats[2 * row + 1], past = (float)((double)entropy[row] - stats[2 * row + 1]);  // H + log q = past - t / temperature
+    const float log_z = (float)stats[2 * row + 1], past = (float)((double)entropy[row] - stats[2 * row + 1]);  // H - log Z
     const bool bad = m != m, empty = m == -INFINITY;
     const X top = bad || empty ? (X)0 : (X)m;
     const int act = actions[row];
@@ -1184,7 +1185,7 @@ __global__ __launch_bounds__(HEAD_THREADS, (sizeof(X) == 4 ? 4 : 2)) void mg_eva
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         const float t = (float)(top - x[e]);
-        g[e] = -scale.weight(t, log_z) * head_fma(gh, past - head_finite(t) * scale.inv_temp, gp);
+        g[e] = -scale.weight(t, log_z) * fmaf(gh, scale.surprise(t, past), gp);
       }
       if ((unsigned)(act - v0) < 8u) {
 #pragma unroll
@@ -1211,8 +1212,9 @@ static int head_check(const char* who, const mg_logits* a) {
   if (!a) return mg_fail_msg(w + ": NULL arguments");
   if (a->rows < 0 || a->width < 1) return mg_fail_msg(w + ": a row has at least one token");
   if (a->type < 0 || a->type > 2) return mg_fail_msg(w + ": type must be MG_F32, MG_BF16 or MG_F16");
-  if (!(a->temperature > 0.0 && a->temperature < INFINITY)) return mg_fail_msg(w + ": temperature must be positive and finite");
-  if (!(a->repetition > 0.0 && a->repetition < INFINITY)) return mg_fail_msg(w + ": repetition must be positive and finite");
+  // (so that neither they nor their inverses leave the range of 32 bits)
+  if (!(a->temperature >= 1e-30 && a->temperature <= 1e30)) return mg_fail_msg(w + ": temperature must be from 1e-30 to 1e30");
+  if (!(a->repetition >= 1e-30 && a->repetition <= 1e30)) return mg_fail_msg(w + ": repetition must be from 1e-30 to 1e30");
   if (!(std::abs(a->presence) < INFINITY && std::abs(a->frequency) < INFINITY)) return mg_fail_msg(w + ": penalties must be finite");
   if (a->allowed && a->allowed_kind != MG_ALLOWED_BOOL && a->allowed_kind != MG_ALLOWED_BITS)
     return mg_fail_msg(w + ": allowed_kind must be MG_ALLOWED_BOOL or MG_ALLOWED_BITS");

@@ -188,10 +188,10 @@ def rollout_phase(
             "truncateds": t.to(torch.float32),
         }
         experience.store(td, training_env_id)
-        if controls is not None:
-            controls.took(key, td["actions"])
         if on_step is not None:
             on_step(td, training_env_id)
+        if controls is not None:
+            controls.took(key, td["actions"])
         env.send_actions(td["actions"])  # the device tensor itself: no .cpu().numpy()
         if info:
             result.raw_infos.extend(info)

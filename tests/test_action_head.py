@@ -126,6 +126,9 @@ def test_refusals():
         ("temperature", l, dict(temperature=0.0)),
         ("temperature", l, dict(temperature=-1.0)),
         ("temperature", l, dict(temperature=float("nan"))),
+        ("temperature", l, dict(temperature=9e-31)),
+        ("temperature", l, dict(temperature=INF)),
+        ("repetition", l, dict(repetition=1.1e30, history=h)),
         ("repetition", l, dict(repetition=0.0, history=h)),
         ("repetition", l, dict(repetition=INF, history=h)),
         ("finite", l, dict(presence=INF, history=h)),
@@ -149,8 +152,9 @@ def test_refusals():
                 continue  # it has no gradient to lose
             with pytest.raises(RuntimeError, match=text):
                 call(logits, **c)
-    with pytest.raises(RuntimeError, match="bool"):
-        pack_allowed(a.int())
+    for bad in (a.int(), a[:, :0]):
+        with pytest.raises(RuntimeError, match="bool"):
+            pack_allowed(bad)
 
 
 def test_library_refuses_bad_arguments_before_any_launch():
@@ -167,11 +171,26 @@ def test_library_refuses_bad_arguments_before_any_launch():
         f = getattr(L, name)
         assert f(None, *[None] * n) != 0
         for change, text in (({"type": 5}, b"type"), ({"width": 0}, b"token"), ({"rows": -1}, b"token"), ({"temperature": 0.0}, b"temperature"),
-                             ({"repetition": -1.0}, b"repetition"), ({"presence": INF}, b"finite"), ({"logits": None}, b"NULL"),
+                             ({"repetition": -1.0}, b"repetition"), ({"temperature": 1e31}, b"temperature"), ({"presence": INF}, b"finite"), ({"logits": None}, b"NULL"),
                              ({"logits": 4096, "allowed": 4096, "allowed_kind": 7}, b"allowed_kind"), ({"logits": 4096}, b"NULL")):  # fmt: skip
             a = native.MgLogits(**(good | change))
             assert f(ct.byref(a), *[None] * n) != 0 and text in L.mg_last_error(), (name, change)
         assert f(ct.byref(native.MgLogits(**(good | {"rows": 0}))), *[None] * n) == 0
+
+
+@pytest.mark.gpu
+def test_pack_allowed_in_a_captured_graph():
+    a = torch.rand(7, 157, device="cuda") < 0.5
+    pack_allowed(a)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        w = pack_allowed(a)
+    for _ in range(4):
+        a.copy_(torch.rand(7, 157, device="cuda") < 0.5)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(w, pack_allowed(a))
 
 
 def test_pack_allowed():
@@ -410,6 +429,54 @@ def test_extreme_controls():
     u = torch.rand(50, generator=torch.Generator().manual_seed(2))
     a, _, _ = sample_actions(big.cuda(), u.cuda(), **_cuda(c))
     assert np.array_equal(a.cpu().numpy(), _picked(l, _np(u)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("v", [6, 100, 900, 3000, 20000])
+def test_far_tokens_and_ends_of_the_temperature(v, bias):
+    """Logits of 32 bits that lie further apart than their temperature allows a quotient for, under large outer gradients:
+    what has no weight has no part in the gradient, and log-probabilities are right up to the last finite one."""
+    logits = torch.randn(8, v, generator=torch.Generator().manual_seed(v))
+    logits[:, 1] = torch.tensor([-1e38, -3.4e38, -2e38, -3e36, -1e30, -1e37, -5e37, -1e35])
+    logits[4:, 2] = 1e30
+    allowed = torch.ones(8, v, dtype=torch.bool)
+    allowed[:, 3] = False
+    kw = dict(allowed=allowed) | (dict(bias=torch.zeros(v)) if bias else {})
+    actions = np.array([1, 1, 1, 1, 2, 1, 3, 0])
+    for temperature in (1e-30, 1e-3, 0.02, 1.0, 1e3, 1e30):
+        l, _ = _adjusted(logits, temperature=temperature, **kw)
+        s = _stats(l)
+        x = logits.cuda().requires_grad_()
+        logp, h = evaluate_actions(x, torch.from_numpy(actions).cuda(), temperature=temperature, **_cuda(kw))
+        logz, tol_h = _tol(s)
+        i = np.arange(8)
+        want = l[i, actions] - s["m"] - np.log(s["z"])
+        big = 1.0 - 8 * U  # within roundings of the largest number a value may be infinite
+        got, most = _np(logp), float(np.finfo(np.float32).max)
+        fine = np.abs(want) < most * big
+        assert np.all(np.isneginf(got[np.abs(want) > most * (1 + 8 * U)])) and np.all(np.abs(got - want)[fine] <= (logz + 5 * U * np.abs(want))[fine])
+        assert np.all(np.abs(_np(h) - s["h"]) <= tol_h)
+        for g in (1.0, 4096.0):  # a scaled loss
+            (d,) = torch.autograd.grad([logp, h], x, [torch.full_like(logp, g), torch.full_like(h, g)], retain_graph=True)
+            d = _np(d)
+            q = s["e"] / s["z"][:, None]
+            hit = np.zeros_like(q)
+            hit[i, actions] = np.isfinite(l[i, actions])
+            lq = np.where(q > 0, -np.where(np.isinf(s["d"]), 0, s["d"]) - np.log(s["z"])[:, None], 0.0)
+            value = (hit - hit.sum(1, keepdims=True) * q - q * (lq + s["h"][:, None])) * np.where(allowed, g / temperature, 0.0)
+            assert np.isfinite(d[np.abs(value) < 1e37]).all() and not np.isnan(d).any()
+            # where q is nothing, nothing but the action's own gradient is left
+            nothing = (s["d"] > 200) & (hit == 0)
+            assert np.all(d[nothing] == 0)
+            relq = 5 * U * np.abs(lq) + logz[:, None] + 8 * U
+            err = q * relq + 4 * U * hit + q * (relq * np.abs(lq + s["h"][:, None]) + 5 * U * np.abs(lq) + (logz + tol_h)[:, None] + 8 * U * (np.abs(lq) + s["h"][:, None]))
+            # (weights below 2^-126 may be 0: what they are multiplied by there is up to 1 + 104 + H)
+            tol = (err + 2.0**-126 * 200) * g / temperature + 5 * U * np.abs(value) + 1e-37
+            fine = np.abs(value) < 1e37
+            assert np.all(np.abs(d - value)[fine] <= tol[fine]), (temperature, g)
+        a, _, _ = sample_actions(x, torch.full((8,), 0.999, device="cuda"), temperature=temperature, **_cuda(kw))
+        assert np.array_equal(a.cpu().numpy(), _picked(l, np.full(8, np.float32(0.999), dtype=np.float64)))
 
 
 @pytest.mark.gpu
