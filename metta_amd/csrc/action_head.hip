@@ -12,14 +12,16 @@
 // or +infinity among its allowed tokens has action -1 and NaN.
 //
 // Rows of up to HEAD_NARROW columns are held in registers, E adjacent columns per lane, by as many lanes as that takes
-// (one lane for five actions, a wave for five hundred); rows of up to HEAD_ROW columns by a block, eight columns per
-// thread.  Their logits are read once.  Wider rows are cut into parts of one or four chunks, a block each; what a part found (maximum, sum, ...) goes to a workspace and a second launch joins
-// the parts of a row.  A history is counted in LDS by the block that needs it, for the columns that it holds.
+// (one lane for five actions, a wave for five hundred); rows of up to HEAD_ROW columns by a block, in chunks of eight columns
+// per thread.  Their logits are read once.  Wider rows are cut into parts of one or four chunks, a block each; what a part
+// found (maximum, sum, ...) goes to a workspace and a second launch joins the parts of a row.  A history is counted in LDS by
+// the block that needs it, for the columns that it holds.
 //
-// Sampling is done in 64 bits from the exponential on: an action that falls next to a border of the distribution is then
-// the definition's whatever the order of the sums, and a 64-bit multiply-add costs what a 32-bit one costs here.
-// Log-probabilities and entropies of given actions need no more than 32 bits; there only the logits themselves are held in 64
-// where a bias or a penalty could cancel large ones.
+// The logits are held in 64 bits where a bias or a penalty could cancel large ones, the differences from the largest and all
+// that follows in 32, which log-probabilities, entropies and gradients need no more than.  A sampled action is the one that
+// 64 bits find all the same, whatever the order of the sums: the error of the running sum is bounded, and a row in which the
+// target comes within that bound of a token's border (one in hundreds or thousands) is done once more in 64 bits.  The parts
+// of wide rows are summed in 64 bits from the start, since hardly a row of theirs is clear of all its borders.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -39,21 +41,21 @@ extern int mg_fail_msg(const std::string& m);  // mettagrid_hip.hip: sets mg_las
 
 // ---- arithmetic -------------------------------------------------------------------------------------------------------
 
-// 2^y for y <= 0: n = rint(y), and the series in (y - n) ln 2, |y - n| <= 1/2, to its 12th term, which leaves 2e-16.  (y of
-// less than -1075 gives 0.)  15 instructions, where the library's e^x takes 40.
+// 2^y for y <= 0: n = rint(y), and with r = y - n, |r| <= 1/2, the polynomial 1 + r q(r), q of degree 10 through
+// (2^r - 1) / r at the Chebyshev points, which is 2e-17 off.  (y of less than -1075 gives 0.)  14 instructions, where the
+// library's e^x takes 40.
 __device__ __forceinline__ double head_exp_two(double y) {
   const double n = rint(y), r = y - n;
-  double p = 2.5678435993488196e-11;
-  p = fma(p, r, 4.44553827187081e-10);
-  p = fma(p, r, 7.054911620801121e-09);
-  p = fma(p, r, 1.0178086009239696e-07);
-  p = fma(p, r, 1.3215486790144305e-06);
-  p = fma(p, r, 1.5252733804059838e-05);
-  p = fma(p, r, 0.00015403530393381606);
-  p = fma(p, r, 0.0013333558146428441);
-  p = fma(p, r, 0.009618129107628477);
-  p = fma(p, r, 0.055504108664821576);
-  p = fma(p, r, 0.2402265069591007);
+  double p = 4.4549605981865186e-10;
+  p = fma(p, r, 7.072585949269223e-09);
+  p = fma(p, r, 1.0178062445845774e-07);
+  p = fma(p, r, 1.321544258792169e-06);
+  p = fma(p, r, 1.525273382983612e-05);
+  p = fma(p, r, 0.0001540353044173605);
+  p = fma(p, r, 0.0013333558146416936);
+  p = fma(p, r, 0.009618129107606888);
+  p = fma(p, r, 0.0555041086648216);
+  p = fma(p, r, 0.24022650695910097);
   p = fma(p, r, 0.6931471805599453);
   p = fma(p, r, 1.0);
   return ldexp(p, (int)n);
@@ -331,6 +333,9 @@ struct HeadRaw {
   }
 };
 
+// which of the grid's blocks this is (head_grid)
+__device__ __forceinline__ long head_block() { return (long)blockIdx.y * gridDim.x + blockIdx.x; }
+
 // ---- lanes ------------------------------------------------------------------------------------------------------------
 
 __device__ __forceinline__ int head_lane() { return threadIdx.x & 63; }
@@ -371,8 +376,8 @@ template <typename V>
 __device__ __forceinline__ V head_group_sum(V x, int lanes) {
   return head_group(x, lanes, [](V a, V b) { return a + b; });
 }
-// the sum of the lanes before this one in its group
-__device__ __forceinline__ double head_group_before(double x, int lanes, int lane) {
+// the sum of the lanes before this one in its group, and of all of them
+__device__ __forceinline__ double head_group_before(double x, int lanes, int lane, double& all) {
   double sum = x;
   auto add = [&](double up, int o) { sum += lane >= o ? up : 0.0; };
   if (lanes > 1) add(head_dpp<0x111>(sum, 0.0), 1);
@@ -388,6 +393,7 @@ __device__ __forceinline__ double head_group_before(double x, int lanes, int lan
     const double half = __shfl(sum, 31);
     sum += lane & 32 ? half : 0.0;
   }
+  all = __shfl(sum, head_lane() | (lanes - 1));
   return sum - x;
 }
 
@@ -473,9 +479,9 @@ __device__ __forceinline__ void head_count_rows(const HeadArgs& a, const HeadNar
 template <int E, bool ONE, typename X, typename W>
 struct HeadHeld {
   X x[E], m;
-  W t[E], w[E], z, s, z_lane;  // t = M - x, w = its weight; t and w say nothing where the row is bad or empty
+  W t[E], w[E], z, s;  // t = M - x, w = its weight; t and w say nothing where the row is bad or empty
+  double z_lane, before, all;  // (of a group whose running sum is wanted) z of this lane's columns, of the lanes before it, of all
   float slope[E];
-  unsigned ok;
   long row;         // clamped: the groups behind the last row do that row's work once more
   int lane, v0, n;  // this lane's columns, n of them (or fewer than one) in the row
   bool bad, empty, mine;  // mine: the row is this group's own
@@ -489,12 +495,12 @@ struct HeadHeld {
     n = ONE ? E : a.width - v0;
   }
 
-  template <bool GRAD>
+  template <bool GRAD, bool RUN>
   __device__ __forceinline__ void hold(const HeadArgs& a, const HeadNarrow& g, const HeadRow& r, const HeadScale<W>& scale, const unsigned* counts) {
     constexpr bool adjust = std::is_same<X, double>::value;
     HeadRaw<E> raw;
     raw.template fetch<ONE, adjust>(r, a.logits, a.type, row * a.logits_row + v0, v0, n);
-    ok = raw.template columns<ONE, GRAD, adjust>(r, a.type, v0, n, counts, x, slope);
+    raw.template columns<ONE, GRAD, adjust>(r, a.type, v0, n, counts, x, slope);
     m = x[0];
 #pragma unroll
     for (int e = 1; e < E; e++) m = head_max(m, x[e]);
@@ -512,9 +518,10 @@ struct HeadHeld {
       if (sizeof(W) == 8) lost = lost || far != far;
     }
     if (lost) z = NAN;
-    z_lane = z;
+    if constexpr (RUN) z_lane = all = z, before = 0.0;
     if (!ONE) {
-      z = head_group_sum(z, g.lanes);
+      if constexpr (RUN) before = head_group_before(z_lane, g.lanes, lane, all), z = (W)all;
+      else z = head_group_sum(z, g.lanes);
       s = head_group_sum(s, g.lanes);
     }
     s = scale.finish(s);
@@ -522,22 +529,102 @@ struct HeadHeld {
     bad = !(m < (X)INFINITY) || z != z;
     empty = !bad && m == (X)-INFINITY;
   }
+  // the lanes of this row
+  __device__ __forceinline__ unsigned long long group(const HeadNarrow& g) const {
+    return ONE ? 1ull << head_lane() : ~0ull >> (64 - g.lanes) << (head_lane() - lane);
+  }
+  // whether this lane has the token that is meant: the one at which the running sum passes the target, or (SUM false) the first
+  // of the largest.  Where no lane has (a uniform of 1 or more, or one that the roundings between two lanes took): the last
+  // with any weight.
+  template <bool SUM>
+  __device__ __forceinline__ bool picks(const HeadNarrow& g, double target) const {
+    if (ONE) return true;
+    bool pass = false;
+    if (SUM) {
+      pass = z_lane > 0.0 && before + z_lane > target;
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; e++) pass = pass || x[e] == m;
+    }
+    const unsigned long long over = __ballot(pass) & group(g), some = SUM ? __ballot(z_lane > 0.0) & group(g) : over;
+    return head_lane() == (bad || empty ? head_lane() - lane : over ? __ffsll(over) - 1 : 63 - __clzll((long long)some));
+  }
 };
+
+// Which of a thread's E tokens a running sum passes the target at, and its t: the last with any weight, if it does not.  (A
+// token without weight is never picked, also where the sum of what came before is rounded up over the target.)
+template <typename W>
+struct HeadPick {
+  int e;
+  W t;
+  double before, at;  // the running sum before it and with it
+};
+template <int E, typename W>
+__device__ __forceinline__ HeadPick<W> head_pick(const W* w, const W* t, double run, double target) {
+  HeadPick<W> pick{0, 0, run, run};
+  bool over = false;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const bool take = !over && w[e] > 0;
+    pick.e = take ? e : pick.e;
+    pick.t = take ? t[e] : pick.t;
+    pick.before = take ? run : pick.before;
+    run += w[e];
+    pick.at = take ? run : pick.at;
+    over = over || (take && run > target);
+  }
+  return pick;
+}
+// How far a running sum of 32-bit weights and a target made with their whole sum z may be off together.  A weight at distance d
+// is off by 3 u d (difference, scale, product; u = 2^-24) and 1.43 u (the hardware's exp2, over all its arguments), a thread's
+// sum of eight by 7 u more, everything else is added in 64 bits: (3 s + 8.5 z) u with s = sum of d w, and the target the
+// same, where 2 (4 s + 12 z) u is taken; what is below 2^-126 does not count beside that, since z is 1 or more.
+__device__ __forceinline__ double head_margin(double z, double s) { return 0x1p-23 * (4.0 * s + 12.0 * z); }
+__device__ __forceinline__ bool head_sure(const HeadPick<float>& pick, double target, double margin) {
+  return pick.before + margin < target && pick.at - margin > target;
+}
+template <int E, typename X>
+__device__ __forceinline__ int head_first(const X* x, X m) {
+  int first = 0;
+#pragma unroll
+  for (int e = E - 1; e >= 0; e--) first = x[e] == m ? e : first;
+  return first;
+}
+// t and weights of E tokens from their x, once more: what is kept from the first time takes the registers of other waves.  (The
+// empty assembly is what stops the compiler from keeping it.)
+template <int E, typename W, typename X>
+__device__ __forceinline__ void head_again(const X* x, X m, const HeadScale<W>& scale, W* t, W* w) {
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    X xe = x[e];
+    asm volatile("" : "+v"(xe));
+    t[e] = head_far<W, X>(m, xe);
+    w[e] = scale.weight(t[e]);
+  }
+}
+template <typename W>
+__device__ __forceinline__ void head_sampled(long row, bool bad, bool empty, int action, W t, W z, W s, const HeadScale<W>& scale, int* actions,
+                                             float* log_prob, float* entropy) {
+  const W log_z = head_log(z);
+  actions[row] = bad || empty ? -1 : action;
+  log_prob[row] = bad ? NAN : empty ? 0.f : (float)(-t * scale.inv_temp - log_z);
+  entropy[row] = bad ? NAN : empty ? 0.f : (float)(log_z + s * head_inverse(z));
+}
 
 template <int E>
 __global__ __launch_bounds__(HEAD_THREADS) void mg_adjust_narrow_kernel(HeadArgs a, HeadNarrow g, void* __restrict__ out,
                                                                        const void* __restrict__ dout, void* __restrict__ dlogits) {
   __shared__ unsigned counts[HEAD_THREADS][E + 1];
-  for (long row0 = (long)blockIdx.x * g.rows; row0 < a.rows; row0 += (long)gridDim.x * g.rows) {
-    if (a.history) head_count_rows<E>(a, g, row0, counts);
-    HeadHeld<E, false, double, double> h;
-    h.place(a, g, row0);
-    if (!h.mine) continue;
-    const HeadRow r = head_row(a, h.row);
-    HeadAdjust<E> it;
-    it.template fetch<false>(a, r, h.row, h.v0, h.n, dout);
-    it.store(a, r, h.row, h.v0, h.n, counts[threadIdx.x], out, dout, dlogits);
-  }
+  const long row0 = head_block() * g.rows;
+  if (row0 >= a.rows) return;
+  if (a.history) head_count_rows<E>(a, g, row0, counts);
+  HeadHeld<E, false, double, double> h;
+  h.place(a, g, row0);
+  if (!h.mine) return;
+  const HeadRow r = head_row(a, h.row);
+  HeadAdjust<E> it;
+  it.template fetch<false>(a, r, h.row, h.v0, h.n, dout);
+  it.store(a, r, h.row, h.v0, h.n, counts[threadIdx.x], out, dout, dlogits);
 }
 
 template <int E, bool ONE, typename X>
@@ -546,47 +633,48 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_sample_narrow_kernel(HeadArgs
                                                                        float* __restrict__ entropy) {
   constexpr bool adjust = std::is_same<X, double>::value;
   __shared__ unsigned counts[adjust ? HEAD_THREADS : 1][E + 1];
-  for (long row0 = (long)blockIdx.x * g.rows; row0 < a.rows; row0 += (long)gridDim.x * g.rows) {
-    if constexpr (adjust) {
-      if (a.history) head_count_rows<E>(a, g, row0, counts);
-    }
-    HeadHeld<E, ONE, X, double> h;
-    h.place(a, g, row0);
-    const HeadRow r = head_row(a, h.row);
-    const HeadScale<double> scale(r);
-    h.template hold<false>(a, g, r, scale, counts[adjust ? threadIdx.x : 0]);
-    int hit = a.width, last = -1;
-    if (uniforms) {
-      const double target = fmax((double)uniforms[h.row], 0.0) * h.z;
-      double run = ONE ? 0.0 : head_group_before(h.z_lane, g.lanes, h.lane);
+  const long row0 = head_block() * g.rows;
+  if (row0 >= a.rows) return;
+  if constexpr (adjust) {
+    if (a.history) head_count_rows<E>(a, g, row0, counts);
+  }
+  HeadHeld<E, ONE, X, float> h;
+  h.place(a, g, row0);
+  const HeadRow r = head_row(a, h.row);
+  const HeadScale<float> scale(r);
+  const unsigned* mine = counts[adjust ? threadIdx.x : 0];
+  if (!uniforms) {
+    h.template hold<false, false>(a, g, r, scale, mine);
+    if (h.template picks<false>(g, 0.0) && h.mine)
+      head_sampled(h.row, h.bad, h.empty, h.v0 + head_first<E>(h.x, h.m), 0.f, h.z, h.s, scale, actions, log_prob, entropy);
+    return;
+  }
+  h.template hold<false, true>(a, g, r, scale, mine);
+  const double u = fmax((double)uniforms[h.row], 0.0), target = u < 1.0 ? u * h.all : INFINITY;
+  bool unsure = false;
+  if (h.template picks<true>(g, target)) {
+    const HeadPick<float> pick = head_pick<E>(h.w, h.t, h.before, target);
+    unsure = !h.bad && !h.empty && !head_sure(pick, target, head_margin(h.all, h.s));
+    if (h.mine && !unsure) head_sampled(h.row, h.bad, h.empty, h.v0 + pick.e, pick.t, h.z, h.s, scale, actions, log_prob, entropy);
+  }
+  const unsigned long long again = __ballot(unsure);
+  if (!again) return;
+  // the same in 64 bits
+  const HeadScale<double> exact(r);
+  double t[E], w[E], s = 0.0;
+  head_again<E>(h.x, h.m, exact, t, w);
+  h.z_lane = 0.0;
 #pragma unroll
-      for (int e = E - 1; e >= 0; e--) last = last < 0 && h.w[e] > 0.0 ? h.v0 + e : last;
-#pragma unroll
-      for (int e = 0; e < E; e++) {
-        run += h.w[e];
-        // (a token without weight is never picked, also where a lane's sum of what came before is rounded up over the target)
-        if (run > target && hit == a.width && h.w[e] > 0.0) hit = h.v0 + e;
-      }
-    } else {
-#pragma unroll
-      for (int e = E - 1; e >= 0; e--)
-        if (h.x[e] == h.m && e < h.n) hit = h.v0 + e;
-    }
-    if (!ONE) {
-      hit = head_group_min(hit, g.lanes);
-      last = head_group_max(last, g.lanes);
-    }
-    if (hit == a.width) hit = last;  // a uniform of 1 or more
-    double t = 0.0;
-#pragma unroll
-    for (int e = 0; e < E; e++) t = h.v0 + e == hit ? h.t[e] : t;
-    if (!ONE) t = __shfl(t, (head_lane() & ~(g.lanes - 1)) + (hit >= 0 && hit < a.width ? hit / E : 0));
-    if (h.mine && h.lane == 0) {
-      const double log_z = head_log(h.z);
-      actions[h.row] = h.bad || h.empty ? -1 : hit;
-      log_prob[h.row] = h.bad ? NAN : h.empty ? 0.f : (float)(-t * scale.inv_temp - log_z);
-      entropy[h.row] = h.bad ? NAN : h.empty ? 0.f : (float)(log_z + h.s * head_inverse(h.z));
-    }
+  for (int e = 0; e < E; e++) h.z_lane += w[e], s = exact.sum(t[e], w[e], s);
+  h.all = h.z_lane, h.before = 0.0;
+  if (!ONE) {
+    h.before = head_group_before(h.z_lane, g.lanes, h.lane, h.all);
+    s = head_group_sum(s, g.lanes);
+  }
+  const double line = u < 1.0 ? u * h.all : INFINITY;
+  if (h.template picks<true>(g, line) && h.mine && (again & h.group(g))) {
+    const HeadPick<double> pick = head_pick<E>(w, t, h.before, line);
+    head_sampled(h.row, false, false, h.v0 + pick.e, pick.t, h.all, exact.finish(s), exact, actions, log_prob, entropy);
   }
 }
 
@@ -595,26 +683,26 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_kernel(HeadAr
                                                                          float* __restrict__ log_prob, float* __restrict__ entropy) {
   constexpr bool adjust = std::is_same<X, double>::value;
   __shared__ unsigned counts[adjust ? HEAD_THREADS : 1][E + 1];
-  for (long row0 = (long)blockIdx.x * g.rows; row0 < a.rows; row0 += (long)gridDim.x * g.rows) {
-    if constexpr (adjust) {
-      if (a.history) head_count_rows<E>(a, g, row0, counts);
-    }
-    HeadHeld<E, ONE, X, float> h;
-    h.place(a, g, row0);
-    const HeadRow r = head_row(a, h.row);
-    const HeadScale<float> scale(r);
-    const int act = actions[h.row];
-    h.template hold<false>(a, g, r, scale, counts[adjust ? threadIdx.x : 0]);
-    X at = -INFINITY;  // (behind the row's end, where an action outside of it could lie, too)
+  const long row0 = head_block() * g.rows;
+  if (row0 >= a.rows) return;
+  if constexpr (adjust) {
+    if (a.history) head_count_rows<E>(a, g, row0, counts);
+  }
+  HeadHeld<E, ONE, X, float> h;
+  h.place(a, g, row0);
+  const HeadRow r = head_row(a, h.row);
+  const HeadScale<float> scale(r);
+  const int act = actions[h.row];
+  h.template hold<false, false>(a, g, r, scale, counts[adjust ? threadIdx.x : 0]);
+  X at = -INFINITY;  // (behind the row's end, where an action outside of it could lie, too)
 #pragma unroll
-    for (int e = 0; e < E; e++) at = h.v0 + e == act ? h.x[e] : at;
-    if (!ONE) at = head_group_max(at, g.lanes);
-    const float d = at == (X)-INFINITY ? INFINITY : head_far<float, X>(h.m, at) * scale.inv_temp;
-    if (h.mine && h.lane == 0) {
-      const float log_z = head_log(h.z);
-      log_prob[h.row] = h.bad ? NAN : h.empty ? 0.f : (float)(-d - log_z);
-      entropy[h.row] = h.bad ? NAN : h.empty ? 0.f : (float)(log_z + h.s * head_inverse(h.z));
-    }
+  for (int e = 0; e < E; e++) at = h.v0 + e == act ? h.x[e] : at;
+  if (!ONE) at = head_group_max(at, g.lanes);
+  const float d = at == (X)-INFINITY ? INFINITY : head_far<float, X>(h.m, at) * scale.inv_temp;
+  if (h.mine && h.lane == 0) {
+    const float log_z = head_log(h.z);
+    log_prob[h.row] = h.bad ? NAN : h.empty ? 0.f : (float)(-d - log_z);
+    entropy[h.row] = h.bad ? NAN : h.empty ? 0.f : (float)(log_z + h.s * head_inverse(h.z));
   }
 }
 
@@ -625,34 +713,34 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_backward_kern
                                                                                   void* __restrict__ dlogits) {
   constexpr bool adjust = std::is_same<X, double>::value;
   __shared__ unsigned counts[adjust ? HEAD_THREADS : 1][E + 1];
-  for (long row0 = (long)blockIdx.x * g.rows; row0 < a.rows; row0 += (long)gridDim.x * g.rows) {
-    if constexpr (adjust) {
-      if (a.history) head_count_rows<E>(a, g, row0, counts);
-    }
-    HeadHeld<E, ONE, X, float> h;
-    h.place(a, g, row0);
-    const HeadRow r = head_row(a, h.row);
-    const HeadScale<float> scale(r);
-    const int act = actions[h.row];
-    const float gp_row = dlog_prob ? dlog_prob[h.row] : 0.f, gh = (dentropy ? dentropy[h.row] : 0.f) * scale.inv_temp;
-    h.template hold<true>(a, g, r, scale, counts[adjust ? threadIdx.x : 0]);
-    bool left = false;  // whether the action is a token that is left
-#pragma unroll
-    for (int e = 0; e < E; e++) left = left || (h.v0 + e == act && e < h.n && h.x[e] > (X)-INFINITY);
-    if (!ONE) left = head_group_max((int)left, g.lanes) != 0;
-    // (a bad row's NaN reaches every token that is left)
-    const float gp = h.bad ? NAN : left ? gp_row * scale.inv_temp : 0.f, inv_z = head_inverse(h.z);
-    const float past = h.s * inv_z;  // H - log Z
-    float y[E];
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-      const float q = h.w[e] * inv_z;
-      float d = (h.v0 + e == act ? gp : 0.f) - q * fmaf(gh, scale.surprise(h.t[e], past), gp);
-      if (adjust) d *= h.slope[e];
-      y[e] = h.x[e] != (X)-INFINITY ? d : 0.f;
-    }
-    if (h.mine) head_store<E>(dlogits, a.type, h.row * a.width + h.v0, h.n, y);
+  const long row0 = head_block() * g.rows;
+  if (row0 >= a.rows) return;
+  if constexpr (adjust) {
+    if (a.history) head_count_rows<E>(a, g, row0, counts);
   }
+  HeadHeld<E, ONE, X, float> h;
+  h.place(a, g, row0);
+  const HeadRow r = head_row(a, h.row);
+  const HeadScale<float> scale(r);
+  const int act = actions[h.row];
+  const float gp_row = dlog_prob ? dlog_prob[h.row] : 0.f, gh = (dentropy ? dentropy[h.row] : 0.f) * scale.inv_temp;
+  h.template hold<true, false>(a, g, r, scale, counts[adjust ? threadIdx.x : 0]);
+  bool left = false;  // whether the action is a token that is left
+#pragma unroll
+  for (int e = 0; e < E; e++) left = left || (h.v0 + e == act && e < h.n && h.x[e] > (X)-INFINITY);
+  if (!ONE) left = head_group_max((int)left, g.lanes) != 0;
+  // (a bad row's NaN reaches every token that is left)
+  const float gp = h.bad ? NAN : left ? gp_row * scale.inv_temp : 0.f, inv_z = head_inverse(h.z);
+  const float past = h.s * inv_z;  // H - log Z
+  float y[E];
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const float q = h.w[e] * inv_z;
+    float d = (h.v0 + e == act ? gp : 0.f) - q * fmaf(gh, scale.surprise(h.t[e], past), gp);
+    if (adjust) d *= h.slope[e];
+    y[e] = h.x[e] != (X)-INFINITY ? d : 0.f;
+  }
+  if (h.mine) head_store<E>(dlogits, a.type, h.row * a.width + h.v0, h.n, y);
 }
 
 // ---- wide rows --------------------------------------------------------------------------------------------------------
@@ -694,41 +782,46 @@ __device__ __forceinline__ V head_lane_of(V x, int lane) {
   }
 }
 
-// over a block of up to 16 waves; every thread gets the result
+// over a block of up to 16 waves; every thread gets the result.  (Two calls with the same `red` want a barrier between them.)
 template <typename V, typename F>
 __device__ __forceinline__ V head_block(V x, V none, V* red, F f) {
   x = head_lane_of(head_scan(x, none, f), 63);
-  __syncthreads();
   if (head_lane() == 0) red[threadIdx.x >> 6] = x;
   __syncthreads();
   V y = red[0];
   for (int w = 1; w < (int)(blockDim.x >> 6); w++) y = f(y, red[w]);
   return y;
 }
-template <typename V>
-__device__ __forceinline__ V head_block_max(V x, V* red) {
-  return head_block<V>(x, std::is_same<V, int>::value ? (V)-1 : (V)-INFINITY, red, [](V a, V b) { return a > b ? a : b; });
-}
 __device__ __forceinline__ int head_block_min(int x, int* red) {
   return head_block<int>(x, 0x7FFFFFFF, red, [](int a, int b) { return a < b ? a : b; });
 }
-template <typename V>
-__device__ __forceinline__ V head_block_sum(V x, V* red) {
-  return head_block<V>(x, (V)0, red, [](V a, V b) { return a + b; });
-}
-// the sum of the threads before this one, and of all
-__device__ __forceinline__ double head_block_before(double x, double* red, double& all) {
-  const double to_here = head_scan(x, 0.0, [](double a, double b) { return a + b; });
-  __syncthreads();
-  if (head_lane() == 63) red[threadIdx.x >> 6] = to_here;
-  __syncthreads();
-  double base = 0.0;
-  all = 0.0;
-  for (int w = 0; w < (int)(blockDim.x >> 6); w++) {
-    if (w == (int)(threadIdx.x >> 6)) base = all;
-    all += red[w];
+
+// Where a running sum over a block passes a target: among the n sums of whole waves in `red`, which all threads look at alike,
+// the first that does, or the last with anything in it; then among the lanes of that wave; then among a lane's tokens.
+struct HeadSpot { int entry; double base; };  // what comes before the entry
+__device__ __forceinline__ HeadSpot head_spot(const double* red, int n, double run, double target) {
+  HeadSpot spot{0, run};
+  bool over = false;
+  for (int k = 0; k < n; k++) {
+    const double x = red[k];
+    const bool take = !over && x > 0.0;
+    spot.entry = take ? k : spot.entry;
+    spot.base = take ? run : spot.base;
+    run += x;
+    over = over || (take && run > target);
   }
-  return base + (to_here - x);
+  return spot;
+}
+__device__ __forceinline__ double head_total(const double* red, int n) {
+  double all = 0.0;
+  for (int k = 0; k < n; k++) all += red[k];
+  return all;
+}
+// whether this lane is the one; what comes before it
+__device__ __forceinline__ bool head_lane_picks(double mine, double base, double target, double& before) {
+  before = base + (head_scan(mine, 0.0, [](double a, double b) { return a + b; }) - mine);
+  const unsigned long long over = __ballot(mine > 0.0 && before + mine > target), some = __ballot(mine > 0.0);
+  return head_lane() == (over ? __ffsll(over) - 1 : 63 - __clzll((long long)some));
 }
 
 // A part is CHUNKS * HEAD_CHUNK columns.
@@ -760,22 +853,22 @@ template <int CHUNKS>
 __global__ __launch_bounds__(HEAD_THREADS) void mg_adjust_wide_kernel(HeadArgs a, void* __restrict__ out, const void* __restrict__ dout,
                                                                      void* __restrict__ dlogits) {
   constexpr bool ADJUST = true;
-  for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
-    HEAD_PART_COUNTS()
-    const HeadRow r = head_row(a, row);
-    HeadAdjust<8> it[CHUNKS];
-    HEAD_PART_FETCH(it[c].template fetch<FULL>(a, r, row, (int)(part0 + at), n, dout))
+  const long row = (long)blockIdx.z * gridDim.y + blockIdx.y;
+  if (row >= a.rows) return;
+  HEAD_PART_COUNTS()
+  const HeadRow r = head_row(a, row);
+  HeadAdjust<8> it[CHUNKS];
+  HEAD_PART_FETCH(it[c].template fetch<FULL>(a, r, row, (int)(part0 + at), n, dout))
 #pragma unroll
-    for (int c = 0; c < CHUNKS; c++) {
-      const int at = c * HEAD_CHUNK + threadIdx.x * 8, n = part_n - at;
-      if (n > 0) it[c].store(a, r, row, (int)(part0 + at), n, counts + at, out, dout, dlogits);
-    }
+  for (int c = 0; c < CHUNKS; c++) {
+    const int at = c * HEAD_CHUNK + threadIdx.x * 8, n = part_n - at;
+    if (n > 0) it[c].store(a, r, row, (int)(part0 + at), n, counts + at, out, dout, dlogits);
   }
 }
 
 // What a block of THREADS knows of a part of CHUNKS * THREADS * 8 columns (X, W: as for narrow rows).
 struct HeadRed {
-  double d[2][16];
+  double m[16], z[16], s[16];
   int i[16];
 };
 template <int CHUNKS, int THREADS, typename X, typename W>
@@ -784,14 +877,15 @@ struct HeadPart {
   X x[CHUNKS][8], m;
   W w[CHUNKS][8], z, s;  // s = sum (M - x) exp(-d) / temperature
   float slope[CHUNKS][8];
-  unsigned ok[CHUNKS];
+  W z_lane[CHUNKS];  // (where the running sum is wanted) z of this thread's columns of a chunk
   bool bad, empty;
 
   __device__ __forceinline__ W far(int c, int e) const { return head_far<W, X>(top(), x[c][e]); }
   __device__ __forceinline__ X top() const { return m < (X)INFINITY && m > (X)-INFINITY ? m : (X)0; }
   static __device__ __forceinline__ int at(int c) { return (c * THREADS + threadIdx.x) * 8; }
 
-  template <bool GRAD>
+  // RUN: red.z gets the sums of waves, chunk by chunk
+  template <bool GRAD, bool RUN>
   __device__ __forceinline__ void hold(const HeadArgs& a, const HeadRow& r, const HeadScale<W>& scale, long row, long part0, int part_n,
                                        const unsigned* counts, HeadRed& red) {
     HeadRaw<8> raw[CHUNKS];
@@ -799,15 +893,16 @@ struct HeadPart {
     m = -INFINITY;
 #pragma unroll
     for (int c = 0; c < CHUNKS; c++) {
-      ok[c] = raw[c].template columns<false, GRAD, adjust>(r, a.type, (int)(part0 + at(c)), part_n - at(c), counts + at(c), x[c], slope[c]);
+      raw[c].template columns<false, GRAD, adjust>(r, a.type, (int)(part0 + at(c)), part_n - at(c), counts + at(c), x[c], slope[c]);
 #pragma unroll
       for (int e = 0; e < 8; e++) m = head_max(m, x[c][e]);
     }
-    m = head_block<X>(m, -INFINITY, (X*)red.d[0], [](X p, X q) { return head_max(p, q); });
+    m = head_block<X>(m, -INFINITY, (X*)red.m, [](X p, X q) { return head_max(p, q); });
     z = s = 0;
     bool lost = false;  // a NaN
 #pragma unroll
     for (int c = 0; c < CHUNKS; c++) {
+      if constexpr (RUN) z = 0;
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         const W t = far(c, e);
@@ -816,16 +911,28 @@ struct HeadPart {
         s = scale.sum(t, w[c][e], s);
         if (sizeof(W) == 8) lost = lost || t != t;
       }
+      if constexpr (RUN) z_lane[c] = z;
     }
     if (lost) z = NAN;
-    auto add = [](W p, W q) { return p + q; };
-    z = head_lane_of(head_scan<W>(z, 0, add), 63);
+    auto add = [](auto p, auto q) { return p + q; };
+    // (all sums before the first is stored: a branch in between, and what makes one of them is kept until after it)
+    constexpr int SUMS = RUN ? CHUNKS : 1;
+    double here[SUMS];
+    if constexpr (RUN) {
+#pragma unroll
+      for (int c = 0; c < CHUNKS; c++) here[c] = head_lane_of(head_scan<double>(z_lane[c], 0.0, add), 63);
+    } else {
+      here[0] = head_lane_of(head_scan<W>(z, 0, add), 63);
+    }
     s = head_lane_of(head_scan<W>(s, 0, add), 63);
-    __syncthreads();
-    if (head_lane() == 0) red.d[0][threadIdx.x >> 6] = z, red.d[1][threadIdx.x >> 6] = s;
-    __syncthreads();
-    z = s = 0;
-    for (int k = 0; k < THREADS / 64; k++) z += (W)red.d[0][k], s += (W)red.d[1][k];
+    if (head_lane() == 0) {
+#pragma unroll
+      for (int c = 0; c < SUMS; c++) red.z[c * (THREADS / 64) + (threadIdx.x >> 6)] = here[c];
+      red.s[threadIdx.x >> 6] = s;
+    }
+    __syncthreads();  // (and nobody reads red.m any more, so that the next row may use it)
+    z = (W)head_total(red.z, SUMS * (THREADS / 64));
+    s = (W)head_total(red.s, THREADS / 64);
     s = scale.finish(s);
     // +infinity is the largest, NaN has lost to everything but makes the sum NaN
     bad = !(m < (X)INFINITY) || z != z;
@@ -844,53 +951,88 @@ struct HeadPart {
   }
 };
 
-// ---- rows of up to HEAD_ROW columns: a block holds the row, eight columns per thread ------------------------------------
+// ---- rows of up to HEAD_ROW columns: a block holds the row ---------------------------------------------------------------
 
-template <int THREADS, typename X>
-__global__ __launch_bounds__(THREADS) void mg_sample_row_kernel(HeadArgs a, const float* __restrict__ uniforms, int* __restrict__ actions,
-                                                                    float* __restrict__ log_prob, float* __restrict__ entropy) {
+// A row whose action 32 bits cannot tell, in 64: m is the row's largest, u its uniform.  It is read again.
+template <int CHUNKS, int THREADS, typename X>
+__device__ __forceinline__ void head_sample_again(const HeadArgs& a, const HeadRow& r, long row, X m, double u, const unsigned* counts, HeadRed& red,
+                                                  int* actions, float* log_prob, float* entropy) {
+  constexpr int WAVES = THREADS / 64;
   constexpr bool adjust = std::is_same<X, double>::value;
-  __shared__ unsigned counts[adjust ? THREADS * 8 : 1];
-  __shared__ HeadRed red;
-  __shared__ double picked;
-  for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    if (adjust && a.history) head_count_columns(a, row, counts, 0, a.width);
-    const HeadRow r = head_row(a, row);
-    const HeadScale<double> scale(r);
-    HeadPart<1, THREADS, X, double> h;
-    h.template hold<false>(a, r, scale, row, 0, a.width, counts, red);
-    int hit = -1;
-    double t = 0.0;
-    if (!h.bad && !h.empty && !uniforms) hit = h.first(0, red);
-    if (!h.bad && !h.empty && uniforms) {
-      const double target = fmax((double)uniforms[row], 0.0) * h.z;
-      int over = a.width, last = -1;  // this thread's first above the target, its last with any weight
-      double mine = 0.0, all;
+  const HeadScale<double> scale(r);
+  const int wave = threadIdx.x >> 6;
+  auto look = [&](int c, double* t, double* w) {
+    const int at = (c * THREADS + threadIdx.x) * 8;
+    X x[8];
+    HeadRaw<8> raw;
+    raw.template fetch<false, adjust>(r, a.logits, a.type, row * a.logits_row + at, at, a.width - at);
+    raw.template columns<false, false, adjust>(r, a.type, at, a.width - at, counts + at, x, (float*)nullptr);
+    head_again<8>(x, m, scale, t, w);
+    double sum = 0.0;
 #pragma unroll
-      for (int e = 0; e < 8; e++) mine += h.w[0][e];
-      double run = head_block_before(mine, red.d[0], all);
+    for (int e = 0; e < 8; e++) sum += w[e];
+    return sum;
+  };
+  auto add = [](double p, double q) { return p + q; };
+  double t[8], w[8], s = 0.0;
+#pragma unroll 1
+  for (int c = 0; c < CHUNKS; c++) {
+    const double here = head_scan(look(c, t, w), 0.0, add);
+    if (head_lane() == 63) red.z[c * WAVES + wave] = here;
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        run += h.w[0][e];
-        if (run > target && over == a.width && h.w[0][e] > 0.0) over = h.at(0) + e;
-        if (h.w[0][e] > 0.0) last = h.at(0) + e;
-      }
-      hit = head_block_min(over, red.i);
-      if (hit == a.width) hit = head_block_max(last, red.i);  // a uniform of 1 or more
-#pragma unroll
-      for (int e = 0; e < 8; e++)
-        if (h.at(0) + e == hit) picked = h.far(0, e);
-      __syncthreads();
-      t = picked;
-    }
-    if (threadIdx.x == 0) {
-      const double log_z = head_log(h.z);
-      actions[row] = h.bad || h.empty ? -1 : hit;
-      log_prob[row] = h.bad ? NAN : h.empty ? 0.f : (float)(-t * scale.inv_temp - log_z);
-      entropy[row] = h.bad ? NAN : h.empty ? 0.f : (float)(log_z + h.s * head_inverse(h.z));
-    }
-    __syncthreads();
+    for (int e = 0; e < 8; e++) s = scale.sum(t[e], w[e], s);
   }
+  s = head_scan(s, 0.0, add);
+  if (head_lane() == 63) red.s[wave] = s;
+  __syncthreads();
+  const double z = head_total(red.z, CHUNKS * WAVES), target = u < 1.0 ? u * z : INFINITY;
+  const HeadSpot spot = head_spot(red.z, CHUNKS * WAVES, 0.0, target);
+  if (spot.entry % WAVES != wave) return;
+  const int c = spot.entry / WAVES;
+  double before;
+  if (!head_lane_picks(look(c, t, w), spot.base, target, before)) return;
+  const HeadPick<double> pick = head_pick<8>(w, t, before, target);
+  head_sampled(row, false, false, (c * THREADS + (int)threadIdx.x) * 8 + pick.e, pick.t, z, scale.finish(head_total(red.s, WAVES)), scale, actions,
+               log_prob, entropy);
+}
+
+template <int CHUNKS, int THREADS, typename X>
+__global__ __launch_bounds__(THREADS) void mg_sample_row_kernel(HeadArgs a, const float* __restrict__ uniforms, int* __restrict__ actions,
+                                                               float* __restrict__ log_prob, float* __restrict__ entropy) {
+  constexpr int WAVES = THREADS / 64;
+  constexpr bool adjust = std::is_same<X, double>::value;
+  __shared__ unsigned counts[adjust ? CHUNKS * THREADS * 8 : 1];
+  __shared__ HeadRed red;
+  const long row = head_block();
+  if (row >= a.rows) return;
+  if (adjust && a.history) head_count_columns(a, row, counts, 0, a.width);
+  const HeadRow r = head_row(a, row);
+  const HeadScale<float> scale(r);
+  HeadPart<CHUNKS, THREADS, X, float> h;
+  h.template hold<false, true>(a, r, scale, row, 0, a.width, counts, red);
+  if (h.bad || h.empty || !uniforms) {
+    const int first = h.bad || h.empty ? -1 : h.first(0, red);
+    if (threadIdx.x == 0) head_sampled(row, h.bad, h.empty, first, 0.f, h.z, h.s, scale, actions, log_prob, entropy);
+    return;
+  }
+  const double all = head_total(red.z, CHUNKS * WAVES), u = fmax((double)uniforms[row], 0.0), target = u < 1.0 ? u * all : INFINITY;
+  const HeadSpot spot = head_spot(red.z, CHUNKS * WAVES, 0.0, target);
+  if (spot.entry % WAVES == (int)threadIdx.x >> 6) {
+#pragma unroll
+    for (int c = 0; c < CHUNKS; c++) {
+      double before;
+      if (c != spot.entry / WAVES || !head_lane_picks(h.z_lane[c], spot.base, target, before)) continue;
+      float t[8], w[8];
+      head_again<8>(h.x[c], h.m, scale, t, w);
+      const HeadPick<float> pick = head_pick<8>(w, t, before, target);
+      const bool sure = head_sure(pick, target, head_margin(all, h.s));
+      if (sure) head_sampled(row, false, false, h.at(c) + pick.e, pick.t, h.z, h.s, scale, actions, log_prob, entropy);
+      red.i[0] = sure;
+    }
+  }
+  __syncthreads();
+  if (!red.i[0])
+    head_sample_again<CHUNKS, THREADS, X>(a, r, row, h.m, u, counts, red, actions, log_prob, entropy);
 }
 
 template <int CHUNKS, int THREADS, typename X>
@@ -898,30 +1040,38 @@ __global__ __launch_bounds__(THREADS) void mg_evaluate_row_kernel(HeadArgs a, co
                                                                  float* __restrict__ entropy, double* __restrict__ stats) {
   __shared__ unsigned counts[std::is_same<X, double>::value ? CHUNKS * THREADS * 8 : 1];
   __shared__ HeadRed red;
-  __shared__ float picked;
-  for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    if (std::is_same<X, double>::value && a.history) head_count_columns(a, row, counts, 0, a.width);
-    const HeadRow r = head_row(a, row);
-    const HeadScale<float> scale(r);
-    const int act = actions[row];
-    if (threadIdx.x == 0) picked = INFINITY;
-    HeadPart<CHUNKS, THREADS, X, float> h;
-    h.template hold<false>(a, r, scale, row, 0, a.width, counts, red);
+  const long row = head_block();
+  if (row >= a.rows) return;
+  if (std::is_same<X, double>::value && a.history) head_count_columns(a, row, counts, 0, a.width);
+  const HeadRow r = head_row(a, row);
+  const HeadScale<float> scale(r);
+  const int act = actions[row];
+  HeadPart<CHUNKS, THREADS, X, float> h;
+  h.template hold<false, false>(a, r, scale, row, 0, a.width, counts, red);
+  if ((int)threadIdx.x == (act >= 0 && act < a.width ? act / 8 % THREADS : 0)) {  // who holds the action's column
+    X x = -INFINITY;
 #pragma unroll
     for (int c = 0; c < CHUNKS; c++) {
 #pragma unroll
-      for (int e = 0; e < 8; e++)
-        if (h.at(c) + e == act && act < a.width && h.x[c][e] != (X)-INFINITY) picked = h.far(c, e) * scale.inv_temp;
+      for (int e = 0; e < 8; e++) x = h.at(c) + e == act ? h.x[c][e] : x;
     }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      const float log_z = head_log(h.z);
-      log_prob[row] = h.bad ? NAN : h.empty ? 0.f : -picked - log_z;
-      entropy[row] = h.bad ? NAN : h.empty ? 0.f : log_z + h.s * head_inverse(h.z);
-      if (stats) stats[2 * row] = h.bad ? NAN : (double)h.m, stats[2 * row + 1] = h.bad ? NAN : h.empty ? 0.0 : (double)log_z;
-    }
-    __syncthreads();
+    const float log_z = head_log(h.z), d = x == (X)-INFINITY ? INFINITY : head_far<float, X>(h.m, x) * scale.inv_temp;
+    log_prob[row] = h.bad ? NAN : h.empty ? 0.f : -d - log_z;
+    entropy[row] = h.bad ? NAN : h.empty ? 0.f : log_z + h.s * head_inverse(h.z);
+    if (stats) stats[2 * row] = h.bad ? NAN : (double)h.m, stats[2 * row + 1] = h.bad ? NAN : h.empty ? 0.0 : (double)log_z;
   }
+}
+
+// whether the action's token is left: allowed, and neither logit nor bias at -infinity
+__device__ __forceinline__ bool head_left(const HeadArgs& a, const HeadRow& r, long row, int act) {
+  if (act < 0 || act >= a.width) return false;
+  HeadRow one = r;
+  one.kind = 0;
+  HeadRaw<1> raw;
+  float l[1];
+  raw.fetch<true, false>(one, a.logits, a.type, row * a.logits_row + act, act, 1);
+  raw.values(a.type, l);
+  return head_allowed(r, act) && l[0] > -INFINITY && (!r.bias || r.bias[act] > -INFINITY);
 }
 
 template <typename X>
@@ -932,38 +1082,29 @@ __global__ __launch_bounds__(HEAD_THREADS / 2) void mg_evaluate_row_backward_ker
   constexpr bool adjust = std::is_same<X, double>::value;
   __shared__ unsigned counts[adjust ? THREADS * 8 : 1];
   __shared__ HeadRed red;
-  __shared__ int left;  // whether the action is a token that is left
-  for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    if (adjust && a.history) head_count_columns(a, row, counts, 0, a.width);
-    const HeadRow r = head_row(a, row);
-    const HeadScale<float> scale(r);
-    const int act = actions[row];
-    const float gp_row = dlog_prob ? dlog_prob[row] : 0.f, gh = (dentropy ? dentropy[row] : 0.f) * scale.inv_temp;
-    if (threadIdx.x == 0) left = 0;
-    HeadPart<CHUNKS, THREADS, X, float> h;
-    h.template hold<true>(a, r, scale, row, 0, a.width, counts, red);
+  const long row = head_block();
+  if (row >= a.rows) return;
+  if (adjust && a.history) head_count_columns(a, row, counts, 0, a.width);
+  const HeadRow r = head_row(a, row);
+  const HeadScale<float> scale(r);
+  const int act = actions[row];
+  const float gp_row = dlog_prob ? dlog_prob[row] : 0.f, gh = (dentropy ? dentropy[row] : 0.f) * scale.inv_temp;
+  const bool left = head_left(a, r, row, act);
+  HeadPart<CHUNKS, THREADS, X, float> h;
+  h.template hold<true, false>(a, r, scale, row, 0, a.width, counts, red);
+  // (a bad row's NaN reaches every token that is left)
+  const float gp = h.bad ? NAN : left ? gp_row * scale.inv_temp : 0.f, inv_z = head_inverse(h.z), past = h.s * inv_z;
 #pragma unroll
-    for (int c = 0; c < CHUNKS; c++) {
+  for (int c = 0; c < CHUNKS; c++) {
+    float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; e++)
-        if (h.at(c) + e == act && act < a.width && h.x[c][e] > (X)-INFINITY) left = 1;
+    for (int e = 0; e < 8; e++) {
+      const float q = h.w[c][e] * inv_z;
+      float d = (h.at(c) + e == act ? gp : 0.f) - q * fmaf(gh, scale.surprise(h.far(c, e), past), gp);
+      if (adjust) d *= h.slope[c][e];
+      y[e] = h.x[c][e] != (X)-INFINITY ? d : 0.f;
     }
-    __syncthreads();
-    // (a bad row's NaN reaches every token that is left)
-    const float gp = h.bad ? NAN : left ? gp_row * scale.inv_temp : 0.f, inv_z = head_inverse(h.z), past = h.s * inv_z;
-#pragma unroll
-    for (int c = 0; c < CHUNKS; c++) {
-      float y[8];
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const float q = h.w[c][e] * inv_z;
-        float d = (h.at(c) + e == act ? gp : 0.f) - q * fmaf(gh, scale.surprise(h.far(c, e), past), gp);
-        if (adjust) d *= h.slope[c][e];
-        y[e] = h.x[c][e] != (X)-INFINITY ? d : 0.f;
-      }
-      if (h.at(c) < a.width) head_store<8>(dlogits, a.type, row * a.width + h.at(c), a.width - h.at(c), y);
-    }
-    __syncthreads();
+    if (h.at(c) < a.width) head_store<8>(dlogits, a.type, row * a.width + h.at(c), a.width - h.at(c), y);
   }
 }
 
@@ -974,18 +1115,17 @@ template <int CHUNKS, bool FIRST, typename X, typename W>
 __global__ __launch_bounds__(HEAD_THREADS) void mg_head_parts_kernel(HeadArgs a, double* __restrict__ found) {
   constexpr bool ADJUST = std::is_same<X, double>::value;
   __shared__ HeadRed red;
-  for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
-    HEAD_PART_COUNTS()
-    const HeadRow r = head_row(a, row);
-    const HeadScale<W> scale(r);
-    HeadPart<CHUNKS, HEAD_THREADS, X, W> h;
-    h.template hold<false>(a, r, scale, row, part0, part_n, counts, red);
-    const int first = FIRST ? h.first(part0, red) : 0;
-    if (threadIdx.x == 0) {
-      double* f = found + (row * gridDim.x + blockIdx.x) * HEAD_FOUND;
-      f[0] = h.m; f[1] = h.z; f[2] = h.s; f[3] = h.bad ? 1.0 : 0.0; f[4] = first;
-    }
-    __syncthreads();
+  const long row = (long)blockIdx.z * gridDim.y + blockIdx.y;
+  if (row >= a.rows) return;
+  HEAD_PART_COUNTS()
+  const HeadRow r = head_row(a, row);
+  const HeadScale<W> scale(r);
+  HeadPart<CHUNKS, HEAD_THREADS, X, W> h;
+  h.template hold<false, false>(a, r, scale, row, part0, part_n, counts, red);
+  const int first = FIRST ? h.first(part0, red) : 0;
+  if (threadIdx.x == 0) {
+    double* f = found + (row * gridDim.x + blockIdx.x) * HEAD_FOUND;
+    f[0] = h.m; f[1] = h.z; f[2] = h.s; f[3] = h.bad ? 1.0 : 0.0; f[4] = first;
   }
 }
 
@@ -1024,89 +1164,74 @@ __global__ __launch_bounds__(THREADS) void mg_sample_join_kernel(HeadArgs a, int
   constexpr int PART = THREADS * 8;
   constexpr bool adjust = std::is_same<X, double>::value;
   __shared__ unsigned counts[adjust ? PART : 1];
-  __shared__ double red[THREADS / 64], picked_t, picked_run;
-  __shared__ int red_int[THREADS / 64], picked;
-  for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const HeadRow r = head_row(a, row);
-    const HeadScale<double> scale(r);
-    const double* f = found + row * parts * HEAD_FOUND;
-    const HeadJoined j = head_join(f, parts, scale, head_lane());
-    int hit = -1;
-    double t_hit = 0.0;
-    if (!j.bad && !j.empty) {
-      const double target = uniforms ? fmax((double)uniforms[row], 0.0) * j.z : 0.0;
-      if (threadIdx.x < 64) {  // one wave finds the part: the first whose running sum is above the target, or the last with any
-        double run = 0.0, before = 0.0;
-        int part = -1, last = -1, best = a.width;
-        for (int i0 = 0; i0 < parts && part < 0; i0 += 64) {
-          const int i = i0 + threadIdx.x;
-          const double mi = i < parts ? f[i * HEAD_FOUND] : -INFINITY;
-          const double w = mi == -INFINITY ? 0.0 : scale.weight(j.m - mi) * f[i * HEAD_FOUND + 1];
-          const double to_here = run + head_scan(w, 0.0, [](double p, double q) { return p + q; });
-          if (!uniforms && mi == j.m) best = min(best, (int)f[i * HEAD_FOUND + 4]);
-          const unsigned long long over = __ballot(w > 0.0 && to_here > target), some = __ballot(w > 0.0);
-          if (uniforms && over) {
-            const int k = __ffsll(over) - 1;
-            part = i0 + k;
-            before = head_lane_of(to_here - w, k);
-          } else if (some) {
-            const int k = 63 - __clzll((long long)some);
-            last = i0 + k;
-            before = head_lane_of(to_here - w, k);
-          }
-          run = head_lane_of(to_here, 63);
-        }
-        best = head_group_min(best, 64);
-        if (threadIdx.x == 0) picked = !uniforms ? best : part >= 0 ? part : last, picked_run = before;
+  __shared__ double red[16];
+  const long row = head_block();
+  if (row >= a.rows) return;
+  const HeadRow r = head_row(a, row);
+  const HeadScale<double> scale(r);
+  const double* f = found + row * parts * HEAD_FOUND;
+  const HeadJoined j = head_join(f, parts, scale, head_lane());
+  const double u = uniforms ? fmax((double)uniforms[row], 0.0) : 0.0, target = u < 1.0 ? u * j.z : INFINITY;
+  HeadPick<double> pick{0, 0.0, 0.0, 0.0};
+  bool picks = threadIdx.x == 0;
+  int v0 = 0;
+  if (!j.bad && !j.empty) {
+    // every wave finds the part: the first whose running sum is above the target, or the last with any (without uniforms:
+    // the first of those with the largest)
+    double start = 0.0, run = 0.0;
+    int part = -1, last = -1, best = a.width;
+    for (int i0 = 0; i0 < parts && part < 0; i0 += 64) {
+      const int i = i0 + head_lane();
+      const double mi = i < parts ? f[i * HEAD_FOUND] : -INFINITY;
+      const double w = mi == -INFINITY ? 0.0 : scale.weight(j.m - mi) * f[i * HEAD_FOUND + 1];
+      const double to_here = run + head_scan(w, 0.0, [](double p, double q) { return p + q; });
+      if (!uniforms && mi == j.m) best = min(best, (int)f[i * HEAD_FOUND + 4]);
+      const unsigned long long over = __ballot(w > 0.0 && to_here > target), some = __ballot(w > 0.0);
+      if (uniforms && over) {
+        const int k = __ffsll(over) - 1;
+        part = i0 + k;
+        start = head_lane_of(to_here - w, k);
+      } else if (some) {
+        const int k = 63 - __clzll((long long)some);
+        last = i0 + k;
+        start = head_lane_of(to_here - w, k);
       }
+      run = head_lane_of(to_here, 63);
+    }
+    if (!uniforms) {
+      v0 = head_group_min(best, 64);
+    } else {
+      part = part >= 0 ? part : last;
+      const long part0 = (long)part * PART;
+      const int part_n = (int)min((long)PART, a.width - part0);
+      if (adjust && a.history) head_count_columns(a, row, counts, part0, part_n);
+      const int at = threadIdx.x * 8, n = part_n - at;
+      X x[8];
+      double t[8], w[8], mine = 0.0;
+      HeadRaw<8> raw;
+      raw.template fetch<false, adjust>(r, a.logits, a.type, row * a.logits_row + part0 + at, (int)(part0 + at), n);
+      raw.template columns<false, false, adjust>(r, a.type, (int)(part0 + at), n, counts + at, x, (float*)nullptr);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        t[e] = j.m - (double)x[e];
+        w[e] = scale.weight(t[e]);
+        mine += w[e];
+      }
+      const double here = head_scan(mine, 0.0, [](double p, double q) { return p + q; });
+      if (head_lane() == 63) red[threadIdx.x >> 6] = here;
       __syncthreads();
-      if (!uniforms) {
-        hit = picked;
-      } else {
-        const long part0 = (long)picked * PART;
-        const int part_n = (int)min((long)PART, a.width - part0);
-        if (adjust && a.history) head_count_columns(a, row, counts, part0, part_n);
-        const int at = threadIdx.x * 8, n = part_n - at;
-        X x[8];
-        double t[8], w[8], mine = 0.0;
-        HeadRaw<8> raw;
-        raw.template fetch<false, adjust>(r, a.logits, a.type, row * a.logits_row + part0 + at, (int)(part0 + at), n);
-        raw.template columns<false, false, adjust>(r, a.type, (int)(part0 + at), n, counts + at, x, (float*)nullptr);
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          t[e] = j.m - (double)x[e];
-          w[e] = scale.weight(t[e]);
-          mine += w[e];
-        }
-        double all;
-        double run = picked_run + head_block_before(mine, red, all);
-        int over = a.width, last = -1;
-        double t_over = 0.0, t_last = 0.0;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          run += w[e];
-          if (run > target && over == a.width && w[e] > 0.0) over = (int)(part0 + at + e), t_over = t[e];
-          if (w[e] > 0.0) last = (int)(part0 + at + e), t_last = t[e];
-        }
-        hit = head_block_min(over, red_int);
-        if (hit < a.width) {
-          if (over == hit) picked_t = t_over;
-        } else {  // a uniform of 1 or more, or one that the roundings of a border took
-          hit = head_block_max(last, red_int);
-          if (last == hit) picked_t = t_last;
-        }
-        __syncthreads();
-        t_hit = picked_t;
+      const HeadSpot spot = head_spot(red, THREADS / 64, start, target);
+      picks = false;
+      if (spot.entry == (int)threadIdx.x >> 6) {
+        double before;
+        picks = head_lane_picks(mine, spot.base, target, before);
+        if (picks) pick = head_pick<8>(w, t, before, target);
       }
+      v0 = (int)(part0 + at);
+      __syncthreads();
     }
-    if (threadIdx.x == 0) {
-      const double log_z = head_log(j.z);
-      actions[row] = j.bad || j.empty ? -1 : hit;
-      log_prob[row] = j.bad ? NAN : j.empty ? 0.f : (float)(-t_hit * scale.inv_temp - log_z);
-      entropy[row] = j.bad ? NAN : j.empty ? 0.f : (float)(log_z + j.s / j.z);
-    }
-    __syncthreads();
   }
+  if (picks) head_sampled(row, j.bad, j.empty, v0 + pick.e, pick.t, j.z, j.s, scale, actions, log_prob, entropy);
 }
 
 // one wave per row
@@ -1142,66 +1267,57 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_join_kernel(HeadArgs
   }
 }
 
-// (four waves per SIMD: 69 us on 2048 x 32003 bf16 against 80 with three and more registers each)
 template <int CHUNKS, typename X>
-__global__ __launch_bounds__(HEAD_THREADS, (sizeof(X) == 4 ? 4 : 2)) void mg_evaluate_wide_backward_kernel(HeadArgs a, const int* __restrict__ actions,
+__global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_wide_backward_kernel(HeadArgs a, const int* __restrict__ actions,
                                                                                 const float* __restrict__ entropy,
                                                                                 const double* __restrict__ stats,
                                                                                 const float* __restrict__ dlog_prob,
                                                                                 const float* __restrict__ dentropy,
                                                                                 void* __restrict__ dlogits) {
   constexpr bool ADJUST = std::is_same<X, double>::value;
-  for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
-    HEAD_PART_COUNTS()
-    const HeadRow r = head_row(a, row);
-    const HeadScale<float> scale(r);
-    const double m = stats[2 * row];
-    const float log_z = (float)stats[2 * row + 1], past = (float)((double)entropy[row] - stats[2 * row + 1]);  // H - log Z
-    const bool bad = m != m, empty = m == -INFINITY;
-    const X top = bad || empty ? (X)0 : (X)m;
-    const int act = actions[row];
-    float gp = 0;
-    const float gh = (dentropy ? dentropy[row] : 0.f) * scale.inv_temp;
-    if (dlog_prob && act >= 0 && act < a.width) {  // the action's token is left if it is allowed and not at -infinity
-      HeadRow one = r;
-      one.kind = 0;
-      HeadRaw<1> raw;
-      float l[1];
-      raw.fetch<true, false>(one, a.logits, a.type, row * a.logits_row + act, act, 1);
-      raw.values(a.type, l);
-      if (head_allowed(r, act) && l[0] > -INFINITY && (!r.bias || r.bias[act] > -INFINITY)) gp = dlog_prob[row] * scale.inv_temp;
+  const long row = (long)blockIdx.z * gridDim.y + blockIdx.y;
+  if (row >= a.rows) return;
+  HEAD_PART_COUNTS()
+  const HeadRow r = head_row(a, row);
+  const HeadScale<float> scale(r);
+  const double m = stats[2 * row];
+  const float log_z = (float)stats[2 * row + 1], past = (float)((double)entropy[row] - stats[2 * row + 1]);  // H - log Z
+  const bool bad = m != m, empty = m == -INFINITY;
+  const X top = bad || empty ? (X)0 : (X)m;
+  const int act = actions[row];
+  float gp = 0;
+  const float gh = (dentropy ? dentropy[row] : 0.f) * scale.inv_temp;
+  if (dlog_prob && head_left(a, r, row, act)) gp = dlog_prob[row] * scale.inv_temp;
+  constexpr bool adjust = ADJUST;
+  HeadRaw<8> raw[CHUNKS];
+  HEAD_PART_FETCH((raw[c].template fetch<FULL, adjust>(r, a.logits, a.type, row * a.logits_row + part0 + at, (int)(part0 + at), n)))
+#pragma unroll
+  for (int c = 0; c < CHUNKS; c++) {
+    const int at = c * HEAD_CHUNK + threadIdx.x * 8, n = part_n - at;
+    if (n <= 0) continue;
+    const int v0 = (int)(part0 + at);
+    X x[8];
+    float g[8], slope[8], y[8];
+    const unsigned ok = raw[c].template columns<false, true, adjust>(r, a.type, v0, n, counts + at, x, slope);
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const float t = (float)(top - x[e]);
+      g[e] = -scale.weight(t, log_z) * fmaf(gh, scale.surprise(t, past), gp);
     }
-    constexpr bool adjust = ADJUST;
-    HeadRaw<8> raw[CHUNKS];
-    HEAD_PART_FETCH((raw[c].template fetch<FULL, adjust>(r, a.logits, a.type, row * a.logits_row + part0 + at, (int)(part0 + at), n)))
+    if ((unsigned)(act - v0) < 8u) {
 #pragma unroll
-    for (int c = 0; c < CHUNKS; c++) {
-      const int at = c * HEAD_CHUNK + threadIdx.x * 8, n = part_n - at;
-      if (n <= 0) continue;
-      const int v0 = (int)(part0 + at);
-      X x[8];
-      float g[8], slope[8], y[8];
-      const unsigned ok = raw[c].template columns<false, true, adjust>(r, a.type, v0, n, counts + at, x, slope);
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const float t = (float)(top - x[e]);
-        g[e] = -scale.weight(t, log_z) * fmaf(gh, scale.surprise(t, past), gp);
-      }
-      if ((unsigned)(act - v0) < 8u) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) if (v0 + e == act) g[e] += gp;
-      }
-      if (bad || empty) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) g[e] = bad ? NAN : 0;
-      }
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        if (adjust) g[e] *= slope[e];
-        y[e] = __uint_as_float(__float_as_uint(g[e]) & head_bit(ok, e));
-      }
-      head_store<8>(dlogits, a.type, row * a.width + v0, n, y);
+      for (int e = 0; e < 8; e++) if (v0 + e == act) g[e] += gp;
     }
+    if (bad || empty) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) g[e] = bad ? NAN : 0;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      if (adjust) g[e] *= slope[e];
+      y[e] = __uint_as_float(__float_as_uint(g[e]) & head_bit(ok, e));
+    }
+    head_store<8>(dlogits, a.type, row * a.width + v0, n, y);
   }
 }
 
@@ -1237,21 +1353,25 @@ static int head_chunks(const mg_logits* a) {
   return a->width > 2 * HEAD_CHUNK && (int64_t)((a->width - 1) / (4 * HEAD_CHUNK) + 1) * a->rows >= 2048 ? 4 : 1;
 }
 static int head_parts(const mg_logits* a) { return (a->width - 1) / (head_chunks(a) * HEAD_CHUNK) + 1; }
-static dim3 head_wide_grid(const mg_logits* a) { return dim3(head_parts(a), (unsigned)(a->rows < 32768 ? a->rows : 32768)); }
+// A block does one row (or, of narrow ones, as many as its lanes hold) and no loop over them: the compiler would keep what does
+// not change from row to row in registers, the constants of a rare path too.
+static dim3 head_wide_grid(const mg_logits* a) {
+  const int64_t y = a->rows < 32768 ? a->rows : 32768;
+  return dim3(head_parts(a), (unsigned)y, (unsigned)((a->rows + y - 1) / y));
+}
+static dim3 head_grid(int64_t blocks) {
+  const int64_t x = blocks < 1 << 20 ? blocks : 1 << 20;
+  return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
+}
 static bool head_narrow(const mg_logits* a) { return a->width <= HEAD_NARROW; }
 static bool head_remembers(const mg_logits* a) { return a->width > MG_EVALUATE_STATS_WIDTH; }  // what the forward pass found
 static bool head_wide(const mg_logits* a) { return a->width > HEAD_ROW; }
-static unsigned head_row_blocks(const mg_logits* a) { return (unsigned)(a->rows < 1 << 20 ? a->rows : 1 << 20); }
 
 // lanes per row: as many as hold the row with E columns each; a power of two where they work on it together
 static HeadNarrow head_layout(const mg_logits* a, int e, bool together) {
   int lanes = together ? 1 : (a->width + e - 1) / e;
   while (lanes * e < a->width) lanes *= 2;
   return HeadNarrow{lanes, HEAD_THREADS / lanes};
-}
-static unsigned head_blocks(int64_t rows, int per_block) {
-  const int64_t n = (rows + per_block - 1) / per_block;
-  return (unsigned)(n < (1 << 23) ? n : 1 << 23);  // (a grid has fewer than 2^32 threads; the kernels loop)
 }
 
 template <int V> using head_int = std::integral_constant<int, V>;
@@ -1272,18 +1392,10 @@ static void head_by_width(const mg_logits* a, F f) {
   }
   f(head_int<8>(), head_bool<false>(), head_layout(a, 8, true));
 }
-// the threads of a block that holds a row
+// how a block holds a row: chunks of eight columns per thread, and threads.  Rather more chunks than more threads to wait for
+// (evaluation of 4096 x 8192 bf16: 33 us with 256 threads, 56 with 1024).
 template <typename F>
 static void head_by_row(const mg_logits* a, F f) {
-  if (a->width <= HEAD_CHUNK / 2) f(head_int<HEAD_THREADS / 2>());
-  else if (a->width <= HEAD_CHUNK) f(head_int<HEAD_THREADS>());
-  else if (a->width <= 2 * HEAD_CHUNK) f(head_int<2 * HEAD_THREADS>());
-  else f(head_int<4 * HEAD_THREADS>());
-}
-// the chunks of a row that each thread of a smaller block holds: fewer threads to wait for, where 32 bits leave the registers
-// (4096 x 8192 bf16: 33 us with 256 threads, 56 with 1024)
-template <typename F>
-static void head_by_row_chunks(const mg_logits* a, F f) {
   if (a->width <= HEAD_CHUNK / 2) f(head_int<1>(), head_int<HEAD_THREADS / 2>());
   else if (a->width <= HEAD_CHUNK) f(head_int<1>(), head_int<HEAD_THREADS>());
   else if (a->width <= 2 * HEAD_CHUNK) f(head_int<2>(), head_int<HEAD_THREADS>());
@@ -1320,7 +1432,7 @@ static int head_adjust(const char* who, const mg_logits* a, void* out, const voi
   const hipStream_t s = (hipStream_t)stream;
   if (a->width <= HEAD_CHUNK / 2) {
     const HeadNarrow g = head_layout(a, 8, false);
-    hipLaunchKernelGGL(mg_adjust_narrow_kernel<8>, dim3(head_blocks(a->rows, g.rows)), dim3(HEAD_THREADS), 0, s, head_args(a), g, out, dout, dlogits);
+    hipLaunchKernelGGL(mg_adjust_narrow_kernel<8>, head_grid((a->rows + g.rows - 1) / g.rows), dim3(HEAD_THREADS), 0, s, head_args(a), g, out, dout, dlogits);
   } else {
     head_by_chunks(a, [&](auto c) {
       hipLaunchKernelGGL(mg_adjust_wide_kernel<decltype(c)::value>, head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), out, dout, dlogits);
@@ -1359,13 +1471,13 @@ extern "C" int mg_sample_actions(const mg_logits* a, const float* uniforms, int3
     using X = std::remove_pointer_t<decltype(null)>;
     if (head_narrow(a)) {
       head_by_width(a, [&](auto e, auto one, HeadNarrow g) {
-        hipLaunchKernelGGL((mg_sample_narrow_kernel<decltype(e)::value, decltype(one)::value, X>), dim3(head_blocks(a->rows, g.rows)),
+        hipLaunchKernelGGL((mg_sample_narrow_kernel<decltype(e)::value, decltype(one)::value, X>), head_grid((a->rows + g.rows - 1) / g.rows),
                            dim3(HEAD_THREADS), 0, s, head_args(a), g, uniforms, actions, log_prob, entropy);
       });
     } else if (!head_wide(a)) {
-      head_by_row(a, [&](auto c) {
-        hipLaunchKernelGGL((mg_sample_row_kernel<decltype(c)::value, X>), dim3(head_row_blocks(a)), dim3(decltype(c)::value), 0, s, head_args(a),
-                           uniforms, actions, log_prob, entropy);
+      head_by_row(a, [&](auto c, auto t) {
+        hipLaunchKernelGGL((mg_sample_row_kernel<decltype(c)::value, decltype(t)::value, X>), head_grid(a->rows), dim3(decltype(t)::value), 0, s,
+                           head_args(a), uniforms, actions, log_prob, entropy);
       });
     } else {
       head_by_chunks(a, [&](auto c) {
@@ -1374,7 +1486,7 @@ extern "C" int mg_sample_actions(const mg_logits* a, const float* uniforms, int3
           hipLaunchKernelGGL((mg_head_parts_kernel<C, false, X, double>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), (double*)a->workspace);
         else
           hipLaunchKernelGGL((mg_head_parts_kernel<C, true, X, double>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), (double*)a->workspace);
-        hipLaunchKernelGGL((mg_sample_join_kernel<C * HEAD_THREADS, X>), dim3(head_row_blocks(a)), dim3(C * HEAD_THREADS), 0, s, head_args(a),
+        hipLaunchKernelGGL((mg_sample_join_kernel<C * HEAD_THREADS, X>), head_grid(a->rows), dim3(C * HEAD_THREADS), 0, s, head_args(a),
                            head_parts(a), (const double*)a->workspace, uniforms, actions, log_prob, entropy);
       });
     }
@@ -1396,12 +1508,12 @@ extern "C" int mg_evaluate_actions(const mg_logits* a, const int32_t* actions, f
     using X = std::remove_pointer_t<decltype(null)>;
     if (head_narrow(a)) {
       head_by_width(a, [&](auto e, auto one, HeadNarrow g) {
-        hipLaunchKernelGGL((mg_evaluate_narrow_kernel<decltype(e)::value, decltype(one)::value, X>), dim3(head_blocks(a->rows, g.rows)), dim3(HEAD_THREADS), 0, s,
+        hipLaunchKernelGGL((mg_evaluate_narrow_kernel<decltype(e)::value, decltype(one)::value, X>), head_grid((a->rows + g.rows - 1) / g.rows), dim3(HEAD_THREADS), 0, s,
                            head_args(a), g, actions, log_prob, entropy);
       });
     } else if (!head_wide(a)) {
-      head_by_row_chunks(a, [&](auto c, auto t) {
-        hipLaunchKernelGGL((mg_evaluate_row_kernel<decltype(c)::value, decltype(t)::value, X>), dim3(head_row_blocks(a)), dim3(decltype(t)::value), 0,
+      head_by_row(a, [&](auto c, auto t) {
+        hipLaunchKernelGGL((mg_evaluate_row_kernel<decltype(c)::value, decltype(t)::value, X>), head_grid(a->rows), dim3(decltype(t)::value), 0,
                            s, head_args(a), actions, log_prob, entropy, stats);
       });
     } else {
@@ -1430,11 +1542,11 @@ extern "C" int mg_evaluate_actions_backward(const mg_logits* a, const int32_t* a
     using X = std::remove_pointer_t<decltype(null)>;
     if (head_narrow(a))
       head_by_width(a, [&](auto e, auto one, HeadNarrow g) {
-        hipLaunchKernelGGL((mg_evaluate_narrow_backward_kernel<decltype(e)::value, decltype(one)::value, X>), dim3(head_blocks(a->rows, g.rows)), dim3(HEAD_THREADS),
+        hipLaunchKernelGGL((mg_evaluate_narrow_backward_kernel<decltype(e)::value, decltype(one)::value, X>), head_grid((a->rows + g.rows - 1) / g.rows), dim3(HEAD_THREADS),
                            0, s, head_args(a), g, actions, dlog_prob, dentropy, dlogits);
       });
     else if (!head_remembers(a))
-      hipLaunchKernelGGL(mg_evaluate_row_backward_kernel<X>, dim3(head_row_blocks(a)), dim3(HEAD_THREADS / 2), 0, s, head_args(a), actions,
+      hipLaunchKernelGGL(mg_evaluate_row_backward_kernel<X>, head_grid(a->rows), dim3(HEAD_THREADS / 2), 0, s, head_args(a), actions,
                          dlog_prob, dentropy, dlogits);
     else
       head_by_chunks(a, [&](auto c) {

@@ -480,22 +480,33 @@ def test_far_tokens_and_ends_of_the_temperature(v, bias):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("v", [3, 64, 300, 40000])
-def test_uniforms_next_to_borders(v):
+@pytest.mark.parametrize("controls", [False, True])
+@pytest.mark.parametrize("v", [3, 8, 9, 64, 300, 700, 1500, 3000, 8000, 40000])
+def test_uniforms_next_to_borders(v, controls):
     """Uniforms set right at the borders of the distribution, one step of 32 bits below, on and above them: the picked
     action is still the one of the 64-bit definition."""
     g = torch.Generator().manual_seed(v)
     logits = torch.randn(1, v, generator=g)
-    s = _stats(_adjusted(logits, temperature=0.9)[0])
+    c = dict(temperature=0.9)
+    if controls:
+        c.update(bias=torch.randn(v, generator=g), allowed=torch.rand(v, generator=g) < 0.7, history=torch.arange(0, v, 3)[None, :200].int(),
+                 repetition=1.2, frequency=0.1)  # fmt: skip
+        c["allowed"][1] = True
+    l = _adjusted(logits, **c)[0]
+    s = _stats(l)
     run = np.cumsum(s["e"][0]) / s["z"][0]
     at = np.unique(np.linspace(0, v - 2, min(v - 1, 400)).astype(int))
     border = run[at].astype(np.float32)
     u = np.concatenate([border, np.nextafter(border, np.float32(0)), np.nextafter(border, np.float32(1))])
     u = np.minimum(u, np.float32(1 - 2.0**-24))
     rows = logits.repeat(len(u), 1)
-    a, _, _ = sample_actions(rows.cuda(), torch.from_numpy(u).cuda(), temperature=0.9)
-    want = _picked(_adjusted(logits, temperature=0.9)[0].repeat(len(u), 0), u.astype(np.float64))
+    if controls:
+        c["history"] = c["history"].repeat(len(u), 1)
+    a, logp, h = sample_actions(rows.cuda(), torch.from_numpy(u).cuda(), **_cuda(c))
+    l = l.repeat(len(u), 0)
+    want = _picked(l, u.astype(np.float64))
     assert np.array_equal(a.cpu().numpy(), want)
+    _check_rows(logp, h, l, want)
 
 
 @pytest.mark.gpu
