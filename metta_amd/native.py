@@ -17,6 +17,7 @@ _LIB_PATH_WIDE = Path(__file__).resolve().parent / "libmettagrid_hip_r32.so"
 NARROW_MAX_RESOURCES, WIDE_MAX_RESOURCES = 16, 32
 _lib = None
 _lib_wide = None
+_operators = None
 
 
 class MgBuffers(ct.Structure):
@@ -94,10 +95,6 @@ class MgLogits(ct.Structure):
         ("type", ct.c_int32),
     ]
 
-
-MARK_STEPS = 16  # MG_RECURRENCE_MARK_STEPS
-STATS_WIDTH = 1024  # MG_EVALUATE_STATS_WIDTH
-ALLOWED_BOOL, ALLOWED_BITS = 1, 2  # MG_ALLOWED_*
 
 # name -> (restype, argtypes); every symbol include/mettagrid_hip.h declares
 _vp, _i32p, _u32p, _u8p, _f32p, _f64p = (
@@ -211,6 +208,35 @@ def load(wide: bool = False) -> ct.CDLL:
     else:
         _lib = L
     return L
+
+
+# what metta_amd/csrc/operators.cpp calls
+OPERATORS = (
+    "mg_last_error",
+    "mg_gated_recurrence_workspace",
+    "mg_gated_recurrence",
+    "mg_gated_recurrence_backward",
+    "mg_logits_workspace",
+    "mg_adjust_logits",
+    "mg_adjust_logits_backward",
+    "mg_sample_actions",
+    "mg_evaluate_actions",
+    "mg_evaluate_actions_backward",
+)
+
+
+def operators():
+    """The operators on tensors (metta_amd/csrc/operators.cpp), bound to the library that `load` gives."""
+    global _operators
+    if _operators is None:
+        L = load()
+        try:
+            from metta_amd import _operators as module
+        except ImportError as e:
+            raise ImportError(f"metta_amd/_operators.so cannot be loaded: build it with `make -C metta_amd/csrc` ({e})") from e
+        module.bind({name: ct.cast(getattr(L, name), ct.c_void_p).value for name in OPERATORS})
+        _operators = module
+    return _operators
 
 
 def load_for(num_resources: int) -> ct.CDLL:

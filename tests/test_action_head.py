@@ -685,5 +685,5 @@ def test_saved_tensors_are_watched_and_second_derivatives_refused():
         logp.sum().backward()
     for out in (evaluate_actions(x, torch.zeros(4, dtype=torch.int64, device="cuda"))[0], adjust_logits(x)):
         (d,) = torch.autograd.grad(out.sum(), x, create_graph=True)
-        with pytest.raises(RuntimeError, match="once_differentiable|does not require grad"):
+        with pytest.raises(RuntimeError, match="differentiable once"):
             d.sum().backward()

@@ -452,7 +452,7 @@ def test_saved_tensors_that_move(packed, dtype):
 def test_second_derivatives_are_refused():
     x = torch.randn(2, 20, 4, device="cuda", requires_grad=True)
     (d,) = torch.autograd.grad(gated_recurrence(x, x)[0].sum(), x, create_graph=True)
-    with pytest.raises(RuntimeError, match="once_differentiable|does not require grad"):
+    with pytest.raises(RuntimeError, match="differentiable once"):
         d.sum().backward()
 
 
