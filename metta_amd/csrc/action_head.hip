@@ -13,7 +13,7 @@
 //
 // Rows of up to HEAD_NARROW columns are held in registers, E adjacent columns per lane, by as many lanes as that takes
 // (one lane for five actions, a wave for five hundred); rows of up to HEAD_ROW columns by a block, in chunks of eight columns
-// per thread.  Their logits are read once.  Wider rows are cut into parts of one or four chunks, a block each; what a part
+// per thread.  Their logits are read once.  Wider rows are cut into parts, a block each; what a part
 // found (maximum, sum, ...) goes to a workspace and a second launch joins the parts of a row.  A history is counted in LDS by
 // the block that needs it, for the columns that it holds.
 //
@@ -611,6 +611,9 @@ __device__ __forceinline__ void head_sampled(long row, bool bad, bool empty, int
   entropy[row] = bad ? NAN : empty ? 0.f : (float)(log_z + s * head_inverse(z));
 }
 
+// Adjusted logits or their gradient, E columns per lane and no word between lanes.  Bound by memory without a history (32768 x
+// 512 bf16: 14 us for 67 MB, 4.9 TB/s), by counting it with one (24576 x 157 f32, masks, 32 entries: 14 us each way for 38
+// and 53 MB).
 template <int E>
 __global__ __launch_bounds__(HEAD_THREADS) void mg_adjust_narrow_kernel(HeadArgs a, HeadNarrow g, void* __restrict__ out,
                                                                        const void* __restrict__ dout, void* __restrict__ dlogits) {
@@ -627,6 +630,8 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_adjust_narrow_kernel(HeadArgs
   it.store(a, r, h.row, h.v0, h.n, counts[threadIdx.x], out, dout, dlogits);
 }
 
+// An action per row.  Bound by the launch and the way through it (24 x 5: 1.8 us; 98304 x 5 bf16, masks, 16 entries of history:
+// 6.4 us for 9 MB), from some 50 columns on by its instructions (98304 x 64 bf16: 10.6 us; all in 64 bits: 18).
 template <int E, bool ONE, typename X>
 __global__ __launch_bounds__(HEAD_THREADS) void mg_sample_narrow_kernel(HeadArgs a, HeadNarrow g, const float* __restrict__ uniforms,
                                                                        int* __restrict__ actions, float* __restrict__ log_prob,
@@ -678,6 +683,8 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_sample_narrow_kernel(HeadArgs
   }
 }
 
+// Bound by memory at few columns (2097152 x 5 bf16: 10.6 us for 46 MB, 4.3 TB/s), by its instructions at many (32768 x 512 bf16: 18
+// us).
 template <int E, bool ONE, typename X>
 __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_kernel(HeadArgs a, HeadNarrow g, const int* __restrict__ actions,
                                                                          float* __restrict__ log_prob, float* __restrict__ entropy) {
@@ -706,6 +713,7 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_kernel(HeadAr
   }
 }
 
+// The row's sums are computed again, which costs less than reading them (2097152 x 5 bf16: 13.6 us for 67 MB, 4.9 TB/s).
 template <int E, bool ONE, typename X>
 __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_backward_kernel(HeadArgs a, HeadNarrow g, const int* __restrict__ actions,
                                                                                   const float* __restrict__ dlog_prob,
@@ -824,14 +832,6 @@ __device__ __forceinline__ bool head_lane_picks(double mine, double base, double
   return head_lane() == (over ? __ffsll(over) - 1 : 63 - __clzll((long long)some));
 }
 
-// A part is CHUNKS * HEAD_CHUNK columns.
-#define HEAD_PART_COUNTS()                                                                      \
-  __shared__ unsigned counts[ADJUST ? CHUNKS * HEAD_CHUNK : 1];                                 \
-  constexpr int THREADS [[maybe_unused]] = HEAD_THREADS;                                        \
-  const long part0 = (long)blockIdx.x * (CHUNKS * HEAD_CHUNK);                                  \
-  const int part_n = (int)min((long)CHUNKS * HEAD_CHUNK, a.width - part0);                      \
-  if (ADJUST && a.history) head_count_columns(a, row, counts, part0, part_n);
-
 // `fetch` for every chunk c of the part, whose columns of this thread start at `at` with n of them left; FULL says whether
 // the part lies in the row as a whole
 #define HEAD_PART_FETCH(fetch)                                                                  \
@@ -849,21 +849,20 @@ __device__ __forceinline__ bool head_lane_picks(double mine, double base, double
     }                                                                                           \
   }
 
-template <int CHUNKS>
+// Bound by memory where there is enough of it (1024 x 32003 bf16: 23 us for 131 MB, 5.7 TB/s, part of it in the caches), else by
+// latency (64 x 50001 bf16, all controls, 512 entries of history that every block of a row counts: 8.1 us for 13 MB).
 __global__ __launch_bounds__(HEAD_THREADS) void mg_adjust_wide_kernel(HeadArgs a, void* __restrict__ out, const void* __restrict__ dout,
                                                                      void* __restrict__ dlogits) {
-  constexpr bool ADJUST = true;
-  const long row = (long)blockIdx.z * gridDim.y + blockIdx.y;
+  __shared__ unsigned counts[HEAD_CHUNK];
+  const long row = (long)blockIdx.z * gridDim.y + blockIdx.y, part0 = (long)blockIdx.x * HEAD_CHUNK;
   if (row >= a.rows) return;
-  HEAD_PART_COUNTS()
+  const int part_n = (int)min((long)HEAD_CHUNK, a.width - part0), at = threadIdx.x * 8, n = part_n - at, v0 = (int)(part0 + at);
+  if (a.history) head_count_columns(a, row, counts, part0, part_n);
   const HeadRow r = head_row(a, row);
-  HeadAdjust<8> it[CHUNKS];
-  HEAD_PART_FETCH(it[c].template fetch<FULL>(a, r, row, (int)(part0 + at), n, dout))
-#pragma unroll
-  for (int c = 0; c < CHUNKS; c++) {
-    const int at = c * HEAD_CHUNK + threadIdx.x * 8, n = part_n - at;
-    if (n > 0) it[c].store(a, r, row, (int)(part0 + at), n, counts + at, out, dout, dlogits);
-  }
+  HeadAdjust<8> it;
+  if (part_n == HEAD_CHUNK) it.fetch<true>(a, r, row, v0, 8, dout);
+  else it.fetch<false>(a, r, row, v0, n, dout);
+  if (n > 0) it.store(a, r, row, v0, n, counts + at, out, dout, dlogits);
 }
 
 // What a block of THREADS knows of a part of CHUNKS * THREADS * 8 columns (X, W: as for narrow rows).
@@ -996,6 +995,8 @@ __device__ __forceinline__ void head_sample_again(const HeadArgs& a, const HeadR
                log_prob, entropy);
 }
 
+// An action per row.  Bound by its instructions (16384 x 1024 bf16: 21 us for 34 MB; 4096 x 8192: 37 us for 67 MB; all in 64 bits
+// 39 and 122).
 template <int CHUNKS, int THREADS, typename X>
 __global__ __launch_bounds__(THREADS) void mg_sample_row_kernel(HeadArgs a, const float* __restrict__ uniforms, int* __restrict__ actions,
                                                                float* __restrict__ log_prob, float* __restrict__ entropy) {
@@ -1035,6 +1036,7 @@ __global__ __launch_bounds__(THREADS) void mg_sample_row_kernel(HeadArgs a, cons
     head_sample_again<CHUNKS, THREADS, X>(a, r, row, h.m, u, counts, red, actions, log_prob, entropy);
 }
 
+// 4096 x 8192 bf16: 20 us for 67 MB, 3.4 TB/s; 16384 x 1024: 13 us.
 template <int CHUNKS, int THREADS, typename X>
 __global__ __launch_bounds__(THREADS) void mg_evaluate_row_kernel(HeadArgs a, const int* __restrict__ actions, float* __restrict__ log_prob,
                                                                  float* __restrict__ entropy, double* __restrict__ stats) {
@@ -1074,6 +1076,7 @@ __device__ __forceinline__ bool head_left(const HeadArgs& a, const HeadRow& r, l
   return head_allowed(r, act) && l[0] > -INFINITY && (!r.bias || r.bias[act] > -INFINITY);
 }
 
+// For rows of up to MG_EVALUATE_STATS_WIDTH columns, whose sums are computed again (16384 x 1024 bf16: 20 us for 67 MB).
 template <typename X>
 __global__ __launch_bounds__(HEAD_THREADS / 2) void mg_evaluate_row_backward_kernel(HeadArgs a, const int* __restrict__ actions,
                                                                                const float* __restrict__ dlog_prob,
@@ -1110,14 +1113,19 @@ __global__ __launch_bounds__(HEAD_THREADS / 2) void mg_evaluate_row_backward_ker
 
 // ---- wider rows: parts, and a second launch that joins them ------------------------------------------------------------
 
-// found[row][part] = M, Z, sum (M - x) exp(-d) / temperature (against the part's own M), bad, first column of M
+// found[row][part] = M, Z, sum (M - x) exp(-d) / temperature (against the part's own M), bad, first column of M.  In 32 bits bound
+// by memory (2048 x 32003 bf16, masks: 31 us for 139 MB, 4.4 TB/s), in 64, for sampling, by instructions (1024 x 32003 bf16 with
+// its join 49 us for 66 MB) or, with few rows, latency (16 x 131072 f16, all controls: 9.0 us).
 template <int CHUNKS, bool FIRST, typename X, typename W>
 __global__ __launch_bounds__(HEAD_THREADS) void mg_head_parts_kernel(HeadArgs a, double* __restrict__ found) {
   constexpr bool ADJUST = std::is_same<X, double>::value;
+  __shared__ unsigned counts[ADJUST ? CHUNKS * HEAD_CHUNK : 1];
   __shared__ HeadRed red;
   const long row = (long)blockIdx.z * gridDim.y + blockIdx.y;
   if (row >= a.rows) return;
-  HEAD_PART_COUNTS()
+  const long part0 = (long)blockIdx.x * (CHUNKS * HEAD_CHUNK);
+  const int part_n = (int)min((long)CHUNKS * HEAD_CHUNK, a.width - part0);
+  if (ADJUST && a.history) head_count_columns(a, row, counts, part0, part_n);
   const HeadRow r = head_row(a, row);
   const HeadScale<W> scale(r);
   HeadPart<CHUNKS, HEAD_THREADS, X, W> h;
@@ -1156,14 +1164,14 @@ __device__ __forceinline__ HeadJoined head_join(const double* f, int parts, cons
   return j;
 }
 
-// THREADS * 8 columns are a whole part
-template <int THREADS, typename X>
-__global__ __launch_bounds__(THREADS) void mg_sample_join_kernel(HeadArgs a, int parts, const double* __restrict__ found,
+// The part in which the running sum passes the target is looked at once more for the token (16 x 131072 f16, all controls: 7.2 us,
+// three memory latencies and the count of the history).
+template <typename X>
+__global__ __launch_bounds__(HEAD_THREADS) void mg_sample_join_kernel(HeadArgs a, int parts, const double* __restrict__ found,
                                                                 const float* __restrict__ uniforms, int* __restrict__ actions,
                                                                 float* __restrict__ log_prob, float* __restrict__ entropy) {
-  constexpr int PART = THREADS * 8;
   constexpr bool adjust = std::is_same<X, double>::value;
-  __shared__ unsigned counts[adjust ? PART : 1];
+  __shared__ unsigned counts[adjust ? HEAD_CHUNK : 1];
   __shared__ double red[16];
   const long row = head_block();
   if (row >= a.rows) return;
@@ -1202,8 +1210,8 @@ __global__ __launch_bounds__(THREADS) void mg_sample_join_kernel(HeadArgs a, int
       v0 = head_group_min(best, 64);
     } else {
       part = part >= 0 ? part : last;
-      const long part0 = (long)part * PART;
-      const int part_n = (int)min((long)PART, a.width - part0);
+      const long part0 = (long)part * HEAD_CHUNK;
+      const int part_n = (int)min((long)HEAD_CHUNK, a.width - part0);
       if (adjust && a.history) head_count_columns(a, row, counts, part0, part_n);
       const int at = threadIdx.x * 8, n = part_n - at;
       X x[8];
@@ -1220,7 +1228,7 @@ __global__ __launch_bounds__(THREADS) void mg_sample_join_kernel(HeadArgs a, int
       const double here = head_scan(mine, 0.0, [](double p, double q) { return p + q; });
       if (head_lane() == 63) red[threadIdx.x >> 6] = here;
       __syncthreads();
-      const HeadSpot spot = head_spot(red, THREADS / 64, start, target);
+      const HeadSpot spot = head_spot(red, HEAD_THREADS / 64, start, target);
       picks = false;
       if (spot.entry == (int)threadIdx.x >> 6) {
         double before;
@@ -1234,7 +1242,7 @@ __global__ __launch_bounds__(THREADS) void mg_sample_join_kernel(HeadArgs a, int
   if (picks) head_sampled(row, j.bad, j.empty, v0 + pick.e, pick.t, j.z, j.s, scale, actions, log_prob, entropy);
 }
 
-// one wave per row
+// One wave per row (2048 x 32003: 4.8 us, two memory latencies).
 __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_join_kernel(HeadArgs a, int parts, const double* __restrict__ found,
                                                                        const int* __restrict__ actions, float* __restrict__ log_prob,
                                                                        float* __restrict__ entropy, double* __restrict__ stats) {
@@ -1267,6 +1275,8 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_join_kernel(HeadArgs
   }
 }
 
+// From the forward pass's stats, so that every block works alone.  Bound by memory: 2048 x 32003 bf16, masks: 47 us for 270 MB, 5.7
+// TB/s (part of it still in the caches).
 template <int CHUNKS, typename X>
 __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_wide_backward_kernel(HeadArgs a, const int* __restrict__ actions,
                                                                                 const float* __restrict__ entropy,
@@ -1274,10 +1284,12 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_wide_backward_kernel
                                                                                 const float* __restrict__ dlog_prob,
                                                                                 const float* __restrict__ dentropy,
                                                                                 void* __restrict__ dlogits) {
-  constexpr bool ADJUST = std::is_same<X, double>::value;
-  const long row = (long)blockIdx.z * gridDim.y + blockIdx.y;
+  constexpr bool adjust = std::is_same<X, double>::value;
+  __shared__ unsigned counts[adjust ? CHUNKS * HEAD_CHUNK : 1];
+  const long row = (long)blockIdx.z * gridDim.y + blockIdx.y, part0 = (long)blockIdx.x * (CHUNKS * HEAD_CHUNK);
   if (row >= a.rows) return;
-  HEAD_PART_COUNTS()
+  const int part_n = (int)min((long)CHUNKS * HEAD_CHUNK, a.width - part0);
+  if (adjust && a.history) head_count_columns(a, row, counts, part0, part_n);
   const HeadRow r = head_row(a, row);
   const HeadScale<float> scale(r);
   const double m = stats[2 * row];
@@ -1288,14 +1300,13 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_wide_backward_kernel
   float gp = 0;
   const float gh = (dentropy ? dentropy[row] : 0.f) * scale.inv_temp;
   if (dlog_prob && head_left(a, r, row, act)) gp = dlog_prob[row] * scale.inv_temp;
-  constexpr bool adjust = ADJUST;
+  constexpr int THREADS [[maybe_unused]] = HEAD_THREADS;
   HeadRaw<8> raw[CHUNKS];
   HEAD_PART_FETCH((raw[c].template fetch<FULL, adjust>(r, a.logits, a.type, row * a.logits_row + part0 + at, (int)(part0 + at), n)))
 #pragma unroll
   for (int c = 0; c < CHUNKS; c++) {
-    const int at = c * HEAD_CHUNK + threadIdx.x * 8, n = part_n - at;
+    const int at = c * HEAD_CHUNK + threadIdx.x * 8, n = part_n - at, v0 = (int)(part0 + at);
     if (n <= 0) continue;
-    const int v0 = (int)(part0 + at);
     X x[8];
     float g[8], slope[8], y[8];
     const unsigned ok = raw[c].template columns<false, true, adjust>(r, a.type, v0, n, counts + at, x, slope);
@@ -1348,16 +1359,16 @@ static HeadArgs head_args(const mg_logits* a) {
   return g;
 }
 
-// A part is four chunks where the row has more than two and that leaves enough blocks to fill the GPU, else one.
-static int head_chunks(const mg_logits* a) {
-  return a->width > 2 * HEAD_CHUNK && (int64_t)((a->width - 1) / (4 * HEAD_CHUNK) + 1) * a->rows >= 2048 ? 4 : 1;
-}
-static int head_parts(const mg_logits* a) { return (a->width - 1) / (head_chunks(a) * HEAD_CHUNK) + 1; }
+// A part is a chunk, which is as fast as larger parts or faster (sampling 2048 x 8193 bf16: 38 us, with four chunks 86;
+// adjustment 4096 x 8192: 25 and 28), but for the evaluation of large batches: 2048 x 32003 takes 31 + 47 us in parts of four
+// chunks and 46 + 56 in single ones (64 x 50001: 8.9 and 8.2; 2048 x 8193, of whose parts half would be nearly empty: 22 and 19).
+static int head_chunks(const mg_logits* a) { return a->width > 2 * HEAD_ROW && a->rows * (a->width / HEAD_ROW) >= 2048 ? 4 : 1; }
+static int head_parts(const mg_logits* a, int chunks = 1) { return (a->width - 1) / (chunks * HEAD_CHUNK) + 1; }
 // A block does one row (or, of narrow ones, as many as its lanes hold) and no loop over them: the compiler would keep what does
 // not change from row to row in registers, the constants of a rare path too.
-static dim3 head_wide_grid(const mg_logits* a) {
+static dim3 head_wide_grid(const mg_logits* a, int chunks = 1) {
   const int64_t y = a->rows < 32768 ? a->rows : 32768;
-  return dim3(head_parts(a), (unsigned)y, (unsigned)((a->rows + y - 1) / y));
+  return dim3(head_parts(a, chunks), (unsigned)y, (unsigned)((a->rows + y - 1) / y));
 }
 static dim3 head_grid(int64_t blocks) {
   const int64_t x = blocks < 1 << 20 ? blocks : 1 << 20;
@@ -1392,8 +1403,8 @@ static void head_by_width(const mg_logits* a, F f) {
   }
   f(head_int<8>(), head_bool<false>(), head_layout(a, 8, true));
 }
-// how a block holds a row: chunks of eight columns per thread, and threads.  Rather more chunks than more threads to wait for
-// (evaluation of 4096 x 8192 bf16: 33 us with 256 threads, 56 with 1024).
+// How a block holds a row: chunks of eight columns per thread, and threads.  Rather more chunks than more threads to wait for
+// (evaluation of 4096 x 8192 bf16, before other changes: 33 us with 256 threads, 56 with 1024).
 template <typename F>
 static void head_by_row(const mg_logits* a, F f) {
   if (a->width <= HEAD_CHUNK / 2) f(head_int<1>(), head_int<HEAD_THREADS / 2>());
@@ -1434,9 +1445,7 @@ static int head_adjust(const char* who, const mg_logits* a, void* out, const voi
     const HeadNarrow g = head_layout(a, 8, false);
     hipLaunchKernelGGL(mg_adjust_narrow_kernel<8>, head_grid((a->rows + g.rows - 1) / g.rows), dim3(HEAD_THREADS), 0, s, head_args(a), g, out, dout, dlogits);
   } else {
-    head_by_chunks(a, [&](auto c) {
-      hipLaunchKernelGGL(mg_adjust_wide_kernel<decltype(c)::value>, head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), out, dout, dlogits);
-    });
+    hipLaunchKernelGGL(mg_adjust_wide_kernel, head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), out, dout, dlogits);
   }
   return head_launched(who);
 }
@@ -1480,15 +1489,12 @@ extern "C" int mg_sample_actions(const mg_logits* a, const float* uniforms, int3
                            head_args(a), uniforms, actions, log_prob, entropy);
       });
     } else {
-      head_by_chunks(a, [&](auto c) {
-        constexpr int C = decltype(c)::value;
-        if (uniforms)
-          hipLaunchKernelGGL((mg_head_parts_kernel<C, false, X, double>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), (double*)a->workspace);
-        else
-          hipLaunchKernelGGL((mg_head_parts_kernel<C, true, X, double>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), (double*)a->workspace);
-        hipLaunchKernelGGL((mg_sample_join_kernel<C * HEAD_THREADS, X>), head_grid(a->rows), dim3(C * HEAD_THREADS), 0, s, head_args(a),
-                           head_parts(a), (const double*)a->workspace, uniforms, actions, log_prob, entropy);
-      });
+      if (uniforms)
+        hipLaunchKernelGGL((mg_head_parts_kernel<1, false, X, double>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), (double*)a->workspace);
+      else
+        hipLaunchKernelGGL((mg_head_parts_kernel<1, true, X, double>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), (double*)a->workspace);
+      hipLaunchKernelGGL(mg_sample_join_kernel<X>, head_grid(a->rows), dim3(HEAD_THREADS), 0, s, head_args(a), head_parts(a),
+                         (const double*)a->workspace, uniforms, actions, log_prob, entropy);
     }
   });
   return head_launched(who);
@@ -1518,12 +1524,13 @@ extern "C" int mg_evaluate_actions(const mg_logits* a, const int32_t* actions, f
       });
     } else {
       head_by_chunks(a, [&](auto c) {
-        hipLaunchKernelGGL((mg_head_parts_kernel<decltype(c)::value, false, X, float>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), (double*)a->workspace);
+        constexpr int C = decltype(c)::value;
+        hipLaunchKernelGGL((mg_head_parts_kernel<C, false, X, float>), head_wide_grid(a, C), dim3(HEAD_THREADS), 0, s, head_args(a), (double*)a->workspace);
       });
     }
   });
   if (head_wide(a))
-    hipLaunchKernelGGL(mg_evaluate_join_kernel, dim3((unsigned)((a->rows + 3) / 4)), dim3(HEAD_THREADS), 0, s, head_args(a), head_parts(a),
+    hipLaunchKernelGGL(mg_evaluate_join_kernel, dim3((unsigned)((a->rows + 3) / 4)), dim3(HEAD_THREADS), 0, s, head_args(a), head_parts(a, head_chunks(a)),
                        (const double*)a->workspace, actions, log_prob, entropy, stats);
   return head_launched(who);
 } catch (...) {
@@ -1550,8 +1557,9 @@ extern "C" int mg_evaluate_actions_backward(const mg_logits* a, const int32_t* a
                          dlog_prob, dentropy, dlogits);
     else
       head_by_chunks(a, [&](auto c) {
-        hipLaunchKernelGGL((mg_evaluate_wide_backward_kernel<decltype(c)::value, X>), head_wide_grid(a), dim3(HEAD_THREADS), 0, s, head_args(a), actions,
-                           entropy, stats, dlog_prob, dentropy, dlogits);
+        constexpr int C = decltype(c)::value;
+        hipLaunchKernelGGL((mg_evaluate_wide_backward_kernel<C, X>), head_wide_grid(a, C), dim3(HEAD_THREADS), 0, s, head_args(a), actions, entropy,
+                           stats, dlog_prob, dentropy, dlogits);
       });
   });
   return head_launched(who);

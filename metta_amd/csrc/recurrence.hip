@@ -133,6 +133,8 @@ struct RecPlace {
 __device__ __forceinline__ int rec_wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 // ---- many columns: a thread walks through all of time, the next REC_L steps on their way while it computes ------------
+// Bound by memory: x and gate in, h and a 32nd of it in marks out.  8192 x 256 x 128 bf16: 380 us for 1.67 GB, 4.4 TB/s,
+// where a copy of gigabytes reaches 4.8.
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void mg_recurrence_kernel(RecArgs a, T* __restrict__ h, float* __restrict__ last,
                                                             float* __restrict__ marks) {
@@ -197,7 +199,8 @@ __global__ __launch_bounds__(256) void mg_recurrence_kernel(RecArgs a, T* __rest
   for (int j = 0; j < VEC; j++) last[flat + j] = s[j];
 }
 
-// one step, no marks: a flat pass over the columns
+// One step, no marks: a flat pass over the columns.  98304 x 128 bf16: 27 us for 176 MB, 6.5 TB/s (part of it stays in the
+// caches); 24 x 128 f32: 2.6 us, the time of a launch.
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void mg_recurrence_step_kernel(RecArgs a, T* __restrict__ h, float* last) {
   if (blockIdx.x * 256 + threadIdx.x >= a.groups) return;  // (the state may be overwritten in place)
@@ -220,6 +223,8 @@ __global__ __launch_bounds__(256) void mg_recurrence_step_kernel(RecArgs a, T* _
   if (h) *(rec_vec<T, VEC>*)(h + flat) = o;
 }
 
+// The walk back: a stretch's states are made again from its mark, its gradients go out in time's reverse order.  Bound by memory:
+// x, gate and dh in, their gradients out.  8192 x 256 x 128 bf16: 600 us for 2.75 GB, 4.6 TB/s.
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void mg_recurrence_backward_kernel(RecArgs a, RecMarks m, RecGrads d) {
   const RecPlace<VEC> at(a, blockIdx.x * 256 + threadIdx.x);
@@ -327,7 +332,8 @@ __device__ __forceinline__ void rec_join(const RecArgs& a, RecExchange<VEC>& ex,
   }
 }
 
-// the pair of one split of time: forwards s -> a s + w x, backwards v -> a (v + dh), 0 at a reset
+// The pair of one split of time: forwards s -> a s + w x, backwards v -> a (v + dh), 0 at a reset.  It reads what the tiles will
+// read again, which is what cutting time costs: 1 x 65536 x 128 f32: 14 us for 67 MB, 4.9 TB/s.
 template <typename T, int VEC, bool BACK>
 __global__ __launch_bounds__(64 * REC_W) void mg_recurrence_pairs_kernel(RecArgs a, RecGrads d) {
   __shared__ RecExchange<VEC> ex;
@@ -387,6 +393,9 @@ __global__ __launch_bounds__(64 * REC_W) void mg_recurrence_pairs_kernel(RecArgs
   }
 }
 
+// Tile after tile: the waves' pairs meet in LDS, then each wave goes on from the state that enters it.  Bound by memory where
+// there are enough blocks (1 x 65536 x 128 f32 in 512 of them: 21 us for 101 MB, 4.7 TB/s), else by the way through a tile
+// (250 x 129 x 100 f16, two tiles: 14 us for 19 MB).
 template <typename T, int VEC>
 __global__ __launch_bounds__(64 * REC_W) void mg_recurrence_tile_kernel(RecArgs a, T* __restrict__ h, float* __restrict__ last,
                                                                         float* __restrict__ marks) {
@@ -473,6 +482,7 @@ __global__ __launch_bounds__(64 * REC_W) void mg_recurrence_tile_kernel(RecArgs 
   }
 }
 
+// The same from the last tile to the first (1 x 65536 x 128 f32: 37 us for 169 MB, 4.6 TB/s; 250 x 129 x 100 f16: 18 us).
 template <typename T, int VEC>
 __global__ __launch_bounds__(64 * REC_W) void mg_recurrence_tile_backward_kernel(RecArgs a, RecMarks m, RecGrads d) {
   __shared__ RecExchange<VEC> ex;

@@ -304,9 +304,10 @@ def test_evaluate(shape, dtype):
 
 
 @pytest.mark.gpu
-def test_many_wide_rows():
-    """Enough rows beyond 8192 tokens that a block takes four times as many columns of each."""
-    n, v = 1030, 8300
+@pytest.mark.parametrize("v", [8300, 16500])
+def test_many_wide_rows(v):
+    """Rows beyond 8192 tokens that fill the GPU; beyond 16384 a block takes four times as many columns of each."""
+    n = 1030
     logits, c, u = _case(n, v, torch.bfloat16, seed=7, length=40, scale=3.0)
     l, slope = _adjusted(logits, **c)
     dev = _cuda(c)

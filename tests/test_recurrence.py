@@ -464,3 +464,45 @@ def test_overlapping_states_are_refused():
         with pytest.raises(RuntimeError, match="overlap"):
             gated_recurrence_step(x, x, flat[8:24].view(2, 8), out_state=flat[at : at + 16].view(2, 8))
     gated_recurrence_step(x, x, flat[8:24].view(2, 8), out_state=flat[24:40].view(2, 8))
+
+
+@pytest.mark.gpu
+def test_in_place_states_are_noticed_and_inference_mode():
+    x = torch.randn(3, 8, device="cuda")
+    state = torch.zeros(3, 8, device="cuda")
+    w = torch.ones(3, 8, device="cuda", requires_grad=True)
+    product = (w * state).sum()  # keeps the state for its gradient
+    gated_recurrence_step(x, x, state, out_state=state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.backward()
+    want, _ = gated_recurrence_step(x, x, torch.zeros(3, 8, device="cuda"))
+    with torch.inference_mode():
+        state = torch.zeros(3, 8, device="cuda")
+        h, s = gated_recurrence_step(x, x, state, out_state=state)
+        y, last = gated_recurrence(x[:, None], x[:, None])
+        assert s is state and torch.equal(h, want) and torch.equal(y[:, 0], want) and torch.equal(last, want)
+
+
+@pytest.mark.gpu
+def test_from_several_threads():
+    """Calls on streams of their own, forwards and backwards, from threads at the same time."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    inputs = [[t.cuda() for t in _inputs(3, 70 + 300 * k, 32, torch.bfloat16, seed=k)] for k in range(4)]
+
+    def work(k):
+        x, gate, state, resets, dh, dlast = inputs[k]
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(5):
+                leaves = [t.clone().requires_grad_() for t in (x, gate, state)]
+                h, last = gated_recurrence(*leaves, resets)
+                out = [h.detach(), last.detach(), *torch.autograd.grad([h, last], leaves, [dh, dlast])]
+            s.synchronize()
+        return out
+
+    torch.cuda.synchronize()
+    want = [work(k) for k in range(4)]
+    with ThreadPoolExecutor(4) as pool:
+        for a, b in zip(pool.map(work, range(4)), want):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
