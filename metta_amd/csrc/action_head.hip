@@ -754,15 +754,24 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_backward_kern
 // ---- wide rows --------------------------------------------------------------------------------------------------------
 // Thread t of a block holds columns 8 t ... 8 t + 7 of each of its part's chunks.
 
-// counts of the n columns from v0 on, all threads together; barriers inside
+// counts of the n columns from v0 on, all threads together, four entries each on their way at a time; barriers inside
 __device__ __forceinline__ void head_count_columns(const HeadArgs& a, long row, unsigned* counts, long v0, int n) {
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += blockDim.x) counts[i] = 0;
   __syncthreads();
   const int* h = a.history + row * a.history_row;
-  for (int i = threadIdx.x; i < a.history_len; i += blockDim.x) {
-    const long v = (long)h[i] - v0;
-    if (h[i] >= 0 && v >= 0 && v < n) atomicAdd(&counts[v], 1u);
+  for (long i0 = threadIdx.x; i0 < a.history_len; i0 += 4L * blockDim.x) {
+    int v[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const long i = i0 + u * (long)blockDim.x;
+      v[u] = i < a.history_len ? h[i] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const long at = v[u] - v0;
+      if (v[u] >= 0 && at >= 0 && at < n) atomicAdd(&counts[at], 1u);
+    }
   }
   __syncthreads();
 }

@@ -89,7 +89,7 @@ def reset_state(policy, state, done: torch.Tensor):
 class ActionControls:
     """Controls of the action head (`allowed`, `bias`, `temperature`, `repetition`, `presence`, `frequency`; see
     metta_amd/action_head.py) for a rollout, and the recent actions that the penalties look at: the last `history_length`
-    of every agent, forgotten when its episode ends."""
+    of every agent, forgotten when its episode ends (an environment that is started anew wants new controls)."""
 
     def __init__(self, history_length: int = 0, **controls):
         if "history" in controls:
