@@ -866,11 +866,11 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_adjust_wide_kernel(HeadArgs a
   const long row = (long)blockIdx.z * gridDim.y + blockIdx.y, part0 = (long)blockIdx.x * HEAD_CHUNK;
   if (row >= a.rows) return;
   const int part_n = (int)min((long)HEAD_CHUNK, a.width - part0), at = threadIdx.x * 8, n = part_n - at, v0 = (int)(part0 + at);
-  if (a.history) head_count_columns(a, row, counts, part0, part_n);
   const HeadRow r = head_row(a, row);
   HeadAdjust<8> it;
   if (part_n == HEAD_CHUNK) it.fetch<true>(a, r, row, v0, 8, dout);
   else it.fetch<false>(a, r, row, v0, n, dout);
+  if (a.history) head_count_columns(a, row, counts, part0, part_n);
   if (n > 0) it.store(a, r, row, v0, n, counts + at, out, dout, dlogits);
 }
 
@@ -895,9 +895,10 @@ struct HeadPart {
   // RUN: red.z gets the sums of waves, chunk by chunk
   template <bool GRAD, bool RUN>
   __device__ __forceinline__ void hold(const HeadArgs& a, const HeadRow& r, const HeadScale<W>& scale, long row, long part0, int part_n,
-                                       const unsigned* counts, HeadRed& red) {
+                                       unsigned* counts, HeadRed& red) {
     HeadRaw<8> raw[CHUNKS];
     HEAD_PART_FETCH((raw[c].template fetch<FULL, adjust>(r, a.logits, a.type, row * a.logits_row + part0 + at, (int)(part0 + at), n)))
+    if (adjust && a.history) head_count_columns(a, row, counts, part0, part_n);  // (while the columns are on their way)
     m = -INFINITY;
 #pragma unroll
     for (int c = 0; c < CHUNKS; c++) {
@@ -1015,7 +1016,6 @@ __global__ __launch_bounds__(THREADS) void mg_sample_row_kernel(HeadArgs a, cons
   __shared__ HeadRed red;
   const long row = head_block();
   if (row >= a.rows) return;
-  if (adjust && a.history) head_count_columns(a, row, counts, 0, a.width);
   const HeadRow r = head_row(a, row);
   const HeadScale<float> scale(r);
   HeadPart<CHUNKS, THREADS, X, float> h;
@@ -1045,7 +1045,7 @@ __global__ __launch_bounds__(THREADS) void mg_sample_row_kernel(HeadArgs a, cons
     head_sample_again<CHUNKS, THREADS, X>(a, r, row, h.m, u, counts, red, actions, log_prob, entropy);
 }
 
-// 4096 x 8192 bf16: 20 us for 67 MB, 3.4 TB/s; 16384 x 1024: 13 us.
+// Bound by memory and by the two barriers of a row (4096 x 8192 bf16: 20 us for 67 MB, 3.4 TB/s; 16384 x 1024: 13 us for 34 MB).
 template <int CHUNKS, int THREADS, typename X>
 __global__ __launch_bounds__(THREADS) void mg_evaluate_row_kernel(HeadArgs a, const int* __restrict__ actions, float* __restrict__ log_prob,
                                                                  float* __restrict__ entropy, double* __restrict__ stats) {
@@ -1053,7 +1053,6 @@ __global__ __launch_bounds__(THREADS) void mg_evaluate_row_kernel(HeadArgs a, co
   __shared__ HeadRed red;
   const long row = head_block();
   if (row >= a.rows) return;
-  if (std::is_same<X, double>::value && a.history) head_count_columns(a, row, counts, 0, a.width);
   const HeadRow r = head_row(a, row);
   const HeadScale<float> scale(r);
   const int act = actions[row];
@@ -1085,7 +1084,7 @@ __device__ __forceinline__ bool head_left(const HeadArgs& a, const HeadRow& r, l
   return head_allowed(r, act) && l[0] > -INFINITY && (!r.bias || r.bias[act] > -INFINITY);
 }
 
-// For rows of up to MG_EVALUATE_STATS_WIDTH columns, whose sums are computed again (16384 x 1024 bf16: 20 us for 67 MB).
+// For rows of up to MG_EVALUATE_STATS_WIDTH columns, whose sums are computed again (16384 x 1024 bf16: 20 us for 67 MB, 3.4 TB/s).
 template <typename X>
 __global__ __launch_bounds__(HEAD_THREADS / 2) void mg_evaluate_row_backward_kernel(HeadArgs a, const int* __restrict__ actions,
                                                                                const float* __restrict__ dlog_prob,
@@ -1096,7 +1095,6 @@ __global__ __launch_bounds__(HEAD_THREADS / 2) void mg_evaluate_row_backward_ker
   __shared__ HeadRed red;
   const long row = head_block();
   if (row >= a.rows) return;
-  if (adjust && a.history) head_count_columns(a, row, counts, 0, a.width);
   const HeadRow r = head_row(a, row);
   const HeadScale<float> scale(r);
   const int act = actions[row];
@@ -1124,7 +1122,7 @@ __global__ __launch_bounds__(HEAD_THREADS / 2) void mg_evaluate_row_backward_ker
 
 // found[row][part] = M, Z, sum (M - x) exp(-d) / temperature (against the part's own M), bad, first column of M.  In 32 bits bound
 // by memory (2048 x 32003 bf16, masks: 31 us for 139 MB, 4.4 TB/s), in 64, for sampling, by instructions (1024 x 32003 bf16 with
-// its join 49 us for 66 MB) or, with few rows, latency (16 x 131072 f16, all controls: 9.0 us).
+// its join 49 us for 66 MB) or, with few rows, latency (16 x 131072 f16, all controls: 8.6 us).
 template <int CHUNKS, bool FIRST, typename X, typename W>
 __global__ __launch_bounds__(HEAD_THREADS) void mg_head_parts_kernel(HeadArgs a, double* __restrict__ found) {
   constexpr bool ADJUST = std::is_same<X, double>::value;
@@ -1134,7 +1132,6 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_head_parts_kernel(HeadArgs a,
   if (row >= a.rows) return;
   const long part0 = (long)blockIdx.x * (CHUNKS * HEAD_CHUNK);
   const int part_n = (int)min((long)CHUNKS * HEAD_CHUNK, a.width - part0);
-  if (ADJUST && a.history) head_count_columns(a, row, counts, part0, part_n);
   const HeadRow r = head_row(a, row);
   const HeadScale<W> scale(r);
   HeadPart<CHUNKS, HEAD_THREADS, X, W> h;
@@ -1173,8 +1170,8 @@ __device__ __forceinline__ HeadJoined head_join(const double* f, int parts, cons
   return j;
 }
 
-// The part in which the running sum passes the target is looked at once more for the token (16 x 131072 f16, all controls: 7.2 us,
-// three memory latencies and the count of the history).
+// The part in which the running sum passes the target is looked at once more for the token (16 x 131072 f16, all controls: 6.6 us,
+// a chain of memory latencies and the count of the history).
 template <typename X>
 __global__ __launch_bounds__(HEAD_THREADS) void mg_sample_join_kernel(HeadArgs a, int parts, const double* __restrict__ found,
                                                                 const float* __restrict__ uniforms, int* __restrict__ actions,
@@ -1221,12 +1218,12 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_sample_join_kernel(HeadArgs a
       part = part >= 0 ? part : last;
       const long part0 = (long)part * HEAD_CHUNK;
       const int part_n = (int)min((long)HEAD_CHUNK, a.width - part0);
-      if (adjust && a.history) head_count_columns(a, row, counts, part0, part_n);
       const int at = threadIdx.x * 8, n = part_n - at;
       X x[8];
       double t[8], w[8], mine = 0.0;
       HeadRaw<8> raw;
       raw.template fetch<false, adjust>(r, a.logits, a.type, row * a.logits_row + part0 + at, (int)(part0 + at), n);
+      if (adjust && a.history) head_count_columns(a, row, counts, part0, part_n);
       raw.template columns<false, false, adjust>(r, a.type, (int)(part0 + at), n, counts + at, x, (float*)nullptr);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
@@ -1298,7 +1295,6 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_wide_backward_kernel
   const long row = (long)blockIdx.z * gridDim.y + blockIdx.y, part0 = (long)blockIdx.x * (CHUNKS * HEAD_CHUNK);
   if (row >= a.rows) return;
   const int part_n = (int)min((long)CHUNKS * HEAD_CHUNK, a.width - part0);
-  if (adjust && a.history) head_count_columns(a, row, counts, part0, part_n);
   const HeadRow r = head_row(a, row);
   const HeadScale<float> scale(r);
   const double m = stats[2 * row];
@@ -1312,6 +1308,7 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_wide_backward_kernel
   constexpr int THREADS [[maybe_unused]] = HEAD_THREADS;
   HeadRaw<8> raw[CHUNKS];
   HEAD_PART_FETCH((raw[c].template fetch<FULL, adjust>(r, a.logits, a.type, row * a.logits_row + part0 + at, (int)(part0 + at), n)))
+  if (adjust && a.history) head_count_columns(a, row, counts, part0, part_n);
 #pragma unroll
   for (int c = 0; c < CHUNKS; c++) {
     const int at = c * HEAD_CHUNK + threadIdx.x * 8, n = part_n - at, v0 = (int)(part0 + at);
