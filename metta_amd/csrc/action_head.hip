@@ -206,6 +206,7 @@ __device__ __forceinline__ void head_store(void* p, int type, long at, int n, co
 // the first is looked at waits for the memory once.  FULL: all E columns are in the row, for every lane.
 template <int E>
 struct HeadRaw {
+  static constexpr bool BORDER = 32 % E != 0 && E > 4;  // a group's mask bits may lie in two words (narrower groups start at column 0)
   unsigned logits[E], allowed[(E + 3) / 4];
   float bias[E];
 
@@ -222,7 +223,12 @@ struct HeadRaw {
     }
 #pragma unroll
     for (int e = 0; e < (E + 3) / 4; e++) allowed[e] = 0;
-    if (r.kind == MG_ALLOWED_BITS) allowed[0] = FULL || n > 0 ? ((const unsigned*)r.allowed)[v0 >> 5] : 0u;
+    if (r.kind == MG_ALLOWED_BITS) {
+      allowed[0] = FULL || n > 0 ? ((const unsigned*)r.allowed)[v0 >> 5] : 0u;
+      if constexpr (BORDER) {
+        if (!FULL && (v0 & 31) + min(n, E) > 32) allowed[1] = ((const unsigned*)r.allowed)[(v0 >> 5) + 1];
+      }
+    }
     if (r.kind == MG_ALLOWED_BOOL) bytes<FULL>((const unsigned char*)r.allowed + v0, n, allowed);
     if constexpr (BIAS) {
       unsigned b[E];
@@ -257,14 +263,20 @@ struct HeadRaw {
   }
   template <bool FULL>
   static __device__ __forceinline__ void bytes(const unsigned char* p, int n, unsigned* out) {
-    if ((FULL || n >= E) && E % 4 == 0) {
+    if (FULL || n >= E) {
       head_words<E / 4>(p, out);
+      if constexpr (E % 4 != 0) {
+        unsigned b = 0;
+#pragma unroll
+        for (int e = E / 4 * 4; e < E; e++) b |= (unsigned)p[e] << (8 * (e % 4));
+        out[E / 4] = b;
+      }
     } else {
 #pragma unroll
       for (int w = 0; w < (E + 3) / 4; w++) {
         unsigned b = 0;
 #pragma unroll
-        for (int e = 4 * w; e < E && e < 4 * w + 4; e++) b |= (FULL || e < n ? (unsigned)p[e] : 0u) << (8 * (e % 4));
+        for (int e = 4 * w; e < E && e < 4 * w + 4; e++) b |= (e < n ? (unsigned)p[e] : 0u) << (8 * (e % 4));
         out[w] = b;
       }
     }
@@ -287,7 +299,10 @@ struct HeadRaw {
   __device__ __forceinline__ unsigned bits(const HeadRow& r, int v0, int n) const {
     if (n <= 0) return 0;
     const unsigned inside = n >= E ? (1u << E) - 1 : (1u << n) - 1;
-    if (r.kind == MG_ALLOWED_BITS) return (allowed[0] >> (v0 & 31)) & inside;  // (E divides 32 and v0)
+    if (r.kind == MG_ALLOWED_BITS) {
+      if constexpr (BORDER) return (unsigned)(((unsigned long long)allowed[1] << 32 | allowed[0]) >> (v0 & 31)) & inside;
+      return (allowed[0] >> (v0 & 31)) & inside;
+    }
     if (r.kind != MG_ALLOWED_BOOL) return inside;
     unsigned b = 0;
 #pragma unroll
@@ -1407,7 +1422,16 @@ static void head_by_width(const mg_logits* a, F f) {
     case 7: return f(head_int<7>(), one, g);
     case 8: return f(head_int<8>(), one, g);
   }
-  f(head_int<8>(), head_bool<false>(), head_layout(a, 8, true));
+  // as few lanes as eight columns each allow, then as few columns as so many lanes allow (65536 x 157 bf16 in five columns each:
+  // sampling 21 us, evaluation 15 and its gradient 20; in eight, 20 lanes of 32: 27, 18 and 25)
+  const head_bool<false> several;
+  const HeadNarrow group = head_layout(a, 8, true);
+  switch ((a->width + group.lanes - 1) / group.lanes) {
+    case 5: return f(head_int<5>(), several, group);
+    case 6: return f(head_int<6>(), several, group);
+    case 7: return f(head_int<7>(), several, group);
+  }
+  f(head_int<8>(), several, group);
 }
 // How a block holds a row: chunks of eight columns per thread, and threads.  Rather more chunks than more threads to wait for
 // (evaluation of 4096 x 8192 bf16, before other changes: 33 us with 256 threads, 56 with 1024).

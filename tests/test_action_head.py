@@ -111,7 +111,8 @@ def _cuda(c):
 
 
 SHAPES = [(1, 1), (3, 2), (24, 5), (1000, 5), (65, 8), (11, 9), (33, 63), (17, 64), (9, 65), (40, 157), (5, 512), (7, 513), (7, 1000), (3, 1025), (3, 2049),
-          (3, 4097), (2, 8192), (2, 8193), (2, 20001), (1, 131072), (300, 33), (257, 3), (130, 6), (64, 7), (65, 4)]  # fmt: skip
+          (3, 4097), (2, 8192), (2, 8193), (2, 20001), (1, 131072), (300, 33), (257, 3), (130, 6), (64, 7), (65, 4), (70, 13),
+          (12, 100), (9, 180), (6, 430)]  # fmt: skip
 
 # ---- refusals ------------------------------------------------------------------------------------------------------
 
