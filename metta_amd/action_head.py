@@ -5,7 +5,8 @@
 * `evaluate_actions` -- the training form: log-probability and entropy of stored actions, with the gradient;
 * `pack_allowed` -- a boolean mask as bits, an eighth of its size.
 
-The first three are single HIP kernels on torch's current stream (metta_amd/csrc/action_head.hip); there is no CPU path.
+The first three are HIP kernels on torch's current stream (metta_amd/csrc/action_head.hip), one launch each (two for sampling
+and evaluation beyond 8192 tokens); there is no CPU path.
 They share these controls, all keyword arguments, for logits `[..., V]` of float32, bfloat16 or float16:
 
 * `allowed`: bool `[V]` or `[..., V]`, or int32 bits `[ceil(V / 32)]` or `[..., ceil(V / 32)]` (`pack_allowed`);
@@ -55,8 +56,8 @@ def adjust_logits(
     presence: float = 0.0,
     frequency: float = 0.0,
 ) -> Tensor:
-    """The adjusted logits (shape and type of `logits`, -infinity where masked), computed in 64 bits and rounded once.
-    Differentiable once in `logits`."""
+    """The adjusted logits (shape and type of `logits`, -infinity where masked), computed in 64 bits and rounded to 32 and
+    to their type.  Differentiable once in `logits`."""
     return native.operators().adjust_logits(logits, allowed, bias, history, temperature, repetition, presence, frequency)
 
 
@@ -76,7 +77,7 @@ def sample_actions(
 
     With `uniforms` (float32 in [0, 1), one per row, for instance `torch.rand`) the action is the first token at which the
     running sum of the probabilities exceeds the uniform, as 64-bit arithmetic finds it: the same numbers give the same
-    actions whatever the shape of the batch.  Without, it is the most likely token (the lowest of equals).  Carries no
+    actions whatever the shape of the batch (1 and more: the last token with any weight).  Without, it is the most likely token (the lowest of equals).  Carries no
     gradient; `evaluate_actions` does."""
     return native.operators().sample_actions(logits, uniforms, allowed, bias, history, temperature, repetition, presence, frequency)
 
