@@ -13,9 +13,9 @@
 //
 // Rows of up to HEAD_NARROW columns are held in registers, E adjacent columns per lane, by as many lanes as that takes
 // (one lane for five actions, a wave for five hundred); rows of up to HEAD_ROW columns by a block, in chunks of eight columns
-// per thread.  Their logits are read once.  Wider rows are cut into parts, a block each; what a part
-// found (maximum, sum, ...) goes to a workspace and a second launch joins the parts of a row.  A history is counted in LDS by
-// the block that needs it, for the columns that it holds.
+// per thread.  Their logits are read once.  Wider rows are cut into parts, a block each; what a part found (maximum, sum, ...)
+// goes to a workspace and a second launch joins the parts of a row.  A history is counted in LDS by the block that needs it,
+// for the columns that it holds.
 //
 // The logits are held in 64 bits where a bias or a penalty could cancel large ones, the differences from the largest and all
 // that follows in 32, which log-probabilities, entropies and gradients need no more than.  A sampled action is the one that
@@ -954,7 +954,7 @@ struct HeadPart {
       for (int c = 0; c < SUMS; c++) red.z[c * (THREADS / 64) + (threadIdx.x >> 6)] = here[c];
       red.s[threadIdx.x >> 6] = s;
     }
-    __syncthreads();  // (and nobody reads red.m any more, so that the next row may use it)
+    __syncthreads();
     z = (W)head_total(red.z, SUMS * (THREADS / 64));
     s = (W)head_total(red.s, THREADS / 64);
     s = scale.finish(s);
