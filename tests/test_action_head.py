@@ -689,3 +689,16 @@ def test_saved_tensors_are_watched_and_second_derivatives_refused():
         (d,) = torch.autograd.grad(out.sum(), x, create_graph=True)
         with pytest.raises(RuntimeError, match="differentiable once"):
             d.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,v", [(60000, 5), (20000, 64), (10000, 157), (3000, 1024), (400, 8000)])
+def test_many_rows_are_the_definitions(n, v):
+    """Enough rows that some targets come close to a border: the 32-bit sums do not decide those."""
+    g = torch.Generator().manual_seed(n)
+    logits = torch.randn(n, v, generator=g)
+    for kw in ({}, dict(bias=torch.randn(v, generator=g))):
+        u = torch.rand(n, generator=g)
+        a, _, _ = sample_actions(logits.cuda(), u.cuda(), temperature=0.8, **_cuda(kw))
+        want = _picked(_adjusted(logits, temperature=0.8, **kw)[0], _np(u))
+        assert np.array_equal(a.cpu().numpy(), want)
