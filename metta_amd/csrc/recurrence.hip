@@ -285,11 +285,13 @@ __global__ __launch_bounds__(256) void mg_recurrence_backward_kernel(RecArgs a, 
 // One lane per group of columns, one wave per REC_L steps.  LDS holds the pairs of the current tile's waves, twice, so
 // that one barrier per tile is enough.
 // A pair (p, q) stands for s -> p s + q.  p is never negative, so -0 marks a stretch with a reset in it: what stood before
-// it, NaN and infinity too, is gone (a product that underflowed to +0 does not hide them).
-__device__ __forceinline__ float rec_apply(float p, float q, float s) { return __float_as_int(p) < 0 ? q : fmaf(p, s, q); }
+// it, NaN and infinity too, is gone (a product that underflowed to +0 does not hide them).  The mark is told by all its bits:
+// a factor may be a NaN with its sign set, which is no reset.
+__device__ __forceinline__ bool rec_marked(float p) { return __float_as_uint(p) == 0x80000000u; }
+__device__ __forceinline__ float rec_apply(float p, float q, float s) { return rec_marked(p) ? q : fmaf(p, s, q); }
 __device__ __forceinline__ void rec_compose(float later_p, float later_q, float& p, float& q) {
   q = rec_apply(later_p, later_q, q);
-  p = __float_as_int(later_p) < 0 ? -0.f : p * later_p;
+  p = rec_marked(later_p) ? -0.f : p * later_p;
 }
 
 template <int VEC>
@@ -544,7 +546,7 @@ __global__ __launch_bounds__(64 * REC_W) void mg_recurrence_tile_backward_kernel
         for (int j = 0; j < VEC; j++) {
           const float cd = dh ? c[j] + (float)dt.v[i][j] : c[j];
           c[j] = rec_apply(ak[i][j], 0.f, cd);
-          p[j] = __float_as_int(ak[i][j]) < 0 ? -0.f : p[j] * ak[i][j];
+          p[j] = rec_marked(ak[i][j]) ? -0.f : p[j] * ak[i][j];
         }
       }
     }

@@ -506,3 +506,39 @@ def test_from_several_threads():
     with ThreadPoolExecutor(4) as pool:
         for a, b in zip(pool.map(work, range(4)), want):
             assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(2, 10, 8), (2, 10, 7), (2, 200, 8), (2, 200, 7), (2, 1000, 8), (1300, 40, 128)])
+def test_nan_gates(shape, dtype):
+    """A gate of NaN, whatever its sign, reaches every result that depends on it, up to the nearest reset and no further: walks,
+    tiles, and time cut over blocks."""
+    rows, steps, width = shape
+    x, gate, state, resets, dh, dlast = _inputs(*shape, dtype, seed=9, resets=3.0 / steps)
+    plus, minus, ints = {torch.float32: (0x7FC00000, -0x400000, torch.int32), torch.bfloat16: (0x7FC0, -0x40, torch.int16), torch.float16: (0x7E00, -0x200, torch.int16)}[dtype]
+    n, bits, rng = np.zeros(shape, dtype=bool), gate.view(ints).numpy(), np.random.default_rng(1)
+    for r in range(rows):
+        for c in range(width):
+            if (r + c) % 5 != 4:  # (the others have none)
+                t = rng.integers(steps)
+                bits[r, t, c], n[r, t, c] = minus if (r + c) % 2 else plus, True
+    resets[1] = False
+    z = resets.numpy()
+    h, d, before, after = (np.zeros(shape, dtype=bool) for _ in range(4))
+    s = np.zeros((rows, width), dtype=bool)
+    for t in range(steps):
+        before[:, t] = s & ~z[:, t, None]
+        s = before[:, t] | n[:, t]
+        h[:, t] = s
+    back = np.zeros((rows, width), dtype=bool)
+    for t in range(steps - 1, -1, -1):
+        after[:, t] = back
+        back = (back | n[:, t]) & ~z[:, t, None]
+    want = dict(h=h, last=s, dx=after | n, dgate=after | n | before, dstate=back)
+    xs, gs, ss = (t.cuda().requires_grad_() for t in (x, gate, state))
+    out = gated_recurrence(xs, gs, ss, resets.cuda())
+    got = [*out, *torch.autograd.grad(out, [xs, gs, ss], [dh.cuda(), dlast.cuda()])]
+    for (name, nan), t in zip(want.items(), got):
+        assert np.array_equal(torch.isnan(t).cpu().numpy(), nan), name
+        assert bool(torch.isfinite(t[~torch.from_numpy(nan).cuda()]).all()), name
