@@ -124,7 +124,20 @@ void check_core(const Tensor& x, const Tensor& gate, const Tensor& state, const 
   }
   require(width == 0 || rows <= (int64_t(1) << 31) / width, "rows * width must not exceed 2^31");
   for (const Tensor* t : {&gate, &state, &resets}) require(!t->defined() || t->device() == x.device(), "All tensors must be on same device");
-  require(x.is_cuda(), "All tensors must be on GPU");
+}
+void check_device(const Tensor& x) { require(x.is_cuda(), "All tensors must be on GPU"); }
+
+// Whether a contiguous `out` of [rows, width] lies over what a step reads of `t` ([rows, width] from column `from` on), otherwise than
+// element on element: a thread would write what another has yet to read.  (A t that is copied before the launch is no matter.)
+bool written_over(const Tensor& out, const Tensor& t, int64_t from, int64_t width) {
+  if (!out.numel() || !t.numel() || (t.stride(-1) != 1 && t.size(-1) != 1)) return false;
+  const int64_t size = t.element_size(), rows = out.size(0), row = t.stride(0) * size, wide = width * size, bytes = out.numel() * out.element_size();
+  // bytes from out's first to t's
+  const int64_t at = reinterpret_cast<intptr_t>(t.data_ptr()) + from * size - reinterpret_cast<intptr_t>(out.data_ptr());
+  if (at == 0 && size == out.element_size() && (rows == 1 || row == wide)) return false;
+  // the first of t's rows that ends behind out's beginning: does it begin before out's end?
+  const int64_t first = at + wide > 0 ? 0 : row ? -(at + wide) / row + 1 : rows;
+  return first < rows && at + first * row < bytes;
 }
 
 // memory of this call's own (torch's allocator keeps it for the stream, and for a captured graph)
@@ -197,6 +210,7 @@ struct Recurrence : torch::autograd::Function<Recurrence> {
 std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& x_, const Maybe& gate_, const Maybe& state_, const Maybe& resets_) {
   Tensor gate = or_none(gate_), state = or_none(state_);
   check_core(x_, gate, state, or_none(resets_), 3);
+  check_device(x_);
   const Core given(x_, gate);
   if (state.defined()) state = state.contiguous();
   if (x_.numel() == 0) {  // nothing to compute; part of the graph all the same
@@ -228,7 +242,12 @@ std::tuple<Tensor, Tensor> gated_recurrence_step(const Tensor& x, const Maybe& g
     require(!grad || !out.requires_grad(), "out_state is written in place and must not require a gradient");
     const int64_t apart = std::abs(static_cast<const char*>(out.data_ptr()) - static_cast<const char*>(state.data_ptr()));
     require(apart == 0 || apart >= 4 * state.numel(), "out_state may be state itself, but not overlap it otherwise");
+    const int64_t width = out.size(1);
+    require(!written_over(out, x, 0, width) && !written_over(out, gate.defined() ? gate : x, gate.defined() ? 0 : width, width) &&
+                !(resets.defined() && resets.is_contiguous() && written_over(out, resets.unsqueeze(-1), 0, 1)),
+            "out_state may not overlap x, gate or resets other than element on element");
   }
+  check_device(x);
   const at::AutoDispatchBelowADInplaceOrView below;
   if (!out.defined()) out = empty(state.sizes(), x, at::kFloat);
   const Tensor h = x.scalar_type() == at::kFloat ? out : empty(state.sizes(), x, x.scalar_type());

@@ -35,5 +35,6 @@ def gated_recurrence_step(x: Tensor, gate: Optional[Tensor], state: Tensor, rese
     `[rows]` -> (h of x's type, new state float32).  For float32 inputs h IS the new state.
 
     `out_state` (contiguous float32 `[rows, width]`) receives the new state; it may be `state` itself, for a state that
-    stays where it is.  Not differentiable: a call that would need gradients is refused."""
+    stays where it is, or a float32 `x` or `gate`, element on element.  Any other overlap with what the call reads is
+    refused.  Not differentiable: a call that would need gradients is refused."""
     return native.operators().gated_recurrence_step(x, gate, state, resets, out_state)

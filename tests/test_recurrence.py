@@ -542,3 +542,52 @@ def test_nan_gates(shape, dtype):
     for (name, nan), t in zip(want.items(), got):
         assert np.array_equal(torch.isnan(t).cpu().numpy(), nan), name
         assert bool(torch.isfinite(t[~torch.from_numpy(nan).cuda()]).all()), name
+
+
+def _views(flat):
+    """(what, x, gate, state, resets, out_state) that share memory otherwise than element on element."""
+    v = lambda at, *shape: flat[at : at + int(np.prod(shape))].view(*shape)  # noqa: E731
+    x, s = v(200, 3, 8), v(300, 3, 8)
+    yield "packed projection", v(0, 3, 16), None, s, None, v(0, 3, 8)
+    yield "end of a packed projection", v(0, 3, 16), None, s, None, v(40, 3, 8)
+    yield "shifted x", v(0, 3, 8), x, s, None, v(4, 3, 8)
+    yield "shifted gate", x, v(4, 3, 8), s, None, v(0, 3, 8)
+    yield "one element of x", v(23, 3, 8), x, s, None, v(0, 3, 8)
+    yield "rows further apart", v(0, 3, 16)[:, :8], x, s, None, v(0, 3, 8)
+    yield "a row for all", v(0, 1, 8).expand(3, 8), x, s, None, v(0, 3, 8)
+    yield "resets", x, x, s, v(0, 3, 8).view(torch.uint8).flatten()[:3], v(0, 3, 8)
+    yield "16 bits", v(0, 3, 8).view(torch.bfloat16)[:, :8], v(200, 3, 8).view(torch.bfloat16)[:, :8], s, None, v(0, 3, 8)
+
+
+def test_states_written_over_inputs_are_refused():
+    """One thread would write what another has yet to read."""
+    for what, x, gate, state, resets, out in _views(torch.zeros(400)):
+        with pytest.raises(RuntimeError, match="out_state may not overlap"):
+            gated_recurrence_step(x, gate, state, resets, out_state=out)
+    flat = torch.zeros(400)
+    a, b, s = flat[:24].view(3, 8), flat[24:48].view(3, 8), torch.zeros(3, 8)
+    fine = [
+        (a, b, s, b),  # element on element
+        (a, b, s, a),
+        (flat[100:260].view(2, 80)[:, :8], b[:2], s[:2], flat[120:136].view(2, 8)),  # between two rows
+        (a[:1], b[:1], s[:1], flat[8:16].view(1, 8)),  # side by side
+        (flat[:16].view(1, 16), None, s[:1], flat[:8].view(1, 8)),  # one row: candidate on candidate
+    ]
+    for x, gate, state, out in fine:
+        with pytest.raises(RuntimeError, match="on GPU"):
+            gated_recurrence_step(x, gate, state, out_state=out)
+
+
+@pytest.mark.gpu
+def test_states_written_element_on_element():
+    x, gate, state, resets, _, _ = (t.cuda() for t in _inputs(500, 1, 64, torch.float32, seed=4, resets=0.2))
+    x, gate, resets = x[:, 0].contiguous(), gate[:, 0].contiguous(), resets[:, 0].contiguous()
+    want = gated_recurrence_step(x, gate, state, resets)[1]
+    for k in range(2):
+        both = [x.clone(), gate.clone()]
+        h, s = gated_recurrence_step(*both, state, resets, out_state=both[k])
+        assert s is both[k] and torch.equal(s, want)
+    apart = torch.zeros(64, 500, device="cuda").t()  # columns that are not adjacent: copied before the launch
+    apart.copy_(x)
+    memory = torch.as_strided(apart, (500, 64), (64, 1))
+    assert torch.equal(gated_recurrence_step(apart, gate, state, resets, out_state=memory)[1], want)
