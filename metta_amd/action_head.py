@@ -57,7 +57,7 @@ def adjust_logits(
     frequency: float = 0.0,
 ) -> Tensor:
     """The adjusted logits (shape and type of `logits`, -infinity where masked), computed in 64 bits and rounded to 32 and
-    to their type.  Differentiable once in `logits`."""
+    to their type.  Differentiable once, in reverse mode, in `logits`."""
     return native.operators().adjust_logits(logits, allowed, bias, history, temperature, repetition, presence, frequency)
 
 
@@ -95,6 +95,6 @@ def evaluate_actions(
     frequency: float = 0.0,
 ) -> Tuple[Tensor, Tensor]:
     """(log-probabilities, entropies), float32, of `actions` (int32 or int64, logits' shape without its last dimension)
-    under the adjusted logits.  Differentiable once in `logits`.  An action that is masked or outside [0, V) has
+    under the adjusted logits.  Differentiable once, in reverse mode, in `logits`.  An action that is masked or outside [0, V) has
     log-probability -infinity and passes no gradient of it."""
     return native.operators().evaluate_actions(logits, actions, allowed, bias, history, temperature, repetition, presence, frequency)

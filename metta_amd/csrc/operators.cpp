@@ -9,6 +9,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
@@ -70,7 +71,15 @@ Tensor contiguous(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
 // columns next to each other
 Tensor adjacent(const Tensor& t) { return !t.defined() || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
+// whether t is a dual tensor whose tangent a forward-mode derivative would go on with
+bool dual(const Tensor& t) { return t.defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined(); }
 Tensor empty(at::IntArrayRef shape, const Tensor& like, at::ScalarType type) { return at::empty(shape, like.options().dtype(type).requires_grad(false)); }
+
+// A call without requires_grad goes past autograd, which would refuse the tangent of a dual tensor: it is refused, not dropped.
+void reverse_only(const char* who, std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    if (dual(*t)) fail(std::string(who) + " has no forward-mode derivative");
+}
 
 // A backward pass of kernels has no graph of its own: a second derivative through its results is an error, not a wrong number.
 void once(variable_list& grads, const char* who) {
@@ -210,6 +219,7 @@ struct Recurrence : torch::autograd::Function<Recurrence> {
 std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& x_, const Maybe& gate_, const Maybe& state_, const Maybe& resets_) {
   Tensor gate = or_none(gate_), state = or_none(state_);
   check_core(x_, gate, state, or_none(resets_), 3);
+  reverse_only("gated_recurrence", {&x_, &gate, &state});
   check_device(x_);
   const Core given(x_, gate);
   if (state.defined()) state = state.contiguous();
@@ -232,6 +242,7 @@ std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& x_, const Maybe& gate_
 std::tuple<Tensor, Tensor> gated_recurrence_step(const Tensor& x, const Maybe& gate_, const Tensor& state, const Maybe& resets_, const Maybe& out_) {
   const Tensor gate = or_none(gate_), resets = or_none(resets_);
   check_core(x, gate, state, resets, 2);
+  reverse_only("gated_recurrence_step", {&x, &gate, &state});
   const bool grad = at::GradMode::is_enabled();
   require(!grad || !(wants(x) || wants(gate) || wants(state)),
           "gated_recurrence_step has no gradient: call it under torch.no_grad(), or use gated_recurrence");
@@ -240,6 +251,7 @@ std::tuple<Tensor, Tensor> gated_recurrence_step(const Tensor& x, const Maybe& g
     require(out.sizes() == state.sizes() && out.scalar_type() == at::kFloat && out.device() == x.device() && out.is_contiguous(),
             "out_state must be contiguous float32 [rows, width] on x's device");
     require(!grad || !out.requires_grad(), "out_state is written in place and must not require a gradient");
+    require(!dual(out), "out_state is written in place and must not carry a tangent");
     const int64_t apart = std::abs(static_cast<const char*>(out.data_ptr()) - static_cast<const char*>(state.data_ptr()));
     require(apart == 0 || apart >= 4 * state.numel(), "out_state may be state itself, but not overlap it otherwise");
     const int64_t width = out.size(1);
@@ -300,6 +312,7 @@ struct Head {
     if (given_bias.defined()) {
       require(given_bias.scalar_type() == at::kFloat, "bias must be float32");
       require(!gradient || !given_bias.requires_grad() || !at::GradMode::is_enabled(), "bias is a constant: it must not require a gradient");
+      require(!gradient || !dual(given_bias), "bias is a constant: it must not carry a tangent");
     }
     const bool penalties = repetition != 1.0 || presence != 0.0 || frequency != 0.0;
     if (given_history.defined()) {
@@ -412,6 +425,7 @@ struct Adjust : torch::autograd::Function<Adjust> {
 
 Tensor adjust_logits(const Tensor& logits, const Maybe& allowed, const Maybe& bias, const Maybe& history, double temperature, double repetition,
                      double presence, double frequency) {
+  reverse_only("adjust_logits", {&logits});
   const Head h(logits, allowed, bias, history, temperature, repetition, presence, frequency, true);
   if (at::GradMode::is_enabled() && logits.requires_grad()) return Adjust::apply(logits, &h);
   const at::AutoDispatchBelowADInplaceOrView below;
@@ -478,6 +492,7 @@ struct Evaluate : torch::autograd::Function<Evaluate> {
 
 std::tuple<Tensor, Tensor> evaluate_actions(const Tensor& logits, const Tensor& given, const Maybe& allowed, const Maybe& bias, const Maybe& history,
                                             double temperature, double repetition, double presence, double frequency) {
+  reverse_only("evaluate_actions", {&logits});
   Head h(logits, allowed, bias, history, temperature, repetition, presence, frequency, true);
   Tensor actions = h.per_row("actions", given, "int32 or int64", given.scalar_type() == at::kInt || given.scalar_type() == at::kLong);
   if (actions.scalar_type() == at::kLong) actions = actions.clamp(-1, 0x7FFFFFFF).to(at::kInt);  // (kept outside [0, V) where it is outside)

@@ -26,7 +26,7 @@ def gated_recurrence(x: Tensor, gate: Optional[Tensor] = None, state: Optional[T
 
     Without `gate`, `x` is `[rows, steps, 2 * width]`: candidates, then gates (one projection; its gradient comes back as
     one tensor).  `state` float32 `[rows, width]` enters step 0 (None: zeros); where `resets` (bool or uint8
-    `[rows, steps]`) is set, the state entering that step is zero.  Differentiable once in x, gate and state."""
+    `[rows, steps]`) is set, the state entering that step is zero.  Differentiable once, in reverse mode, in x, gate and state."""
     return native.operators().gated_recurrence(x, gate, state, resets)
 
 

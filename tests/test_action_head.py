@@ -702,3 +702,38 @@ def test_many_rows_are_the_definitions(n, v):
         a, _, _ = sample_actions(logits.cuda(), u.cuda(), temperature=0.8, **_cuda(kw))
         want = _picked(_adjusted(logits, temperature=0.8, **kw)[0], _np(u))
         assert np.array_equal(a.cpu().numpy(), want)
+
+
+def test_forward_mode_is_refused():
+    """A dual tensor's tangent is not dropped; sampling carries no derivative of any kind."""
+    from torch.autograd import forward_ad
+
+    l, a, b = torch.zeros(3, 40), torch.zeros(3, dtype=torch.int32), torch.zeros(40)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(l, torch.ones_like(l))
+        with pytest.raises(RuntimeError, match="adjust_logits has no forward-mode"):
+            adjust_logits(dual)
+        with pytest.raises(RuntimeError, match="evaluate_actions has no forward-mode"):
+            evaluate_actions(dual, a)
+        bias = forward_ad.make_dual(b, torch.ones_like(b))
+        for call in (lambda: adjust_logits(l, bias=bias), lambda: evaluate_actions(l, a, bias=bias)):
+            with pytest.raises(RuntimeError, match="bias is a constant"):
+                call()
+        with forward_ad._set_fwd_grad_enabled(False), pytest.raises(RuntimeError, match="on GPU"):
+            adjust_logits(dual, bias=bias)
+        with pytest.raises(RuntimeError, match="on GPU"):
+            sample_actions(dual)
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused_on_device():
+    from torch.autograd import forward_ad
+
+    l, a = torch.randn(3, 40, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(l, torch.ones_like(l))
+        for call in (lambda: adjust_logits(dual), lambda: evaluate_actions(dual, a)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        for t in sample_actions(dual):
+            assert forward_ad.unpack_dual(t).tangent is None

@@ -591,3 +591,34 @@ def test_states_written_element_on_element():
     apart.copy_(x)
     memory = torch.as_strided(apart, (500, 64), (64, 1))
     assert torch.equal(gated_recurrence_step(apart, gate, state, resets, out_state=memory)[1], want)
+
+
+def test_forward_mode_is_refused():
+    """A dual tensor's tangent is not dropped."""
+    from torch.autograd import forward_ad
+
+    x, s = torch.zeros(2, 5, 4), torch.zeros(2, 4)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for args in ((dual(x),), (dual(x), x), (x, dual(x)), (x, x, dual(s))):
+            with pytest.raises(RuntimeError, match="gated_recurrence has no forward-mode"):
+                gated_recurrence(*args)
+        for args in ((dual(x[:, 0]), None, s[:, :2]), (x[:, 0], dual(x[:, 0]), s), (x[:, 0], x[:, 0], dual(s))):
+            with pytest.raises(RuntimeError, match="gated_recurrence_step has no forward-mode"):
+                gated_recurrence_step(*args)
+        with pytest.raises(RuntimeError, match="out_state.*tangent"):
+            gated_recurrence_step(x[:, 0], x[:, 0], s, out_state=dual(s.clone()))
+        with forward_ad._set_fwd_grad_enabled(False), pytest.raises(RuntimeError, match="on GPU"):
+            gated_recurrence(dual(x))
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused_on_device():
+    from torch.autograd import forward_ad
+
+    x = torch.randn(2, 20, 4, device="cuda")
+    with forward_ad.dual_level():
+        for leaf in (x, x.clone().requires_grad_()):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                gated_recurrence(forward_ad.make_dual(leaf, torch.ones_like(x)))
+        gated_recurrence(x)
