@@ -6,11 +6,13 @@
 // The kernels are reached through the C interface of the library that native.py has loaded (`bind`).
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <ATen/ATen.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
@@ -74,6 +76,12 @@ bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 // whether t is a dual tensor whose tangent a forward-mode derivative would go on with
 bool dual(const Tensor& t) { return t.defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined(); }
 Tensor empty(at::IntArrayRef shape, const Tensor& like, at::ScalarType type) { return at::empty(shape, like.options().dtype(type).requires_grad(false)); }
+
+// A launch is no operation of torch's: a trace would hold the results' memory without what fills it.
+void untraced(const char* who) {
+  if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY))
+    fail(std::string(who) + " cannot be traced");
+}
 
 // A call without requires_grad goes past autograd, which would refuse the tangent of a dual tensor: it is refused, not dropped.
 void reverse_only(const char* who, std::initializer_list<const Tensor*> tensors) {
@@ -217,6 +225,7 @@ struct Recurrence : torch::autograd::Function<Recurrence> {
 };
 
 std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& x_, const Maybe& gate_, const Maybe& state_, const Maybe& resets_) {
+  untraced("gated_recurrence");
   Tensor gate = or_none(gate_), state = or_none(state_);
   check_core(x_, gate, state, or_none(resets_), 3);
   reverse_only("gated_recurrence", {&x_, &gate, &state});
@@ -240,6 +249,7 @@ std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& x_, const Maybe& gate_
 }
 
 std::tuple<Tensor, Tensor> gated_recurrence_step(const Tensor& x, const Maybe& gate_, const Tensor& state, const Maybe& resets_, const Maybe& out_) {
+  untraced("gated_recurrence_step");
   const Tensor gate = or_none(gate_), resets = or_none(resets_);
   check_core(x, gate, state, resets, 2);
   reverse_only("gated_recurrence_step", {&x, &gate, &state});
@@ -425,6 +435,7 @@ struct Adjust : torch::autograd::Function<Adjust> {
 
 Tensor adjust_logits(const Tensor& logits, const Maybe& allowed, const Maybe& bias, const Maybe& history, double temperature, double repetition,
                      double presence, double frequency) {
+  untraced("adjust_logits");
   reverse_only("adjust_logits", {&logits});
   const Head h(logits, allowed, bias, history, temperature, repetition, presence, frequency, true);
   if (at::GradMode::is_enabled() && logits.requires_grad()) return Adjust::apply(logits, &h);
@@ -434,6 +445,7 @@ Tensor adjust_logits(const Tensor& logits, const Maybe& allowed, const Maybe& bi
 
 std::tuple<Tensor, Tensor, Tensor> sample_actions(const Tensor& logits, const Maybe& uniforms_, const Maybe& allowed, const Maybe& bias,
                                                   const Maybe& history, double temperature, double repetition, double presence, double frequency) {
+  untraced("sample_actions");
   Head h(logits, allowed, bias, history, temperature, repetition, presence, frequency, false);
   const at::AutoDispatchBelowADInplaceOrView below;
   const Tensor given = or_none(uniforms_);
@@ -492,6 +504,7 @@ struct Evaluate : torch::autograd::Function<Evaluate> {
 
 std::tuple<Tensor, Tensor> evaluate_actions(const Tensor& logits, const Tensor& given, const Maybe& allowed, const Maybe& bias, const Maybe& history,
                                             double temperature, double repetition, double presence, double frequency) {
+  untraced("evaluate_actions");
   reverse_only("evaluate_actions", {&logits});
   Head h(logits, allowed, bias, history, temperature, repetition, presence, frequency, true);
   Tensor actions = h.per_row("actions", given, "int32 or int64", given.scalar_type() == at::kInt || given.scalar_type() == at::kLong);

@@ -737,3 +737,17 @@ def test_forward_mode_is_refused_on_device():
                 call()
         for t in sample_actions(dual):
             assert forward_ad.unpack_dual(t).tangent is None
+
+
+def test_tracing_is_refused():
+    """A trace would hold the results' memory and not the launches that fill it."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    l, a = torch.zeros(3, 40), torch.zeros(3, dtype=torch.int32)
+    for call in (lambda t: adjust_logits(t), lambda t: sample_actions(t)[1], lambda t: evaluate_actions(t, a)[0]):
+        for leaf in (l, l.clone().requires_grad_()):
+            with pytest.raises(RuntimeError, match="cannot be traced"):
+                torch.jit.trace(call, leaf, check_trace=False)
+        for mode in ("real", "fake"):
+            with pytest.raises(RuntimeError, match="cannot be traced"):
+                make_fx(call, tracing_mode=mode)(l)

@@ -622,3 +622,17 @@ def test_forward_mode_is_refused_on_device():
             with pytest.raises(RuntimeError, match="forward-mode"):
                 gated_recurrence(forward_ad.make_dual(leaf, torch.ones_like(x)))
         gated_recurrence(x)
+
+
+def test_tracing_is_refused():
+    """A trace would hold the results' memory and not the launches that fill it."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x = torch.zeros(2, 5, 4)
+    for call in (lambda t: gated_recurrence(t, t)[0], lambda t: gated_recurrence_step(t[:, 0], t[:, 0], t[:, 0])[0]):
+        for leaf in (x, x.clone().requires_grad_()):
+            with pytest.raises(RuntimeError, match="cannot be traced"):
+                torch.jit.trace(call, leaf, check_trace=False)
+        for mode in ("real", "fake"):
+            with pytest.raises(RuntimeError, match="cannot be traced"):
+                make_fx(call, tracing_mode=mode)(x)
