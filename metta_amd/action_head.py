@@ -21,7 +21,7 @@ They share these controls, all keyword arguments, for logits `[..., V]` of float
 
 What stands at a masked token (NaN and infinities too) has no effect.  A row without an allowed token (or with -infinity
 at all of them) gives action -1, log-probability 0, entropy 0 and no gradient; a row with NaN or +infinity at an allowed
-token gives action -1 and NaN.
+token gives action -1 and NaN, and a gradient of NaN at every token that is left (allowed, and not at -infinity).
 """
 
 from __future__ import annotations

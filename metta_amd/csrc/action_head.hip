@@ -1330,7 +1330,7 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_wide_backward_kernel
     if (n <= 0) continue;
     X x[8];
     float g[8], slope[8], y[8];
-    const unsigned ok = raw[c].template columns<false, true, adjust>(r, a.type, v0, n, counts + at, x, slope);
+    raw[c].template columns<false, true, adjust>(r, a.type, v0, n, counts + at, x, slope);
 #pragma unroll
     for (int e = 0; e < 8; e++) {
       const float t = (float)(top - x[e]);
@@ -1340,14 +1340,14 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_wide_backward_kernel
 #pragma unroll
       for (int e = 0; e < 8; e++) if (v0 + e == act) g[e] += gp;
     }
-    if (bad || empty) {
+    if (bad) {
 #pragma unroll
-      for (int e = 0; e < 8; e++) g[e] = bad ? NAN : 0;
+      for (int e = 0; e < 8; e++) g[e] = NAN;
     }
 #pragma unroll
     for (int e = 0; e < 8; e++) {
       if (adjust) g[e] *= slope[e];
-      y[e] = __uint_as_float(__float_as_uint(g[e]) & head_bit(ok, e));
+      y[e] = x[e] != (X)-INFINITY ? g[e] : 0.f;  // (masked, or no part of the row; nothing is left of an empty one)
     }
     head_store<8>(dlogits, a.type, row * a.width + v0, n, y);
   }

@@ -751,3 +751,29 @@ def test_tracing_is_refused():
         for mode in ("real", "fake"):
             with pytest.raises(RuntimeError, match="cannot be traced"):
                 make_fx(call, tracing_mode=mode)(l)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("v", [5, 64, 157, 700, 1500, 5000, 20000])
+def test_gradients_of_bad_rows(v, dtype):
+    """NaN or +infinity at an allowed token makes the gradient of every token that is left NaN, and of none that is not: masked,
+    or at -infinity.  An infinite outer gradient passes by those, too."""
+    g = torch.Generator().manual_seed(v)
+    logits = torch.randn(4, v, generator=g).to(dtype)
+    logits[0, 0], logits[1, v - 1], logits[:, 2] = float("nan"), INF, -INF
+    allowed = torch.ones(4, v, dtype=torch.bool)
+    allowed[:, 3] = False
+    logits[:, 3] = float("nan")
+    history = torch.tensor([[1, 2, 3, -1]], dtype=torch.int32).expand(4, 4)
+    outer = torch.tensor([1.0, 1.0, INF, 1.0], device="cuda")
+    for kw in (dict(), dict(bias=torch.randn(v, generator=g)), dict(history=history, repetition=1.5, presence=0.25)):
+        x = logits.cuda().requires_grad_()
+        out = evaluate_actions(x, torch.ones(4, dtype=torch.int32, device="cuda"), **_cuda(dict(allowed=allowed, **kw)))
+        for outs in (out, out[:1], out[1:]):
+            (d,) = torch.autograd.grad(outs, x, [outer] * len(outs), retain_graph=True)
+            nan = torch.isnan(d).cpu()
+            assert bool((d[:, 2:4] == 0).all()), "no part in the row"
+            left = torch.ones(v, dtype=torch.bool)
+            left[2:4] = False
+            assert torch.equal(nan[0], left) and torch.equal(nan[1], left) and not bool(nan[3].any())
