@@ -391,7 +391,8 @@ int mg_adjust_logits_backward(const mg_logits* a, const void* dout, void* dlogit
 
 /* One action per row from the adjusted logits: the first v whose running sum of exp exceeds u * (the whole sum), as
  * 64-bit arithmetic finds it; without uniforms (NULL) the first of the largest.  log_prob and entropy f32 [rows].
- * A row without an allowed token: -1, 0, 0; with NaN or +infinity at an allowed token: -1, NaN, NaN. */
+ * A row without an allowed token: -1, 0, 0; with NaN or +infinity at an allowed token, or a uniform of NaN: -1, NaN,
+ * NaN.  Uniforms below 0 are taken as 0; from 1 on they pick the last token with any weight. */
 int mg_sample_actions(const mg_logits* a, const float* uniforms, int32_t* actions, float* log_prob, float* entropy,
                       void* stream);
 

@@ -77,8 +77,8 @@ def sample_actions(
 
     With `uniforms` (float32 in [0, 1), one per row, for instance `torch.rand`) the action is the first token at which the
     running sum of the probabilities exceeds the uniform, as 64-bit arithmetic finds it: the same numbers give the same
-    actions whatever the shape of the batch (1 and more: the last token with any weight).  Without, it is the most likely token (the lowest of equals).  Carries no
-    gradient; `evaluate_actions` does."""
+    actions whatever the shape of the batch.  (1 and more: the last token with any weight; below 0: as 0; NaN: action -1 and
+    NaN.)  Without, it is the most likely token (the lowest of equals).  Carries no gradient; `evaluate_actions` does."""
     return native.operators().sample_actions(logits, uniforms, allowed, bias, history, temperature, repetition, presence, frequency)
 
 

@@ -9,7 +9,7 @@
 //   sampled: the first v with sum_{w <= v} exp(-d_w) > u Z;  without u: the first v with x = M
 //   log q_v = -d_v - log Z;   d x_v of g_p log q_a + g_h H:  (g_p (1[v = a] - q_v) - g_h q_v (log q_v + H)) / temperature
 // A row with nothing left (M = -infinity) has action -1, log-probability 0, entropy 0 and no gradient; a row with NaN
-// or +infinity among its allowed tokens has action -1 and NaN.
+// or +infinity among its allowed tokens, or with a u of NaN, has action -1 and NaN.
 //
 // Rows of up to HEAD_NARROW columns are held in registers, E adjacent columns per lane, by as many lanes as that takes
 // (one lane for five actions, a wave for five hundred); rows of up to HEAD_ROW columns by a block, in chunks of eight columns
@@ -670,7 +670,9 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_sample_narrow_kernel(HeadArgs
     return;
   }
   h.template hold<false, true>(a, g, r, scale, mine);
-  const double u = fmax((double)uniforms[h.row], 0.0), target = u < 1.0 ? u * h.all : INFINITY;
+  const float uniform = uniforms[h.row];
+  h.bad = h.bad || uniform != uniform;
+  const double u = fmax((double)uniform, 0.0), target = u < 1.0 ? u * h.all : INFINITY;
   bool unsure = false;
   if (h.template picks<true>(g, target)) {
     const HeadPick<float> pick = head_pick<E>(h.w, h.t, h.before, target);
@@ -1040,7 +1042,12 @@ __global__ __launch_bounds__(THREADS) void mg_sample_row_kernel(HeadArgs a, cons
     if (threadIdx.x == 0) head_sampled(row, h.bad, h.empty, first, 0.f, h.z, h.s, scale, actions, log_prob, entropy);
     return;
   }
-  const double all = head_total(red.z, CHUNKS * WAVES), u = fmax((double)uniforms[row], 0.0), target = u < 1.0 ? u * all : INFINITY;
+  const float uniform = uniforms[row];
+  if (uniform != uniform) {
+    if (threadIdx.x == 0) head_sampled(row, true, false, -1, 0.f, h.z, h.s, scale, actions, log_prob, entropy);
+    return;
+  }
+  const double all = head_total(red.z, CHUNKS * WAVES), u = fmax((double)uniform, 0.0), target = u < 1.0 ? u * all : INFINITY;
   const HeadSpot spot = head_spot(red.z, CHUNKS * WAVES, 0.0, target);
   if (spot.entry % WAVES == (int)threadIdx.x >> 6) {
 #pragma unroll
@@ -1199,8 +1206,10 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_sample_join_kernel(HeadArgs a
   const HeadRow r = head_row(a, row);
   const HeadScale<double> scale(r);
   const double* f = found + row * parts * HEAD_FOUND;
-  const HeadJoined j = head_join(f, parts, scale, head_lane());
-  const double u = uniforms ? fmax((double)uniforms[row], 0.0) : 0.0, target = u < 1.0 ? u * j.z : INFINITY;
+  const float uniform = uniforms ? uniforms[row] : 0.f;
+  HeadJoined j = head_join(f, parts, scale, head_lane());
+  j.bad = j.bad || uniform != uniform;
+  const double u = fmax((double)uniform, 0.0), target = u < 1.0 ? u * j.z : INFINITY;
   HeadPick<double> pick{0, 0.0, 0.0, 0.0};
   bool picks = threadIdx.x == 0;
   int v0 = 0;

@@ -777,3 +777,27 @@ def test_gradients_of_bad_rows(v, dtype):
             left = torch.ones(v, dtype=torch.bool)
             left[2:4] = False
             assert torch.equal(nan[0], left) and torch.equal(nan[1], left) and not bool(nan[3].any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v", [1, 5, 64, 157, 700, 1500, 5000, 8192, 9000, 20000])
+def test_uniforms_of_nan_show(v):
+    """A uniform of NaN gives action -1 and NaN, as a logit of NaN does; the rows beside it keep theirs.  Uniforms outside of
+    [0, 1) are taken as 0 and as 1."""
+    for kw in (dict(mask=False, bias=None, length=0), dict(empty=False)):
+        logits, c, u = _case(70, v, torch.float32, seed=v, **kw)
+        if "allowed" in c:
+            c["allowed"][:, 0] = True  # no row is empty
+        x, dev = logits.cuda(), _cuda(c)
+        want = [t.clone() for t in sample_actions(x, u.cuda(), **dev)]
+        bad = u.clone()
+        bad[[0, 33, 69]] = torch.tensor([float("nan"), float("nan"), -float("nan")])
+        got = sample_actions(x, bad.cuda(), **dev)
+        for a, b in zip(got, want):
+            keep = ~torch.isnan(bad).cuda()
+            assert torch.equal(a[keep], b[keep])
+        lost = torch.isnan(bad).cuda()
+        assert bool((got[0][lost] == -1).all()) and bool(torch.isnan(got[1][lost]).all()) and bool(torch.isnan(got[2][lost]).all())
+        for outside, inside in ((-1.0, 0.0), (-INF, 0.0), (INF, 1.0), (2.0, 1.0)):
+            for a, b in zip(sample_actions(x, torch.full_like(u, outside).cuda(), **dev), sample_actions(x, torch.full_like(u, inside).cuda(), **dev)):
+                assert torch.equal(a, b)
