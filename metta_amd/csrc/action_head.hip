@@ -128,6 +128,14 @@ __device__ __forceinline__ W head_far(X m, X x) {
   if constexpr (sizeof(W) > sizeof(X)) return (W)m - (W)x;
   else return (W)(m - x);
 }
+// (M - x) / temperature of one token: as far as the temperature brings it back, also where M - x leaves the range of 32 bits;
+// infinity for a token at -infinity
+template <typename X>
+__device__ __forceinline__ float head_distance(const HeadRow& r, X m, X x) {
+  if (x == (X)-INFINITY) return INFINITY;
+  if constexpr (sizeof(X) == 8) return (float)((m - x) * r.inv_temp);
+  else return (0.5f * m - 0.5f * x) * (2.0f * (float)r.inv_temp);
+}
 __device__ __forceinline__ double head_max(double a, double b) { return fmax(a, b); }  // (a NaN loses)
 __device__ __forceinline__ float head_max(float a, float b) { return fmaxf(a, b); }
 
@@ -722,7 +730,7 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_kernel(HeadAr
 #pragma unroll
   for (int e = 0; e < E; e++) at = h.v0 + e == act ? h.x[e] : at;
   if (!ONE) at = head_group_max(at, g.lanes);
-  const float d = at == (X)-INFINITY ? INFINITY : head_far<float, X>(h.m, at) * scale.inv_temp;
+  const float d = head_distance(r, h.m, at);
   if (h.mine && h.lane == 0) {
     const float log_z = head_log(h.z);
     log_prob[h.row] = h.bad ? NAN : h.empty ? 0.f : (float)(-d - log_z);
@@ -1087,7 +1095,7 @@ __global__ __launch_bounds__(THREADS) void mg_evaluate_row_kernel(HeadArgs a, co
 #pragma unroll
       for (int e = 0; e < 8; e++) x = h.at(c) + e == act ? h.x[c][e] : x;
     }
-    const float log_z = head_log(h.z), d = x == (X)-INFINITY ? INFINITY : head_far<float, X>(h.m, x) * scale.inv_temp;
+    const float log_z = head_log(h.z), d = head_distance(r, h.m, x);
     log_prob[row] = h.bad ? NAN : h.empty ? 0.f : -d - log_z;
     entropy[row] = h.bad ? NAN : h.empty ? 0.f : log_z + h.s * head_inverse(h.z);
     if (stats) stats[2 * row] = h.bad ? NAN : (double)h.m, stats[2 * row + 1] = h.bad ? NAN : h.empty ? 0.0 : (double)log_z;

@@ -801,3 +801,29 @@ def test_uniforms_of_nan_show(v):
         for outside, inside in ((-1.0, 0.0), (-INF, 0.0), (INF, 1.0), (2.0, 1.0)):
             for a, b in zip(sample_actions(x, torch.full_like(u, outside).cuda(), **dev), sample_actions(x, torch.full_like(u, inside).cuda(), **dev)):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v", [2, 7, 100, 900, 3000, 20000])
+def test_log_probabilities_of_the_furthest_tokens(v):
+    """Tokens further apart than the largest number of 32 bits, which the temperature brings back into its range."""
+    logits = torch.randn(4, v, generator=torch.Generator().manual_seed(v))
+    logits[:, 0] = torch.tensor([3e38, 3.4e38, 2e38, 1e38])
+    logits[:, 1] = torch.tensor([-3e38, -3.4e38, -2.5e38, -3.3e38])
+    bias = torch.zeros(v)
+    bias[0], bias[1] = 3e38, -3e38
+    actions = torch.ones(4, dtype=torch.int32)
+    for kw in (dict(), dict(bias=bias)):
+        for temperature in (0.5, 1.0, 2.0, 4.0, 7.0, 1e10, 1e30):
+            l, _ = _adjusted(logits, temperature=temperature, **kw)
+            s = _stats(l)
+            x = logits.cuda().requires_grad_()
+            logp, h = evaluate_actions(x, actions.cuda(), temperature=temperature, **_cuda(kw))
+            want, got, most = l[:, 1] - s["m"] - np.log(s["z"]), _np(logp), float(np.finfo(np.float32).max)
+            # difference, scale (a rounding of its own) and product: 3u, and one for the sum
+            assert np.all(np.isneginf(got[want < -most * (1 + 8 * U)])), temperature
+            fine = want > -most * (1 - 8 * U)
+            assert np.all(np.abs(got - want)[fine] <= (5 * U * np.abs(want))[fine]), (temperature, got, want)
+            assert np.all(_np(h) == 0.0)
+            (d,) = torch.autograd.grad([logp, h], x, [torch.ones_like(logp)] * 2)
+            assert bool(torch.isfinite(d).all())
