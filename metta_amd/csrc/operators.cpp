@@ -69,9 +69,12 @@ int type_of(const Tensor& t) {
 bool has(const Maybe& t) { return t && t->defined(); }
 Tensor or_none(const Maybe& t) { return has(t) ? *t : Tensor(); }
 void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-Tensor contiguous(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+// (a view that holds its values negated, like the imaginary part of a conjugate, is written out: kernels read memory as it is)
+Tensor plain(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+Tensor contiguous(const Tensor& t) { return t.defined() ? plain(t).contiguous() : t; }
 // columns next to each other
-Tensor adjacent(const Tensor& t) { return !t.defined() || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+bool adjacent_columns(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1; }
+Tensor adjacent(const Tensor& t) { return !t.defined() ? t : adjacent_columns(t) ? plain(t) : t.contiguous(); }
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 // whether t is a dual tensor whose tangent a forward-mode derivative would go on with
 bool dual(const Tensor& t) { return t.defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined(); }
@@ -147,7 +150,7 @@ void check_device(const Tensor& x) { require(x.is_cuda(), "All tensors must be o
 // Whether a contiguous `out` of [rows, width] lies over what a step reads of `t` ([rows, width] from column `from` on), otherwise than
 // element on element: a thread would write what another has yet to read.  (A t that is copied before the launch is no matter.)
 bool written_over(const Tensor& out, const Tensor& t, int64_t from, int64_t width) {
-  if (!out.numel() || !t.numel() || (t.stride(-1) != 1 && t.size(-1) != 1)) return false;
+  if (!out.numel() || !t.numel() || !adjacent_columns(t) || t.is_neg()) return false;
   const int64_t size = t.element_size(), rows = out.size(0), row = t.stride(0) * size, wide = width * size, bytes = out.numel() * out.element_size();
   // bytes from out's first to t's
   const int64_t at = reinterpret_cast<intptr_t>(t.data_ptr()) + from * size - reinterpret_cast<intptr_t>(out.data_ptr());
@@ -231,7 +234,7 @@ std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& x_, const Maybe& gate_
   reverse_only("gated_recurrence", {&x_, &gate, &state});
   check_device(x_);
   const Core given(x_, gate);
-  if (state.defined()) state = state.contiguous();
+  state = contiguous(state);
   if (x_.numel() == 0) {  // nothing to compute; part of the graph all the same
     const Tensor xs = gate.defined() ? x_ : x_.narrow(2, 0, given.width), gs = gate.defined() ? gate : x_.narrow(2, given.width, given.width);
     return {xs + gs, state.defined() ? state.clone() : at::zeros({x_.size(0), given.width}, x_.options().dtype(at::kFloat).requires_grad(false))};
@@ -258,7 +261,7 @@ std::tuple<Tensor, Tensor> gated_recurrence_step(const Tensor& x, const Maybe& g
           "gated_recurrence_step has no gradient: call it under torch.no_grad(), or use gated_recurrence");
   Tensor out = or_none(out_);
   if (out.defined()) {
-    require(out.sizes() == state.sizes() && out.scalar_type() == at::kFloat && out.device() == x.device() && out.is_contiguous(),
+    require(out.sizes() == state.sizes() && out.scalar_type() == at::kFloat && out.device() == x.device() && out.is_contiguous() && !out.is_neg(),
             "out_state must be contiguous float32 [rows, width] on x's device");
     require(!grad || !out.requires_grad(), "out_state is written in place and must not require a gradient");
     require(!dual(out), "out_state is written in place and must not carry a tangent");
@@ -370,7 +373,7 @@ struct Head {
       const std::string w = std::to_string(width);
       fail(std::string(name) + " must be [" + w + "] or [..., " + w + "] with the logits' leading dimensions");
     }
-    if (t.dim() == 1) return t.contiguous();
+    if (t.dim() == 1) return contiguous(t);
     const Tensor rows = as_rows(t);
     row = rows.stride(0);
     return rows;
@@ -380,7 +383,7 @@ struct Head {
     if (!typed) fail(std::string(name) + " must be " + types);
     if (t.sizes() != at::IntArrayRef(lead)) fail(std::string(name) + " must have the logits' shape without its last dimension");
     require(t.device() == logits.device(), "All tensors must be on same device");
-    return t.contiguous();
+    return contiguous(t);
   }
   Tensor work() {
     const int64_t size = lib.mg_logits_workspace(&a);

@@ -827,3 +827,28 @@ def test_log_probabilities_of_the_furthest_tokens(v):
             assert np.all(_np(h) == 0.0)
             (d,) = torch.autograd.grad([logp, h], x, [torch.ones_like(logp)] * 2)
             assert bool(torch.isfinite(d).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v", [5, 157, 9000])
+def test_negated_views(v):
+    """Views that hold their values negated give what their values give, gradients too."""
+    logits, c, u = _case(6, v, torch.float32, seed=v)
+    dev, l, uni = _cuda(c), logits.cuda(), u.cuda()
+    neg = lambda t: torch._neg_view(-t)  # noqa: E731
+    other = dev | {"bias": neg(dev["bias"])}
+    assert neg(l).is_neg() and torch.equal(neg(l), l)
+    for a, b in zip(sample_actions(neg(l), neg(uni), **other), sample_actions(l, uni, **dev)):
+        assert torch.equal(a, b)
+    actions = sample_actions(l, uni, **dev)[0]
+
+    def grads(view, kw):
+        leaf = l.clone().requires_grad_()
+        t = neg(leaf) if view else leaf
+        w = neg if view else (lambda y: y)
+        logp, h = evaluate_actions(t, actions, **kw)
+        adj = adjust_logits(t, **kw)
+        return [logp, h, adj, *torch.autograd.grad([logp, h], leaf, [w(uni), w(uni)]), *torch.autograd.grad(adj, leaf, w(l))]
+
+    for a, b in zip(grads(True, other), grads(False, dev)):
+        assert torch.equal(a, b)

@@ -636,3 +636,24 @@ def test_tracing_is_refused():
         for mode in ("real", "fake"):
             with pytest.raises(RuntimeError, match="cannot be traced"):
                 make_fx(call, tracing_mode=mode)(x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("steps", [1, 40])
+def test_negated_views(steps):
+    """Views that hold their values negated (the imaginary part of a conjugate) give what their values give, gradients too."""
+    x, gate, state, _, dh, dlast = (t.cuda() for t in _inputs(3, steps, 16, torch.float32, seed=5))
+    neg = lambda t: torch.complex(torch.zeros_like(t), -t).conj().imag  # noqa: E731
+    assert neg(x).is_neg() and torch.equal(neg(x), x)
+    got = gated_recurrence_step(neg(x)[:, 0], neg(gate)[:, 0], neg(state))
+    for a, b in zip(got, gated_recurrence_step(x[:, 0], gate[:, 0], state)):
+        assert torch.equal(a, b)
+    with pytest.raises(RuntimeError, match="out_state"):
+        gated_recurrence_step(x[:, 0], gate[:, 0], state, out_state=torch._neg_view(state.clone()))
+    leaves = [t.clone().requires_grad_() for t in (x, gate, state)]
+    views = [torch._neg_view(-t) for t in leaves]
+    assert all(t.is_neg() for t in views)
+    out, want = gated_recurrence(*views), gated_recurrence(*leaves)
+    assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+    for a, b in zip(torch.autograd.grad(out, leaves, [torch._neg_view(-dh), torch._neg_view(-dlast)]), torch.autograd.grad(want, leaves, [dh, dlast])):
+        assert torch.equal(a, b)
