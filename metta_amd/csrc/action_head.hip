@@ -1284,7 +1284,7 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_sample_join_kernel(HeadArgs a
 __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_join_kernel(HeadArgs a, int parts, const double* __restrict__ found,
                                                                        const int* __restrict__ actions, float* __restrict__ log_prob,
                                                                        float* __restrict__ entropy, double* __restrict__ stats) {
-  const long row = ((long)blockIdx.x * HEAD_THREADS + threadIdx.x) >> 6;
+  const long row = head_block() * (HEAD_THREADS / 64) + (threadIdx.x >> 6);
   if (row >= a.rows) return;
   const HeadRow r = head_row(a, row);
   const HeadJoined j = head_join(found + row * parts * HEAD_FOUND, parts, HeadScale<double>(r), head_lane());
@@ -1408,6 +1408,7 @@ static dim3 head_wide_grid(const mg_logits* a, int chunks = 1) {
   const int64_t y = a->rows < 32768 ? a->rows : 32768;
   return dim3(head_parts(a, chunks), (unsigned)y, (unsigned)((a->rows + y - 1) / y));
 }
+// (a dimension of a grid has fewer than 2^32 threads)
 static dim3 head_grid(int64_t blocks) {
   const int64_t x = blocks < 1 << 20 ? blocks : 1 << 20;
   return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
@@ -1577,8 +1578,8 @@ extern "C" int mg_evaluate_actions(const mg_logits* a, const int32_t* actions, f
     }
   });
   if (head_wide(a))
-    hipLaunchKernelGGL(mg_evaluate_join_kernel, dim3((unsigned)((a->rows + 3) / 4)), dim3(HEAD_THREADS), 0, s, head_args(a), head_parts(a, head_chunks(a)),
-                       (const double*)a->workspace, actions, log_prob, entropy, stats);
+    hipLaunchKernelGGL(mg_evaluate_join_kernel, head_grid((a->rows + HEAD_THREADS / 64 - 1) / (HEAD_THREADS / 64)), dim3(HEAD_THREADS), 0, s, head_args(a),
+                       head_parts(a, head_chunks(a)), (const double*)a->workspace, actions, log_prob, entropy, stats);
   return head_launched(who);
 } catch (...) {
   return 1;

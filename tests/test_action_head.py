@@ -852,3 +852,16 @@ def test_negated_views(v):
 
     for a, b in zip(grads(True, other), grads(False, dev)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_evaluation_of_more_rows_than_a_grid_has_waves():
+    """A wave per row joins the parts of wide rows; 2^26 of them are more threads than one dimension of a grid takes."""
+    n, v = (1 << 26) + 5, 8193
+    logits = torch.randn(1, v, generator=torch.Generator().manual_seed(0)).cuda()
+    actions = (torch.arange(n, device="cuda", dtype=torch.int32) * 7) % v
+    logp, h = evaluate_actions(logits.expand(n, v), actions)
+    one, ent = evaluate_actions(logits.expand(v, v), torch.arange(v, device="cuda", dtype=torch.int32))
+    assert bool((h == ent[0]).all()) and torch.equal(logp, one[actions.long()])
+    some = np.arange(0, v, 100)
+    _check_rows(one.cpu()[some], ent.cpu()[some], _np(logits).repeat(len(some), 0), some)
