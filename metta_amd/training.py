@@ -227,7 +227,7 @@ def evaluate_experience(policy, experience: DeviceExperience, controls=None, row
     logits, values, _ = policy.evaluate(b["env_obs"][rows], state, resets)
     kw = {} if controls is None else dict(controls.controls)
     for name in ("allowed", "bias"):  # one row per agent cannot be told from the store's rows
-        if name in kw and kw[name].dim() > 1:
+        if kw.get(name) is not None and kw[name].dim() > 1:
             raise ValueError(f"{name} must be the same for all agents")
     if controls is not None and controls.history_length:
         kw["history"] = history[rows]

@@ -175,3 +175,30 @@ def test_plain_rollout_with_controls():
         steps, _, state, _ = rollout(env, policy, 3, state=state, generator=g)
         assert steps == 3 * 72
     env.close()
+
+
+def test_evaluation_without_some_controls(monkeypatch):
+    """Controls of None are none, as in the rollout; one row per agent is still refused."""
+    import metta_amd.action_head
+
+    seen = {}
+
+    def evaluate_actions(logits, actions, **kw):
+        seen.update(kw)
+        return torch.zeros(actions.shape), torch.zeros(actions.shape)
+
+    monkeypatch.setattr(metta_amd.action_head, "evaluate_actions", evaluate_actions)
+
+    class Policy:
+        def evaluate(self, obs, state, resets):
+            return torch.zeros(*obs.shape[:2], 5), torch.zeros(obs.shape[:2]), None
+
+    ex = DeviceExperience(2, 8, 4, experience_spec(4), "cpu")
+    bias = torch.zeros(5)
+    logp, entropy, values = evaluate_experience(Policy(), ex, ActionControls(allowed=None, bias=bias, temperature=0.5))
+    assert logp.shape == entropy.shape == values.shape == (2, 4)
+    assert seen["allowed"] is None and seen["bias"] is bias and seen["temperature"] == 0.5
+    evaluate_experience(Policy(), ex, ActionControls(allowed=None, bias=None))
+    for name, t in (("allowed", torch.ones(2, 5, dtype=torch.bool)), ("bias", torch.zeros(2, 5))):
+        with pytest.raises(ValueError, match=f"{name} must be the same for all agents"):
+            evaluate_experience(Policy(), ex, ActionControls(**{name: t}))
