@@ -89,7 +89,8 @@ def reset_state(policy, state, done: torch.Tensor):
 class ActionControls:
     """Controls of the action head (`allowed`, `bias`, `temperature`, `repetition`, `presence`, `frequency`; see
     metta_amd/action_head.py) for a rollout, and the recent actions that the penalties look at: the last `history_length`
-    of every agent, forgotten when its episode ends (an environment that is started anew wants new controls)."""
+    of every agent, forgotten when its episode ends (an environment that is started anew wants new controls).  `rollout` and
+    `rollout_phase` keep histories of their own."""
 
     def __init__(self, history_length: int = 0, **controls):
         if "history" in controls:
@@ -104,7 +105,11 @@ class ActionControls:
             return None
         if key not in self._recent:
             self._recent[key] = [torch.full((n, self.history_length), -1, dtype=torch.int32, device=device), 0]
-        return self._recent[key][0]
+        h = self._recent[key][0]
+        d = torch.device(device)
+        if h.shape[0] != n or h.device.type != d.type or d.index not in (None, h.device.index):
+            raise ValueError(f"this history is of {h.shape[0]} agents on {h.device}, not of {n} on {device}: another environment wants new controls")
+        return h
 
     def ended(self, key, done: torch.Tensor) -> None:
         if key in self._recent:

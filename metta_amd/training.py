@@ -173,8 +173,8 @@ def rollout_phase(
             actions = torch.multinomial(logp_all.exp(), 1, generator=generator).squeeze(1)
             log_prob = logp_all.gather(1, actions.unsqueeze(1)).squeeze(1)
         else:
-            history = controls.history(key, n, o.device)
-            controls.ended(key, done)
+            history = controls.history(("phase", key), n, o.device)  # (`rollout` with the same controls keeps another)
+            controls.ended(("phase", key), done)
             actions, log_prob, _ = controls.sample(logits, history, generator)
             if history is not None:
                 td["action_history"] = history
@@ -191,7 +191,7 @@ def rollout_phase(
         if on_step is not None:
             on_step(td, training_env_id)
         if controls is not None:
-            controls.took(key, td["actions"])
+            controls.took(("phase", key), td["actions"])
         env.send_actions(td["actions"])  # the device tensor itself: no .cpu().numpy()
         if info:
             result.raw_infos.extend(info)

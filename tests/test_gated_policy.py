@@ -202,3 +202,48 @@ def test_evaluation_without_some_controls(monkeypatch):
     for name, t in (("allowed", torch.ones(2, 5, dtype=torch.bool)), ("bias", torch.zeros(2, 5))):
         with pytest.raises(ValueError, match=f"{name} must be the same for all agents"):
             evaluate_experience(Policy(), ex, ActionControls(**{name: t}))
+
+
+def test_histories_are_kept_apart(monkeypatch):
+    """A history that was made for other agents or another device is refused, not used; each of the two loops keeps its own."""
+    from types import SimpleNamespace
+
+    from metta_amd.rollout import rollout
+    from metta_amd.training import rollout_phase
+
+    c = ActionControls(history_length=3, repetition=1.5)
+    c.history(0, 4, "cpu")
+    with pytest.raises(ValueError, match="4 agents.*new controls"):
+        c.history(0, 5, "cpu")
+    with pytest.raises(ValueError, match="new controls"):
+        c.history(0, 4, "meta")
+    assert c.history(0, 4, torch.device("cpu")).shape == (4, 3)
+
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: None)  # everything here is on the CPU
+    n, obs, zero = 2, torch.zeros(2, 4, 3, dtype=torch.uint8), torch.zeros(2)
+    off = torch.zeros(2, dtype=torch.bool)
+
+    class Policy(torch.nn.Linear):
+        def initial_state(self, n, device, dtype=None):
+            return (torch.zeros(n, 1),)
+
+        def forward(self, o, state, resets=None):
+            return torch.zeros(len(o), 5), torch.zeros(len(o)), state
+
+    class Controls(ActionControls):
+        taken, seen = 0, None
+
+        def sample(self, logits, history, generator=None):
+            self.seen = [] if self.seen is None else self.seen
+            self.seen.append(sorted(history[0].tolist()))
+            self.taken += 1
+            return torch.full((len(logits),), self.taken, dtype=torch.int32), torch.zeros(len(logits)), torch.zeros(len(logits))
+
+    vecenv = SimpleNamespace(observations=obs, num_agents=n, recv=lambda: (obs, zero, off, off, None, None, None, None), send=lambda a: None)
+    env = SimpleNamespace(get_observations=lambda: (obs, zero, off, off, None, None, slice(0, 2), None, 2), send_actions=lambda a: None)
+    controls = Controls(history_length=2, presence=1.0)
+    ex = DeviceExperience(2, 4, 2, experience_spec(4, history_length=2), "cpu")
+    rollout_phase(env, Policy(1, 1), ex, controls=controls)
+    rollout(vecenv, Policy(1, 1), 2, controls=controls)
+    rollout_phase(env, Policy(1, 1), ex, controls=controls)
+    assert controls.seen == [[-1, -1], [-1, 1], [-1, -1], [-1, 3], [1, 2], [2, 5]]
