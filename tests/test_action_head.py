@@ -865,3 +865,39 @@ def test_evaluation_of_more_rows_than_a_grid_has_waves():
     assert bool((h == ent[0]).all()) and torch.equal(logp, one[actions.long()])
     some = np.arange(0, v, 100)
     _check_rows(one.cpu()[some], ent.cpu()[some], _np(logits).repeat(len(some), 0), some)
+
+
+@pytest.mark.gpu
+def test_exponentials_are_within_the_margin_of_sampling():
+    """2^-t as the kernels compute it, for every t of 32 bits from 0 to 125.9: within the 2 units of 2^-24 that the margin of sampling
+    takes for it.  Stats of (0, 0), a temperature of log2 e and an outer gradient that their factor makes 1 leave the backward
+    pass of wide rows with minus the exponential itself."""
+    import ctypes as ct
+
+    from metta_amd import native
+
+    L = native.load()
+    rows, v = 16384, 8193  # column 0 is the action's
+    temperature = float(np.log2(np.e))
+    inv = np.float32(1.0 / temperature)
+    outer = next(g for k in range(-4, 5) for g in [np.float32(1.0 / float(inv)) + np.float32(k * 2.0**-23)] if np.float32(g * inv) == np.float32(1.0))
+    assert np.float32(1.0 / temperature * -1.4426950408889634) == np.float32(-1.0)
+    logits = torch.zeros(rows, v, device="cuda")
+    out = torch.empty_like(logits)
+    actions = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    zero = torch.zeros(rows, device="cuda")
+    stats = torch.zeros(rows, 2, dtype=torch.float64, device="cuda")
+    dlogp = torch.full((rows,), float(outer), device="cuda")
+    a = native.MgLogits(logits=logits.data_ptr(), rows=rows, width=v, logits_row=v, temperature=temperature, repetition=1.0)
+    last = int(np.float32(125.9).view(np.int32))
+    each, worst = rows * (v - 1), 0.0
+    for first in range(0, last, each):
+        bits = torch.arange(first, first + each, dtype=torch.int64, device="cuda").clamp_(max=last).to(torch.int32)
+        t = bits.view(torch.float32).view(rows, v - 1)
+        logits[:, 1:] = -t
+        rc = L.mg_evaluate_actions_backward(ct.byref(a), actions.data_ptr(), zero.data_ptr(), stats.data_ptr(), dlogp.data_ptr(), None, out.data_ptr(),
+                                            torch.cuda.current_stream().cuda_stream)
+        assert rc == 0, L.mg_last_error()
+        want = torch.exp2(-t.double())
+        worst = max(worst, float(((-out[:, 1:].double() - want) / want).abs().max()))
+    assert 0.0 < worst <= 2 * U, worst / U
