@@ -338,7 +338,7 @@ def main() -> None:
             os.environ.setdefault("WORLD_SIZE", "1")
         dist.init_process_group(backend="nccl", device_id=dev)
 
-    wl = bench_workload(args.workload)
+    wl = bench_workload(args.workload, policy=args.policy)
     E, A = args.envs or wl["envs"], wl["agents"]
     groups = args.groups or wl["groups"]
     G = groups if groups >= 1 and E % max(groups, 1) == 0 else 1

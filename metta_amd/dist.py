@@ -31,10 +31,11 @@ def bench_shard(rank: int, envs_per_rank: int, pool_len: int, base_seed: int = 0
     return [(base_seed + g) & 0xFFFFFFFF for g in ids], [g % pool_len for g in ids]
 
 
-def bench_workload(name: str, small: bool = False) -> dict:
+def bench_workload(name: str, small: bool = False, policy: str = "lstm") -> dict:
     """The workloads `bench.py --workload` shards over ranks ([3], [4]); `small` = the same
-    configuration family at a size the CPU oracle steps in seconds (tests/test_dist_cpu.py).  `maps` is None where the
-    caller loads the committed pool of reference-generated arena maps."""
+    configuration family at a size the CPU oracle steps in seconds (tests/test_dist_cpu.py); `policy`: the
+    rollout's ("lstm" or "gated").  `maps` is None where the caller loads the committed pool of reference-generated arena
+    maps."""
     from .builder import make_arena, make_combat_stress
 
     if name in ("arena", "rollout"):
@@ -44,7 +45,7 @@ def bench_workload(name: str, small: bool = False) -> dict:
             # the host's launch work per step: 1.03 against 0.67 ms/step)
             "groups": 4 if name == "arena" else 1,
             "describe": "arena envs x 24 agents per GPU (BASELINE configs[1])" if name == "arena"
-            else "arena envs x 24 agents per GPU + LSTM policy forward and sampling in bf16 (BASELINE configs[4])",
+            else f"arena envs x 24 agents per GPU + {'LSTM' if policy == 'lstm' else 'gated recurrent'} policy forward and sampling in bf16 (BASELINE configs[4])",
         }  # fmt: skip
     if name == "combat":
         agents, side = (64, 32) if small else (1024, 256)

@@ -247,3 +247,11 @@ def test_histories_are_kept_apart(monkeypatch):
     rollout(vecenv, Policy(1, 1), 2, controls=controls)
     rollout_phase(env, Policy(1, 1), ex, controls=controls)
     assert controls.seen == [[-1, -1], [-1, 1], [-1, -1], [-1, 3], [1, 2], [2, 5]]
+
+
+def test_the_benchmark_names_its_policy():
+    from metta_amd.dist import bench_workload
+
+    lstm, gated = (bench_workload("rollout", policy=p)["describe"] for p in ("lstm", "gated"))
+    assert "LSTM" in lstm and lstm == bench_workload("rollout")["describe"]
+    assert "gated recurrent policy" in gated and "LSTM" not in gated
