@@ -7,6 +7,7 @@
 
 The first three are HIP kernels on torch's current stream (metta_amd/csrc/action_head.hip), one launch each (two for sampling
 and evaluation beyond 8192 tokens); there is no CPU path.
+Log-probabilities, entropies and gradients are computed in 32 bits, or 64 where the choice of an action needed them.
 They share these controls, all keyword arguments, for logits `[..., V]` of float32, bfloat16 or float16:
 
 * `allowed`: bool `[V]` or `[..., V]`, or int32 bits `[ceil(V / 32)]` or `[..., ceil(V / 32)]` (`pack_allowed`);

@@ -18,10 +18,12 @@
 // for the columns that it holds.
 //
 // The logits are held in 64 bits where a bias or a penalty could cancel large ones, the differences from the largest and all
-// that follows in 32, which log-probabilities, entropies and gradients need no more than.  A sampled action is the one that
-// 64 bits find all the same, whatever the order of the sums: the error of the running sum is bounded, and a row in which the
-// target comes within that bound of a token's border (one in hundreds or thousands) is done once more in 64 bits.  The parts
-// of wide rows are summed in 64 bits from the start, since hardly a row of theirs is clear of all its borders.
+// that follows in 32 (weights, sums, logarithm: log-probabilities and entropies are some 8e-8 off where 64 bits, rounded, are
+// 3e-8, in half of the time; gradients are rounded to the logits' type anyway).  A sampled action is the one that 64 bits find
+// all the same, whatever the order of the sums: the error of the running sum is bounded, and a row in which the target comes
+// within that bound of a token's border is done once more in 64 bits, its log-probability and entropy with it (normal logits:
+// 1 row in 1000 at 157 tokens, 1 in 200 at 1024, 1 in 25 at 8192).  The parts of wide rows are summed in 64 bits from the start:
+// 13 to 20 rows in 100 would be repeated at 32003 tokens and 35 to 56 at 131072, by launches of their own.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -653,8 +655,11 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_adjust_narrow_kernel(HeadArgs
   it.store(a, r, h.row, h.v0, h.n, counts[threadIdx.x], out, dout, dlogits);
 }
 
-// An action per row.  Bound by the launch and the way through it (24 x 5: 1.8 us; 98304 x 5 bf16, masks, 16 entries of history:
-// 6.4 us for 9 MB), from some 50 columns on by its instructions (98304 x 64 bf16: 10.6 us; all in 64 bits: 18).
+// An action per row.  Bound by the launch and the way through it (24 x 5: 2.0 us; 98304 x 5 bf16, masks, 16 entries of history:
+// 6.4 us for 9 MB), from some 50 columns on by its instructions (98304 x 64 bf16: 11 us, 7.5 of them the issue of 4.6 million
+// vector instructions; 32768 x 512: 25 us for 14.8 million, which take 24).  A long history over few columns is bound by its
+// count: a block counts for up to 256 rows, whatever its length, and a wave's lanes add to the same words (4096 x 5, 4096
+// entries: 520 us for 67 MB).
 template <int E, bool ONE, typename X>
 __global__ __launch_bounds__(HEAD_THREADS) void mg_sample_narrow_kernel(HeadArgs a, HeadNarrow g, const float* __restrict__ uniforms,
                                                                        int* __restrict__ actions, float* __restrict__ log_prob,
@@ -708,8 +713,8 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_sample_narrow_kernel(HeadArgs
   }
 }
 
-// Bound by memory at few columns (2097152 x 5 bf16: 10.6 us for 46 MB, 4.3 TB/s), by its instructions at many (32768 x 512 bf16: 18
-// us).
+// Bound by memory at few columns (2097152 x 5 bf16: 10.4 us for 46 MB, 4.4 TB/s), by its instructions at many (32768 x 512 bf16: 18
+// us, as long as the issue of its 11.6 million vector instructions takes).
 template <int E, bool ONE, typename X>
 __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_narrow_kernel(HeadArgs a, HeadNarrow g, const int* __restrict__ actions,
                                                                          float* __restrict__ log_prob, float* __restrict__ entropy) {
@@ -884,7 +889,7 @@ __device__ __forceinline__ bool head_lane_picks(double mine, double base, double
   }
 
 // Bound by memory where there is enough of it (1024 x 32003 bf16: 23 us for 131 MB, 5.7 TB/s, part of it in the caches), else by
-// latency (64 x 50001 bf16, all controls, 512 entries of history that every block of a row counts: 8.1 us for 13 MB).
+// latency (64 x 50001 bf16, all controls, 512 entries of history that every block of a row counts: 8.4 us for 13 MB).
 __global__ __launch_bounds__(HEAD_THREADS) void mg_adjust_wide_kernel(HeadArgs a, void* __restrict__ out, const void* __restrict__ dout,
                                                                      void* __restrict__ dlogits) {
   __shared__ unsigned counts[HEAD_CHUNK];
@@ -1030,8 +1035,9 @@ __device__ __forceinline__ void head_sample_again(const HeadArgs& a, const HeadR
                log_prob, entropy);
 }
 
-// An action per row.  Bound by its instructions (16384 x 1024 bf16: 21 us for 34 MB; 4096 x 8192: 37 us for 67 MB; all in 64 bits
-// 39 and 122).
+// An action per row.  Bound by its instructions at 1024 columns (16384 rows bf16: 21 us for 34 MB, 17 of them the issue of 10.6
+// million vector instructions); at 8192 these are 22 of 37 us (4096 rows), the rest is a row's barriers and its choice of a wave,
+// then of a lane.  All in 64 bits: 39 and 122 us.
 template <int CHUNKS, int THREADS, typename X>
 __global__ __launch_bounds__(THREADS) void mg_sample_row_kernel(HeadArgs a, const float* __restrict__ uniforms, int* __restrict__ actions,
                                                                float* __restrict__ log_prob, float* __restrict__ entropy) {
@@ -1075,7 +1081,8 @@ __global__ __launch_bounds__(THREADS) void mg_sample_row_kernel(HeadArgs a, cons
     head_sample_again<CHUNKS, THREADS, X>(a, r, row, h.m, u, counts, red, actions, log_prob, entropy);
 }
 
-// Bound by memory and by the two barriers of a row (4096 x 8192 bf16: 20 us for 67 MB, 3.4 TB/s; 16384 x 1024: 13 us for 34 MB).
+// Bound by its instructions: the issue of 6.8 million vector instructions is 11 of 13 us (16384 x 1024 bf16, 34 MB), of 8.7 million
+// 14 of 19 (4096 x 8192, 67 MB, 3.5 TB/s).
 template <int CHUNKS, int THREADS, typename X>
 __global__ __launch_bounds__(THREADS) void mg_evaluate_row_kernel(HeadArgs a, const int* __restrict__ actions, float* __restrict__ log_prob,
                                                                  float* __restrict__ entropy, double* __restrict__ stats) {
@@ -1152,7 +1159,8 @@ __global__ __launch_bounds__(HEAD_THREADS / 2) void mg_evaluate_row_backward_ker
 
 // found[row][part] = M, Z, sum (M - x) exp(-d) / temperature (against the part's own M), bad, first column of M.  In 32 bits bound
 // by memory (2048 x 32003 bf16, masks: 31 us for 139 MB, 4.4 TB/s), in 64, for sampling, by instructions (1024 x 32003 bf16 with
-// its join 49 us for 66 MB) or, with few rows, latency (16 x 131072 f16, all controls: 8.6 us).
+// its join 49 us for 66 MB; the issue of 24.3 million vector instructions is 40 of the parts' 43) or, with few rows, latency (16 x
+// 131072 f16, all controls: 9.0 us).  The most likely action, which no 64-bit weight decides, takes the same way (50 us).
 template <int CHUNKS, bool FIRST, typename X, typename W>
 __global__ __launch_bounds__(HEAD_THREADS) void mg_head_parts_kernel(HeadArgs a, double* __restrict__ found) {
   constexpr bool ADJUST = std::is_same<X, double>::value;
@@ -1200,7 +1208,7 @@ __device__ __forceinline__ HeadJoined head_join(const double* f, int parts, cons
   return j;
 }
 
-// The part in which the running sum passes the target is looked at once more for the token (16 x 131072 f16, all controls: 6.6 us,
+// The part in which the running sum passes the target is looked at once more for the token (16 x 131072 f16, all controls: 6.8 us,
 // a chain of memory latencies and the count of the history).
 template <typename X>
 __global__ __launch_bounds__(HEAD_THREADS) void mg_sample_join_kernel(HeadArgs a, int parts, const double* __restrict__ found,
@@ -1280,7 +1288,7 @@ __global__ __launch_bounds__(HEAD_THREADS) void mg_sample_join_kernel(HeadArgs a
   if (picks) head_sampled(row, j.bad, j.empty, v0 + pick.e, pick.t, j.z, j.s, scale, actions, log_prob, entropy);
 }
 
-// One wave per row (2048 x 32003: 4.8 us, two memory latencies).
+// One wave per row (2048 x 32003: 4.5 us, two memory latencies).
 __global__ __launch_bounds__(HEAD_THREADS) void mg_evaluate_join_kernel(HeadArgs a, int parts, const double* __restrict__ found,
                                                                        const int* __restrict__ actions, float* __restrict__ log_prob,
                                                                        float* __restrict__ entropy, double* __restrict__ stats) {
@@ -1452,7 +1460,8 @@ static void head_by_width(const mg_logits* a, F f) {
   f(head_int<8>(), several, group);
 }
 // How a block holds a row: chunks of eight columns per thread, and threads.  Rather more chunks than more threads to wait for
-// (evaluation of 4096 x 8192 bf16, before other changes: 33 us with 256 threads, 56 with 1024).
+// (4096 x 8192 bf16: evaluation 19 us and sampling 37 with 256 threads, 27 and 77 with 1024; only where there are few rows is it
+// the other way round, 64 x 8192: 4.6 and 10.5 us, 3.9 and 9.0).
 template <typename F>
 static void head_by_row(const mg_logits* a, F f) {
   if (a->width <= HEAD_CHUNK / 2) f(head_int<1>(), head_int<HEAD_THREADS / 2>());

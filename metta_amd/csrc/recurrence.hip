@@ -224,7 +224,7 @@ __global__ __launch_bounds__(256) void mg_recurrence_step_kernel(RecArgs a, T* _
 }
 
 // The walk back: a stretch's states are made again from its mark, its gradients go out in time's reverse order.  Bound by memory:
-// x, gate and dh in, their gradients out.  8192 x 256 x 128 bf16: 600 us for 2.75 GB, 4.6 TB/s.
+// x, gate and dh in, their gradients out.  8192 x 256 x 128 bf16: 611 us for 2.75 GB, 4.5 TB/s.
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void mg_recurrence_backward_kernel(RecArgs a, RecMarks m, RecGrads d) {
   const RecPlace<VEC> at(a, blockIdx.x * 256 + threadIdx.x);
@@ -396,7 +396,7 @@ __global__ __launch_bounds__(64 * REC_W) void mg_recurrence_pairs_kernel(RecArgs
 }
 
 // Tile after tile: the waves' pairs meet in LDS, then each wave goes on from the state that enters it.  Bound by memory where
-// there are enough blocks (1 x 65536 x 128 f32 in 512 of them: 21 us for 101 MB, 4.7 TB/s), else by the way through a tile
+// there are enough blocks (1 x 65536 x 128 f32 in 512 of them: 22 us for 101 MB, 4.6 TB/s), else by the way through a tile
 // (250 x 129 x 100 f16, two tiles: 14 us for 19 MB).
 template <typename T, int VEC>
 __global__ __launch_bounds__(64 * REC_W) void mg_recurrence_tile_kernel(RecArgs a, T* __restrict__ h, float* __restrict__ last,
@@ -484,7 +484,7 @@ __global__ __launch_bounds__(64 * REC_W) void mg_recurrence_tile_kernel(RecArgs 
   }
 }
 
-// The same from the last tile to the first (1 x 65536 x 128 f32: 37 us for 169 MB, 4.6 TB/s; 250 x 129 x 100 f16: 18 us).
+// The same from the last tile to the first (1 x 65536 x 128 f32: 38 us for 169 MB, 4.5 TB/s; 250 x 129 x 100 f16: 18 us).
 template <typename T, int VEC>
 __global__ __launch_bounds__(64 * REC_W) void mg_recurrence_tile_backward_kernel(RecArgs a, RecMarks m, RecGrads d) {
   __shared__ RecExchange<VEC> ex;
@@ -608,9 +608,10 @@ static RecPlan rec_plan(const mg_recurrence* r) {
   // a walk through time needs five waves per CU (eight with f32's smaller loads) to keep the memory busy: 1500 x 170 x 128
   // bf16 takes 55 us that way and 66 in tiles, 1024 x 256 x 128 53 and 54
   p.shared = waves < (f32 ? 2048 : 1280) && r->steps > REC_L;
-  // time is cut only where there is less than a block per CU, since the pairs are the price of reading the inputs again
-  // (256 x 1024 x 128 bf16: 50 us in one launch, 87 cut in two), into as many blocks as are resident at a time: two per
-  // CU (f32) or one (1 x 65536 x 128 bf16: 30 us, with two 42)
+  // time is cut where there is less than a block per CU, into as many blocks as are resident at a time: two per CU (f32) or
+  // one (1 x 65536 x 128 bf16: 30 us, with two 42).  The pairs are the price, of reading the inputs again: 256 x 1024 x 128
+  // bf16 takes 50 us forward in one launch and 87 cut in two.  Close below 256 waves the rule costs more than it gives in 16
+  // bits (250 x 1024 x 128: 84 us forward and 128 back, 256: 50 and 95), with f32 it does not (83 and 141, 81 and 144).
   if (p.shared && p.tiles >= 4 && waves < 256) {
     const int64_t want = ((f32 ? 512 : 256) + waves - 1) / waves;
     p.splits = (unsigned)(want < p.tiles ? want : p.tiles);
