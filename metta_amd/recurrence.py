@@ -10,6 +10,8 @@ Types: `x` and `gate` float32, bfloat16 or float16 (one type), `state` always fl
 and the running gradient are kept in 32 bits, outputs and gradients are rounded once.  `x` and `gate` may be strided
 views whose last dimension is adjacent (halves of one projection, a time-major tensor transposed); others are copied.
 A padded tail is held by a gate of +infinity: the state passes such a step unchanged (with any finite x).
+NaN goes as far as the formula takes it, up to the next reset.  An infinite state stays one that is not finite, infinity or
+NaN (joined stretches multiply factors first, and a product that underflowed to 0 makes NaN of infinity).
 """
 
 from __future__ import annotations
